@@ -1,0 +1,164 @@
+// Soft-max attention over pages that hold keys and values in 4 bits (kv4.h):
+//   s = scale * q . (step_k u_k + low_k) = scale * (step_k (q . u_k) + low_k sum(q));   p = softmax(s) over the keys that a query sees;
+//   out = sum p (step_v u_v + low_v)
+// A query at position i sees keys max(0, i - window + 1) .. i (window 0: all).  Scores, soft-max and sums are 32-bit.
+// The keys of a query may be cut into ranges, which leave a result of their own each, with the logarithm of its weight, for a second kernel.
+// (reference: model/attention.py:22-43 for what is computed, over pages in the model's precision)
+#include "kv4.h"
+
+struct Kv4AttnParams {
+  void* out;        // [tokens, heads, hd]
+  float* part_o;    // [columns][splits][hd]: a range's result          (splits > 1)
+  float* part_l;    // [columns][splits]: log2 of its weight, -inf of an empty range
+  const void* q;    // row t at q + t * q_stride, head h at + h * hd
+  const uint8_t* pool;
+  const int *tiles, *token_req, *positions, *block_table;
+  int q_stride, table_stride, n_tiles, heads, kv_heads, hd, page, splits, window;
+  float scale_log2;  // softmax scale * log2(e)
+};
+
+// ------------------------------------------------------------------------------------------------------------------------------------
+// Any head size that is a multiple of 32: a workgroup a (token, head, range of keys); its four waves take blocks of 64 keys in turn, a lane
+// a key for the scores, then a lane a channel (and up to four) for the values.  All arithmetic is plain 32-bit.
+template <typename T, int CH>  // CH: channels of a lane, hd <= 64 CH
+__global__ __launch_bounds__(256) void attn_kv4_plain_kernel(const Kv4AttnParams a) {
+  __shared__ float qs[KV4_MAX_HD];
+  __shared__ float sums[4][3];
+  __shared__ float outs[4][KV4_MAX_HD];
+  const int lane = threadIdx.x % NS_WAVE, wave = threadIdx.x / NS_WAVE;
+  const int t = blockIdx.x / a.heads, head = blockIdx.x % a.heads, split = blockIdx.y;
+  const int kvh = head / (a.heads / a.kv_heads), hd = a.hd, groups = hd / 32, octets = a.page / KV4_TOKENS, record = kv4_record(hd);
+  const int pos = a.positions[t], first = a.window ? max(0, pos - a.window + 1) : 0;
+  const int* table = a.block_table + (size_t)a.token_req[t] * a.table_stride;
+  const T* q = (const T*)a.q + (size_t)t * a.q_stride + head * hd;
+  float qsum = 0.f;
+  for (int c = threadIdx.x; c < hd; c += blockDim.x) {
+    const int g = c / 32, o = c % 32 / 8;
+    qs[(o * groups + g) * 8 + c % 8] = to_f(q[c]);  // in the order of a key's dwords
+  }
+  __syncthreads();
+  for (int c = 0; c < hd; ++c) qsum += qs[c];
+  // blocks of 64 keys, and this range's share of them
+  const int b0 = first / 64, blocks = pos / 64 + 1 - b0, share = (blocks + a.splits - 1) / a.splits;
+  const int from = b0 + split * share, to = min(b0 + blocks, from + share);
+  float m = -INFINITY, l = 0.f, z = 0.f, acc[CH];
+#pragma unroll
+  for (int c = 0; c < CH; ++c) acc[c] = 0.f;
+  for (int b = from + wave; b < to; b += 4) {
+    const int key = 64 * b + lane;
+    const bool seen = key >= first && key <= pos;
+    const int at = min(max(key, first), pos), oct = at / KV4_TOKENS, j = at % KV4_TOKENS;
+    const uint8_t* rec = a.pool + kv4_at(table[oct / octets], a.kv_heads, kvh, octets, oct % octets) * record;
+    const uint32_t* kw = reinterpret_cast<const uint32_t*>(rec + j * (hd / 2));
+    float dot = 0.f;
+    for (int i = 0; i < hd / 8; ++i) {
+      const uint32_t w = kw[i];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) dot = fmaf(qs[8 * i + e], (float)(w >> (4 * (e / 2) + 16 * (e % 2)) & 15u), dot);
+    }
+    const uint32_t km = reinterpret_cast<const uint32_t*>(rec + kv4_marks_at(hd))[j], vm = reinterpret_cast<const uint32_t*>(rec + kv4_marks_at(hd))[KV4_TOKENS + j];
+    const float s = seen ? (kv4_step(km) * dot + kv4_low(km) * qsum) * a.scale_log2 : -INFINITY;
+    const float top = fmaxf(m, wave_max(s)), base = top == -INFINITY ? 0.f : top, shrink = exp2f(m - base);
+    const float p = exp2f(s - base), ps = seen ? p * kv4_step(vm) : 0.f;
+    l = l * shrink + p;
+    z = z * shrink + (seen ? p * kv4_low(vm) : 0.f);
+    m = top;
+#pragma unroll
+    for (int c = 0; c < CH; ++c) acc[c] *= shrink;
+    for (int o = 0; o < 8; ++o) {  // the block's octets
+      const int k0 = 64 * b + 8 * o;
+      if (k0 > pos || k0 + 7 < first) continue;
+      const int vo = k0 / KV4_TOKENS;
+      const uint8_t* vr = a.pool + kv4_at(table[vo / octets], a.kv_heads, kvh, octets, vo % octets) * record + kv4_values_at(hd);
+#pragma unroll
+      for (int c = 0; c < CH; ++c) {
+        const int ch = min(lane + 64 * c, hd - 1);
+        const uint4 w = *reinterpret_cast<const uint4*>(vr + ch / 4 * 16);
+        const uint32_t d[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+        for (int e = 0; e < 8; ++e) acc[c] = fmaf(__shfl(ps, 8 * o + e, NS_WAVE), (float)(d[e / 2] >> (16 * (e % 2) + 4 * (ch % 4)) & 15u), acc[c]);
+      }
+    }
+  }
+  l = wave_sum(l);
+  z = wave_sum(z);
+  if (lane == 0) sums[wave][0] = m, sums[wave][1] = l, sums[wave][2] = z;
+#pragma unroll
+  for (int c = 0; c < CH; ++c)
+    if (lane + 64 * c < hd) outs[wave][lane + 64 * c] = acc[c];
+  __syncthreads();
+  float top = -INFINITY;
+  for (int w = 0; w < 4; ++w) top = fmaxf(top, sums[w][0]);
+  const float base = top == -INFINITY ? 0.f : top;
+  float total = 0.f, low = 0.f, weight[4];
+  bool bad = false;  // (a maximum that is no number is lost in fmaxf; its sum is not)
+  for (int w = 0; w < 4; ++w) {
+    weight[w] = exp2f(sums[w][0] - base);
+    total += sums[w][1] * weight[w];
+    low += sums[w][2] * weight[w];
+    bad |= !(sums[w][0] < INFINITY);
+  }
+  for (int c = threadIdx.x; c < hd; c += blockDim.x) {
+    float o = low;
+    for (int w = 0; w < 4; ++w) o += outs[w][c] * weight[w];
+    o = bad ? NAN : total > 0.f ? o / total : total == 0.f ? 0.f : NAN;
+    if (a.splits == 1)
+      ((T*)a.out)[((size_t)t * a.heads + head) * hd + c] = from_f<T>(o);
+    else
+      a.part_o[((size_t)blockIdx.x * a.splits + split) * hd + c] = o;
+  }
+  if (a.splits > 1 && threadIdx.x == 0) a.part_l[(size_t)blockIdx.x * a.splits + split] = bad ? NAN : top + log2f(total);
+}
+
+// Joining the ranges of a column: out = sum_s o_s 2^(l_s - max l) / sum_s 2^(l_s - max l).  One wave a column; a range whose weight is no number makes it so.
+// ``tile_tokens`` 0: columns are (token, head); otherwise (tile, token of the tile, head), and of a tile with fewer tokens nothing is written.
+template <typename T>
+__global__ __launch_bounds__(64) void attn_kv4_join_kernel(const Kv4AttnParams a, int tile_tokens) {
+  const size_t col = blockIdx.x;
+  const int lane = threadIdx.x, head = col % a.heads;
+  size_t row = col / a.heads;
+  if (tile_tokens) {
+    const int* info = a.tiles + row / tile_tokens * 8;
+    const int token = info[1] + (int)(row % tile_tokens);
+    if (token >= info[3]) return;
+    row = info[2] + token;
+  }
+  const float ls = lane < a.splits ? a.part_l[col * a.splits + lane] : -INFINITY;
+  const float top = wave_max(ls), base = top == -INFINITY ? 0.f : top;
+  const float weight = exp2f(ls - base), total = wave_sum(weight);
+  for (int c = lane; c < a.hd; c += NS_WAVE) {
+    float o = 0.f;
+    for (int s = 0; s < a.splits; ++s) o += a.part_o[(col * a.splits + s) * a.hd + c] * __shfl(weight, s, NS_WAVE);
+    ((T*)a.out)[(row * a.heads + head) * a.hd + c] = from_f<T>(o / total);
+  }
+}
+
+template <typename T>
+static void launch_plain(const Kv4AttnParams& a, int tokens, hipStream_t stream) {
+  const dim3 grid((unsigned)(tokens * a.heads), (unsigned)a.splits);
+  switch ((a.hd + 63) / 64) {
+    case 1: attn_kv4_plain_kernel<T, 1><<<grid, 256, 0, stream>>>(a); break;
+    case 2: attn_kv4_plain_kernel<T, 2><<<grid, 256, 0, stream>>>(a); break;
+    case 3: attn_kv4_plain_kernel<T, 3><<<grid, 256, 0, stream>>>(a); break;
+    default: attn_kv4_plain_kernel<T, 4><<<grid, 256, 0, stream>>>(a);
+  }
+  if (a.splits > 1) attn_kv4_join_kernel<T><<<(unsigned)(tokens * a.heads), 64, 0, stream>>>(a, 0);
+}
+
+extern "C" int ns_attn_kv4_plain(void* out, void* part_o, void* part_l, const void* q, int q_stride, const void* pool, const int* token_req, const int* positions,
+                                 const int* block_table, int table_stride, int tokens, int heads, int kv_heads, int hd, int page, int splits, int window, float scale,
+                                 int dtype, hipStream_t stream) {
+  if (tokens < 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads || hd < 32 || hd > KV4_MAX_HD || hd % 32 || page < KV4_TOKENS || (page & (page - 1)) || window < 0)
+    return NS_ERR_BAD_ARG;
+  if (splits < 1 || splits > 64 || (splits > 1 && (!part_o || !part_l)) || (long long)tokens * heads > 0x7fffffff) return NS_ERR_BAD_ARG;
+  if (tokens == 0) return NS_OK;
+  const Kv4AttnParams a{out, (float*)part_o, (float*)part_l, q, (const uint8_t*)pool, nullptr, token_req, positions, block_table, q_stride, table_stride, 0, heads, kv_heads,
+                        hd, page, splits, window, scale * 1.4426950408889634f};
+  if (dtype == NS_DTYPE_F32)
+    launch_plain<float>(a, tokens, stream);
+  else if (dtype == NS_DTYPE_BF16)
+    launch_plain<bf16_t>(a, tokens, stream);
+  else
+    return NS_ERR_UNSUPPORTED;
+  return ns_launch_status();
+}

@@ -1124,6 +1124,170 @@ def attention_prompt_form(head_dim: int, page_size: int) -> int:
     return int(build.attn(head_dim, page_size).ns_attn_prompt_form())
 
 
+# ------------------------------------------------------------------------------------------------ keys and values in 4 bits
+
+KV4_TOKENS = 8  # tokens that lie together in a record of a 4-bit page (csrc/kv4.h says how); a page is a power of two of tokens, from 8
+KV4_MAX_HEAD = 256
+
+
+def kv4_takes(head_dim: int, page_size: int) -> bool:
+    """The head and page sizes that pages of 4 bits are built for."""
+    return head_dim % 32 == 0 and 32 <= head_dim <= KV4_MAX_HEAD and page_size >= KV4_TOKENS and page_size & (page_size - 1) == 0
+
+
+class Kv4Pages:
+    """Pages of keys and values held in 4 bits.  The channels of a head's key (or value) of one token share a step and a lowest value,
+    both bfloat16, rounded outwards: a code u of 0 to 15 stands for step * u + low.  ``pool`` is uint8 [pages, kv_heads, page / 8, record]: the records
+    of eight tokens of a head, 8 head_dim + 64 bytes (4.5 bits a value at head size 128, 5 at 64).  Pages of zeros stand for zeros."""
+
+    def __init__(self, pool: torch.Tensor, head_dim: int) -> None:
+        record = 8 * head_dim + 64
+        if pool.dtype != torch.uint8 or pool.dim() != 4 or not pool.is_contiguous() or pool.shape[3] != record:
+            raise KernelRefused(f"4-bit pages of head size {head_dim} are a contiguous uint8 tensor [pages, kv_heads, page / {KV4_TOKENS}, {record}]")
+        if not kv4_takes(head_dim, pool.shape[2] * KV4_TOKENS):
+            raise KernelRefused(f"4-bit pages take head sizes that are multiples of 32 up to {KV4_MAX_HEAD} and pages of a power of two of tokens from {KV4_TOKENS}; got head "
+                                f"size {head_dim}, page {pool.shape[2] * KV4_TOKENS}")
+        if pool.data_ptr() % 16:
+            raise KernelRefused("4-bit pages begin at a multiple of 16 bytes")
+        self.pool, self.head_dim = pool, head_dim
+        self.pages, self.kv_heads, self.page = pool.shape[0], pool.shape[1], pool.shape[2] * KV4_TOKENS
+
+    @staticmethod
+    def shape(pages: int, kv_heads: int, page: int, head_dim: int) -> tuple[int, int, int, int]:
+        if not kv4_takes(head_dim, page):
+            raise KernelRefused(f"4-bit pages take head sizes that are multiples of 32 up to {KV4_MAX_HEAD} and pages of a power of two of tokens from {KV4_TOKENS}; got head size "
+                                f"{head_dim}, page {page}")
+        return pages, kv_heads, page // KV4_TOKENS, 8 * head_dim + 64
+
+    @classmethod
+    def empty(cls, pages: int, kv_heads: int, page: int, head_dim: int, device) -> "Kv4Pages":
+        return cls(torch.zeros(cls.shape(pages, kv_heads, page, head_dim), dtype=torch.uint8, device=device), head_dim)
+
+    @classmethod
+    def from_codes(cls, k_codes, k_step, k_low, v_codes, v_step, v_low) -> "Kv4Pages":
+        """Codes uint8 [pages, kv_heads, page, head_dim] of 0 to 15, steps and lowest values bfloat16 [pages, kv_heads, page]: pages that were made elsewhere."""
+        pages, kv_heads, page, hd = k_codes.shape
+        out = cls.empty(pages, kv_heads, page, hd, k_codes.device)
+        for codes, step, low in ((k_codes, k_step, k_low), (v_codes, v_step, v_low)):
+            if codes.shape != k_codes.shape or codes.dtype != torch.uint8 or any(t.shape != (pages, kv_heads, page) or t.dtype != torch.bfloat16 for t in (step, low)):
+                raise KernelRefused("Kv4Pages.from_codes takes uint8 codes [pages, kv_heads, page, head_dim] and bfloat16 steps and lows [pages, kv_heads, page]")
+        k, v, marks = out._fields()
+        # a key's channel 32 g + 8 t + c: byte 4 (t hd / 32 + g) + c / 2 % 4 / 2 + 2 (c % 2) of its row, the upper half of the byte for c / 2 odd
+        c = k_codes.view(pages, kv_heads, page // 8, 8, hd // 32, 4, 2, 2, 2).permute(0, 1, 2, 3, 5, 4, 8, 6, 7)  # .. token, t, g, c % 2, c / 4, c / 2 % 2
+        k.copy_((c[..., 0] | c[..., 1] << 4).reshape(k.shape))
+        # a value's channels 4 m + i: 16 bits per token at 16 m
+        c = v_codes.view(pages, kv_heads, page // 8, 8, hd // 4, 2, 2).permute(0, 1, 2, 4, 3, 5, 6)  # .. m, token, i / 2, i % 2
+        v.copy_((c[..., 0] | c[..., 1] << 4).reshape(v.shape))
+        for i, (step, low) in enumerate(((k_step, k_low), (v_step, v_low))):
+            for half, t in enumerate((low, step)):
+                marks[:, :, :, i, :, half].copy_(t.reshape(pages, kv_heads, page // 8, 8))
+        return out
+
+    def _fields(self):
+        """Views: keys [pages, kv_heads, octets, 4 head_dim], values likewise, marks bfloat16 [pages, kv_heads, octets, 2, 8, 2] (keys, values; token; low, step)."""
+        n = 4 * self.head_dim
+        return self.pool[..., :n], self.pool[..., n : 2 * n], self.pool[..., 2 * n :].view(torch.bfloat16).unflatten(3, (2, 8, 2))
+
+    def codes(self):
+        """-> what ``from_codes`` takes, of all pages."""
+        k, v, marks = self._fields()
+        pages, kv_heads, page, hd = self.pages, self.kv_heads, self.page, self.head_dim
+        parts = lambda t: torch.stack((t & 15, t >> 4), -1)
+        kc = parts(k.reshape(pages, kv_heads, page // 8, 8, 4, hd // 32, 2, 2)).permute(0, 1, 2, 3, 5, 4, 7, 8, 6).reshape(pages, kv_heads, page, hd)
+        vc = parts(v.reshape(pages, kv_heads, page // 8, hd // 4, 8, 2)).permute(0, 1, 2, 4, 3, 5, 6).reshape(pages, kv_heads, page, hd)
+        mark = lambda i, half: marks[:, :, :, i, :, half].reshape(pages, kv_heads, page)
+        return kc, mark(0, 1), mark(0, 0), vc, mark(1, 1), mark(1, 0)
+
+
+def _check_kv4(pages: Kv4Pages, positions, token_req, block_table, kv_heads: int, head_dim: int, what: str) -> int:
+    """What the kernels over 4-bit pages assume of a step's tokens (as for ``_check_pages``, positions and requests are the batch builder's).  -> tokens"""
+    if not isinstance(pages, Kv4Pages):
+        raise KernelRefused(f"{what} takes 4-bit pages (Kv4Pages)")
+    _gpu(pages.pool, positions, token_req, block_table)
+    if pages.kv_heads != kv_heads or pages.head_dim != head_dim:
+        raise KernelRefused(f"{what}: pages of {pages.kv_heads} heads of {pages.head_dim}, asked for {kv_heads} of {head_dim}")
+    _i32(positions, "positions"), _i32(token_req, "token_req")
+    if token_req.numel() != positions.numel():
+        raise KernelRefused(f"{what}: token_req is per token")
+    _kv4_table(block_table, what)
+    return positions.numel()
+
+
+def _kv4_table(block_table, what: str) -> None:
+    if block_table.dtype != torch.int32 or block_table.dim() != 2 or (block_table.numel() and block_table.stride(1) != 1):
+        raise KernelRefused(f"{what}: block_table is int32 [requests, pages] with unit stride along a row")
+
+
+def rope_kv4_write(qkv: torch.Tensor, positions: torch.Tensor, token_req: torch.Tensor, block_table: torch.Tensor, inv_freq: torch.Tensor, pages: Kv4Pages, heads: int,
+                   kv_heads: int, head_dim: int, rotary_dim: int, write_kv: bool = True, interleaved: bool = False, factor: float = 1.0,
+                   q_out: torch.Tensor | None = None) -> None:
+    """``rope_kv_write`` for pages of 4 bits: q rotated inside ``qkv`` [N, (heads + 2 kv_heads) * head_dim], or into ``q_out`` [N, heads * head_dim], which leaves ``qkv`` as it is;
+    k rotated, and k and v of every head quantised in 32-bit (``Kv4Pages``) and written into the pages ``block_table[token_req[t], position // page]``.  A key or value that holds
+    an infinity or no number, or reaches further than 2^100, is kept as no number: whoever sees it gets no number.  Two tokens at one place leave either."""
+    n = _check_kv4(pages, positions, token_req, block_table, kv_heads, head_dim, "rope_kv4_write")
+    _gpu(qkv, inv_freq, q_out)
+    width = (heads + 2 * kv_heads) * head_dim
+    if qkv.dim() != 2 or qkv.shape != (n, width) or (n and qkv.stride(1) != 1):
+        raise KernelRefused(f"rope_kv4_write: qkv must be [{n}, {width}]")
+    if q_out is not None and (q_out.shape != (n, heads * head_dim) or q_out.dtype != qkv.dtype or (n and q_out.stride(1) != 1)):
+        raise KernelRefused(f"rope_kv4_write: q_out must be [{n}, {heads * head_dim}] of qkv's dtype")
+    if rotary_dim % 2 or not 0 <= rotary_dim <= head_dim or inv_freq.dtype != torch.float32 or not inv_freq.is_contiguous() or inv_freq.numel() < rotary_dim // 2:
+        raise KernelRefused("rope_kv4_write: the rotary part is an even number of a head's channels, inv_freq holds rotary_dim/2 float32 values")
+    to = qkv if q_out is None else q_out
+    _check(build.core().ns_rope_kv4_write(_ptr(qkv), c_int(qkv.stride(0)), _ptr(to), c_int(to.stride(0)), _ptr(positions), _ptr(token_req), _ptr(block_table),
+                                          c_int(block_table.stride(0)), _ptr(inv_freq), _ptr(pages.pool), c_int(n), c_int(heads), c_int(kv_heads), c_int(head_dim),
+                                          c_int(rotary_dim), c_int(1 if interleaved else 0), c_float(factor), c_int(pages.page), c_int(1 if write_kv else 0),
+                                          c_int(_dtype_code(qkv)), _stream()), "rope_kv4_write")
+
+
+def kv4_read(pages: Kv4Pages, positions: torch.Tensor, token_req: torch.Tensor, block_table: torch.Tensor, dtype: torch.dtype = torch.bfloat16):
+    """-> (keys, values) [N, kv_heads, head_dim] of the tokens at ``positions`` of requests ``token_req`` as the pages hold them (keys rotated), rounded once to ``dtype``."""
+    n = _check_kv4(pages, positions, token_req, block_table, pages.kv_heads, pages.head_dim, "kv4_read")
+    k, v = (torch.empty((n, pages.kv_heads, pages.head_dim), dtype=dtype, device=pages.pool.device) for _ in range(2))
+    _check(build.core().ns_kv4_read(_ptr(k), _ptr(v), _ptr(pages.pool), _ptr(positions), _ptr(token_req), _ptr(block_table), c_int(block_table.stride(0)), c_int(n),
+                                    c_int(pages.kv_heads), c_int(pages.head_dim), c_int(pages.page), c_int(_dtype_code(k)), _stream()), "kv4_read")
+    return k, v
+
+
+def _check_kv4_attn(q, out, pages: Kv4Pages, heads: int, kv_heads: int, head_dim: int, window: int, splits: int, workspace, cols: int, what: str):
+    _gpu(q, out)
+    n = q.shape[0]
+    if heads < 1 or kv_heads < 1 or heads % kv_heads:
+        raise KernelRefused(f"{what}: {heads} heads are not a multiple of {kv_heads} key/value heads")
+    if pages.kv_heads != kv_heads or pages.head_dim != head_dim:
+        raise KernelRefused(f"{what}: pages of {pages.kv_heads} heads of {pages.head_dim}, asked for {kv_heads} of {head_dim}")
+    if q.dim() != 2 or q.shape[1] < heads * head_dim or (n and q.stride(1) != 1):
+        raise KernelRefused(f"{what}: q must be [tokens, at least {heads * head_dim}]")
+    if out.shape != (n, heads * head_dim) or out.dtype != q.dtype or not out.is_contiguous():
+        raise KernelRefused(f"{what}: out must be contiguous [{n}, {heads * head_dim}] of q's dtype")
+    if window < 0 or not 1 <= splits <= 64:
+        raise KernelRefused(f"{what}: a window is not negative, ranges of keys are 1 to 64")
+    if splits == 1:
+        return None, None
+    if workspace is None:
+        raise KernelRefused(f"{what}: ranges of keys need a workspace")
+    po, pl = workspace
+    _gpu(po, pl)
+    if po.dtype != torch.float32 or pl.dtype != torch.float32 or not po.is_contiguous() or not pl.is_contiguous() or po.numel() < cols * splits * head_dim or pl.numel() < cols * splits:
+        raise KernelRefused(f"{what}: workspace too small")
+    return po, pl
+
+
+def attention_kv4_plain(q, out, pages: Kv4Pages, token_req, positions, block_table, heads: int, kv_heads: int, head_dim: int, scale: float, window: int = 0, splits: int = 1,
+                        workspace: tuple[torch.Tensor, torch.Tensor] | None = None) -> torch.Tensor:
+    """Attention of every token over its request's 4-bit pages, in plain 32-bit arithmetic: bfloat16 and float32, any head size that such pages take.  ``q`` [tokens, >= heads *
+    head_dim] (q inside the stacked projection), ``out`` [tokens, heads * head_dim].  ``splits`` > 1 cuts every token's keys into that many ranges and needs ``workspace`` = float32
+    tensors of tokens * heads * splits * head_dim and tokens * heads * splits values."""
+    n = _check_kv4(pages, positions, token_req, block_table, kv_heads, head_dim, "attention_kv4_plain")
+    if n != q.shape[0]:
+        raise KernelRefused("attention_kv4_plain: positions and token_req are per row of q")
+    po, pl = _check_kv4_attn(q, out, pages, heads, kv_heads, head_dim, window, splits, workspace, n * heads, "attention_kv4_plain")
+    _check(build.core().ns_attn_kv4_plain(_ptr(out), _ptr(po), _ptr(pl), _ptr(q), c_int(q.stride(0)), _ptr(pages.pool), _ptr(token_req), _ptr(positions), _ptr(block_table),
+                                          c_int(block_table.stride(0)), c_int(n), c_int(heads), c_int(kv_heads), c_int(head_dim), c_int(pages.page), c_int(splits), c_int(window),
+                                          c_float(scale), c_int(_dtype_code(q)), _stream()), "attention_kv4_plain")
+    return out
+
+
 # ------------------------------------------------------------------------------------------------ 32-bit streams
 
 MAX_STREAMS = 16

@@ -27,6 +27,8 @@ PORTION_SINGLE_SET_BLOCKS = 128  # 32-key blocks of the longest row from which a
 DECODE_WAVES_PER_UNIT = 4  # decode rows' keys are cut into ranges until about this many waves per compute unit are at work
 LONG_ROW_KEYS = 8192  # rows that may reach this many keys get up to 32 ranges instead of 16
 F32_RANGE_KEYS = 128  # keys of a range of a single token's row in 32-bit: two tiles of 16 for each wave of its workgroup
+KV4_MAX_RANGES = 64  # of a row's keys in 4 bits, and the fewest keys of one
+KV4_RANGE_KEYS = 256
 QKV_JOIN_MAX_RANGES = 4  # 17 to 128 rows: the kernel that joins the ranges of the q/k/v product, rotates and writes the cache reads
 #                          every range, so more of them cost it what they gain the product
 
@@ -221,6 +223,16 @@ def f32_attention(ctx, q, out, cache, table, heads: int, kv_heads: int, head_dim
         longest, edge = (ctx.max_kv_len, 0) if ctx.max_kv_len <= span else (span, 1)
         launch(decode_tiles, True, min(ops.F32_ATTENTION_MAX_RANGES, -(-longest // F32_RANGE_KEYS) + edge), range_keys=F32_RANGE_KEYS)
     return out
+
+
+def kv4_attention(ctx, q, out, pages, table, heads: int, kv_heads: int, head_dim: int, scale: float, window: int = 0) -> torch.Tensor:
+    """Attention of the batch's tokens over pages of 4 bits (``ops.Kv4Pages``)."""
+    n, take = q.shape[0], ctx.arena.take
+    longest = min(ctx.max_kv_len, window) if window else ctx.max_kv_len
+    # a workgroup a token, head and range of keys, until there are four for each compute unit
+    splits = max(1, min(KV4_MAX_RANGES, 4 * ops.compute_units(q.device) // max(1, n * heads), -(-longest // KV4_RANGE_KEYS)))
+    ws = (take((n * heads * splits * head_dim,), torch.float32), take((n * heads * splits,), torch.float32)) if splits > 1 else None
+    return ops.attention_kv4_plain(q, out, pages, ctx.token_req, ctx.positions, table, heads, kv_heads, head_dim, scale, window=window, splits=splits, workspace=ws)
 
 
 class Attention:

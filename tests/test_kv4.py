@@ -1,0 +1,104 @@
+"""4-bit pages on the CPU: the layout's way there and back, and what is refused."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+from nanospec_amd.kernels import ops
+
+
+def _codes(pages, kv_heads, page, hd, seed=0):
+    gen = torch.Generator().manual_seed(seed)
+    codes = lambda: torch.randint(0, 16, (pages, kv_heads, page, hd), dtype=torch.uint8, generator=gen)
+    marks = lambda: torch.randn((pages, kv_heads, page), generator=gen).bfloat16()
+    return codes(), marks(), marks(), codes(), marks(), marks()
+
+
+@pytest.mark.parametrize("hd", [32, 64, 96, 128, 160, 256])
+@pytest.mark.parametrize("page", [8, 32])
+def test_codes_there_and_back(hd, page):
+    made = _codes(3, 2, page, hd)
+    pages = ops.Kv4Pages.from_codes(*made)
+    assert pages.page == page and pages.kv_heads == 2 and pages.pool.shape == (3, 2, page // 8, 8 * hd + 64)
+    assert all(torch.equal(a, b) for a, b in zip(made, pages.codes()))
+
+
+def test_places_of_codes_and_marks():
+    """The bytes that csrc/kv4.h names."""
+    hd, page = 96, 16
+    k, ks, kl, v, vs, vl = _codes(2, 2, page, hd)
+    pool = ops.Kv4Pages.from_codes(k, ks, kl, v, vs, vl).pool
+    for at in ((0, 0, 0, 0), (1, 1, 11, 5), (1, 0, 15, 95), (0, 1, 8, 33), (1, 1, 3, 62)):
+        p, h, tok, ch = at
+        record, j = pool[p, h, tok // 8], tok % 8
+        t, g, c = ch % 32 // 8, ch // 32, ch % 8
+        words = record.view(torch.int32)
+        word = int(words[j * (hd // 8) + t * (hd // 32) + g])
+        assert word >> (4 * (c // 2) + 16 * (c % 2)) & 15 == int(k[at])
+        assert int(record.view(torch.int16)[(4 * hd + 16 * (ch // 4)) // 2 + j]) >> 4 * (ch % 4) & 15 == int(v[at])
+        marks = record[8 * hd :].view(torch.bfloat16)
+        assert marks[2 * j] == kl[p, h, tok] and marks[2 * j + 1] == ks[p, h, tok]
+        assert marks[16 + 2 * j] == vl[p, h, tok] and marks[16 + 2 * j + 1] == vs[p, h, tok]
+
+
+@pytest.mark.parametrize("hd,page", [(16, 16), (80, 16), (288, 16), (64, 4), (64, 24), (0, 16)])
+def test_sizes_that_are_refused(hd, page):
+    assert not ops.kv4_takes(hd, page)
+    with pytest.raises(ops.KernelRefused):
+        ops.Kv4Pages.empty(2, 1, page, hd, "cpu")
+
+
+def test_pools_and_codes_that_are_refused():
+    good = torch.zeros((2, 1, 2, 8 * 64 + 64), dtype=torch.uint8)
+    ops.Kv4Pages(good, 64)
+    for pool, hd in ((good, 32), (good.int(), 64), (good[0], 64), (good.transpose(0, 2), 64), (torch.zeros((2, 1, 3, 576), dtype=torch.uint8), 64),
+                     (torch.zeros(2 * 2 * 576 + 8, dtype=torch.uint8)[8:].view(2, 1, 2, 576), 64)):
+        with pytest.raises(ops.KernelRefused):
+            ops.Kv4Pages(pool, hd)
+    made = list(_codes(2, 1, 8, 32))
+    for i, bad in ((0, made[0].int()), (1, made[1].float()), (4, made[4][:, :, :4]), (3, made[3][..., :16])):
+        with pytest.raises(ops.KernelRefused):
+            ops.Kv4Pages.from_codes(*made[:i], bad, *made[i + 1 :])
+
+
+def _call(monkeypatch, **change):
+    """Arguments that ``rope_kv4_write`` takes but for where they live, with some changed."""
+    monkeypatch.setattr(ops, "_gpu", lambda *tensors: None)  # (the checks of shapes and types are the host's)
+    n, heads, kv, hd = 3, 4, 2, 32
+    args = dict(qkv=torch.zeros(n, (heads + 2 * kv) * hd), positions=torch.zeros(n, dtype=torch.int32), token_req=torch.zeros(n, dtype=torch.int32),
+                block_table=torch.zeros((1, 2), dtype=torch.int32), inv_freq=torch.ones(hd // 2), pages=ops.Kv4Pages.empty(2, kv, 8, hd, "cpu"), heads=heads,
+                kv_heads=kv, head_dim=hd, rotary_dim=hd)
+    args.update(change)
+    return args
+
+
+@pytest.mark.parametrize("change", [
+    dict(qkv=torch.zeros(3, 200)), dict(qkv=torch.zeros(2, 256)), dict(qkv=torch.zeros(256, 3).t()), dict(qkv=torch.zeros(3, 256, dtype=torch.float16)),
+    dict(positions=torch.zeros(3, dtype=torch.int64)), dict(positions=torch.zeros(6, dtype=torch.int32)[::2]), dict(token_req=torch.zeros(2, dtype=torch.int32)),
+    dict(block_table=torch.zeros((1, 2))), dict(block_table=torch.zeros(2, dtype=torch.int32)), dict(block_table=torch.zeros((2, 3), dtype=torch.int32).t()),
+    dict(inv_freq=torch.ones(15)), dict(inv_freq=torch.ones(16).double()), dict(rotary_dim=31), dict(rotary_dim=34), dict(kv_heads=1), dict(head_dim=64),
+    dict(pages=torch.zeros(2, 2, 1, 320, dtype=torch.uint8)), dict(q_out=torch.zeros(3, 64)), dict(q_out=torch.zeros(3, 128).bfloat16())])
+def test_write_refuses(monkeypatch, change):
+    with pytest.raises(ops.KernelRefused):
+        ops.rope_kv4_write(**_call(monkeypatch, **change))
+
+
+@pytest.mark.parametrize("change", [
+    dict(heads=3), dict(kv_heads=4), dict(head_dim=64), dict(q=torch.zeros(3, 100)), dict(q=torch.zeros(128, 3).t()), dict(out=torch.zeros(3, 64)),
+    dict(out=torch.zeros(3, 128).bfloat16()), dict(out=torch.zeros(3, 200)[:, :128]), dict(window=-1), dict(splits=0), dict(splits=65), dict(splits=2),
+    dict(splits=2, workspace=(torch.zeros(8), torch.zeros(24))), dict(splits=2, workspace=(torch.zeros(768), torch.zeros(23))), dict(token_req=torch.zeros(4, dtype=torch.int32)),
+    dict(positions=torch.zeros(2, dtype=torch.int32), token_req=torch.zeros(2, dtype=torch.int32)),
+    dict(q=torch.zeros(3, 128, dtype=torch.float16), out=torch.zeros(3, 128, dtype=torch.float16))])
+def test_attention_refuses(monkeypatch, change):
+    monkeypatch.setattr(ops, "_gpu", lambda *tensors: None)
+    args = dict(q=torch.zeros(3, 128), out=torch.zeros(3, 128), pages=ops.Kv4Pages.empty(2, 2, 8, 32, "cpu"), token_req=torch.zeros(3, dtype=torch.int32),
+                positions=torch.zeros(3, dtype=torch.int32), block_table=torch.zeros((1, 2), dtype=torch.int32), heads=4, kv_heads=2, head_dim=32, scale=1.0)
+    args.update(change)
+    with pytest.raises(ops.KernelRefused):
+        ops.attention_kv4_plain(**args)
+
+
+def test_tensors_on_the_cpu_are_refused():
+    with pytest.raises(ops.KernelRefused, match="GPU"):
+        ops.kv4_read(ops.Kv4Pages.empty(1, 1, 8, 32, "cpu"), torch.zeros(1, dtype=torch.int32), torch.zeros(1, dtype=torch.int32), torch.zeros((1, 1), dtype=torch.int32))

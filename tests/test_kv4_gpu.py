@@ -1,0 +1,233 @@
+"""Keys and values in 4 bits: the write into the pages, the read back, and attention over them, against their definition in 64 bits."""
+
+from __future__ import annotations
+
+import math
+
+import pytest
+import torch
+
+import kv4_oracle as oracle
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+ROUND = {torch.bfloat16: 2.0**-8, torch.float32: 2.0**-24}  # a rounding is off by at most half a step, eps / 2 relative to the value
+
+
+def _ops():
+    from nanospec_amd.kernels import ops
+
+    return ops
+
+
+def _rand(shape, seed, dtype=torch.float32):
+    return torch.randn(shape, generator=torch.Generator().manual_seed(seed)).to(dtype)
+
+
+# ------------------------------------------------------------------------------------------------ the write
+
+
+def _written(lens, starts, heads, kv_heads, hd, rot, page, dtype, seed, interleaved=False, factor=1.0, q_out="in place", qkv=None, pad=0):
+    ops = _ops()
+    n = sum(lens)
+    width = (heads + 2 * kv_heads) * hd
+    qkv = _rand((n, width), seed, dtype) if qkv is None else qkv
+    tables, pages = oracle.scattered_tables([-(-(a + b) // page) for a, b in zip(lens, starts)], 2, seed)
+    positions = torch.cat([torch.arange(s, s + m) for m, s in zip(lens, starts)]).int()
+    reqs = torch.repeat_interleave(torch.arange(len(lens)), torch.tensor(lens)).int()
+    inv = (1.0 / 10000.0 ** (torch.arange(0, max(rot, 2), 2, dtype=torch.float32) / max(rot, 2)))[: max(1, rot // 2)]
+    pool = ops.Kv4Pages.empty(pages, kv_heads, page, hd, DEV)
+    room = torch.full((n + 1, width + pad), 5.0, dtype=dtype, device=DEV)
+    dev = room[:n, pad:]  # rows further apart than they are long; with an odd ``pad`` they begin between 16 bytes
+    dev.copy_(qkv)
+    where = (positions.to(DEV), reqs.to(DEV), tables.to(DEV))
+    q = None if q_out == "in place" else torch.empty((n, heads * hd), dtype=dtype, device=DEV)
+    ops.rope_kv4_write(dev, *where, inv.to(DEV), pool, heads, kv_heads, hd, rot, interleaved=interleaved, factor=factor, q_out=q)
+    torch.cuda.synchronize()
+    x = qkv.double().view(n, heads + 2 * kv_heads, hd)
+    turned = oracle.rotated(x[:, : heads + kv_heads], positions, inv[: rot // 2], rot, interleaved, factor)
+    want = (turned[:, :heads], turned[:, heads:], x[:, heads + kv_heads :])
+    if q is None:
+        torch.testing.assert_close(dev[:, heads * hd :].cpu(), qkv[:, heads * hd :], rtol=0, atol=0, equal_nan=True)  # keys and values stay as the product left them
+    else:
+        torch.testing.assert_close(dev.cpu(), qkv, rtol=0, atol=0, equal_nan=True)
+    assert bool((room[n] == 5).all()) and bool((room[:, :pad] == 5).all())
+    got = (dev[:, : heads * hd] if q is None else q).cpu().double().view(n, heads, hd)
+    return pool, where, want, got, tables, positions, reqs
+
+
+CASES = [
+    # lens, starts, heads, kv_heads, hd, rot, page
+    ([1], [0], 1, 1, 32, 32, 8),
+    ([1, 1, 1], [7, 8, 100], 4, 2, 64, 64, 16),
+    ([5, 1, 19], [3, 15, 0], 6, 2, 96, 96, 8),
+    ([33], [60000], 8, 8, 128, 128, 16),
+    ([9, 2], [30, 31], 7, 1, 256, 128, 32),
+    ([17], [1], 5, 5, 160, 20, 64),
+]
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("form", ["in place", "out", "interleaved", "odd rows"])
+@pytest.mark.parametrize("case", range(len(CASES)))
+def test_write_keeps_what_the_definition_says(case, form, dtype):
+    lens, starts, heads, kv_heads, hd, rot, page = CASES[case]
+    pool, where, (wq, wk, wv), got, tables, positions, reqs = _written(lens, starts, heads, kv_heads, hd, rot, page, dtype, case, interleaved=form == "interleaved",
+                                                                      factor=1.25 if form == "interleaved" else 1.0, q_out="out" if form == "out" else "in place",
+                                                                      pad=3 if form == "odd rows" else 8)
+    # cosine and sine to 4 units of 2^-24 each, two products, a sum and the factor: 8 roundings of 2^-24 of the pair's size; then the rounding to the type
+    pair = 2 * 1.25 * float(max(wq.abs().max(), wk.abs().max()))
+    slack = 8 * 2.0**-24 * pair
+    assert bool(((got - wq).abs() <= slack + ROUND[dtype] * (wq.abs() + slack)).all())
+    codes = pool.codes()
+    page_of = tables[reqs.long(), positions.long() // page].long()
+    at = (page_of, slice(None), positions.long() % page)
+    kc, ks, kl, vc, vs, vl = (c.cpu()[at].double() for c in codes)
+    # values are not computed with: equal to the definition, code for code
+    c, s, low = oracle.quantised(wv)
+    assert torch.equal(vs, s[..., 0]) and torch.equal(vl, low[..., 0]) and torch.equal(vc, c)
+    # keys: the marks are those of rotated keys within ``slack``, and every channel lies within half a step of what its code stands for
+    assert bool((kl <= wk.amin(-1) + slack).all()) and bool((kl >= oracle.outward(wk.amin(-1) - slack, up=False)).all())
+    assert bool((kl + 15 * ks >= wk.amax(-1) - 2 * slack).all())
+    assert bool((ks <= oracle.outward((wk.amax(-1) - kl + 2 * slack) / 15 * (1 + 2.0**-22), up=True)).all())
+    stands = ks[..., None] * kc + kl[..., None]
+    assert bool(((stands - wk).abs() <= ks[..., None] * (0.5 + 2.0**-20) + 2 * slack).all())
+    # the other tokens' places are as they were: zeros
+    touched = torch.zeros(pool.pages, page, dtype=torch.bool)
+    touched[page_of, positions.long() % page] = True
+    for t in codes:
+        t = t.cpu().double().transpose(1, 2)
+        assert bool((t[~touched] == 0).all())
+    # read back: the value of the code in 32 bits, rounded once
+    for out in (torch.bfloat16, torch.float32):
+        k, v = _ops().kv4_read(pool, *where, dtype=out)
+        for got_, c_, s_, l_ in ((k, kc, ks, kl), (v, vc, vs, vl)):
+            assert torch.equal(got_.cpu(), (s_.float()[..., None] * c_.float() + l_.float()[..., None]).to(out))
+
+
+def test_write_of_constant_tiny_huge_and_bad_rows():
+    """Rows of one value, of steps below what is kept, of ranges beyond it, with infinities and with no numbers; beside ordinary ones."""
+    heads, kv_heads, hd, page = 1, 1, 64, 8
+    rows = torch.randn(9, 3 * hd, generator=torch.Generator().manual_seed(1))
+    v = rows[:, 2 * hd :]
+    v[0] = 1.5
+    v[1] *= 2.0**-110
+    v[2, 3] = 2.0**101
+    v[3, 63] = math.inf
+    v[4, 0] = -math.inf
+    v[5, 17] = math.nan
+    v[6] = 0.0
+    v[7] = -v[7].abs() - 3
+    rows[:, hd : 2 * hd] = v
+    pool, where, (wq, wk, wv), *_ = _written([9], [0], heads, kv_heads, hd, 0, page, torch.float32, 3, qkv=rows)
+    c, s, low = oracle.quantised(wv)
+    kc, ks, kl, vc, vs, vl = (t.cpu().double() for t in pool.codes())
+    page_of = where[2].cpu()[0, torch.arange(9) // page].long()
+    at = (page_of, 0, torch.arange(9) % page)
+    for codes, steps, lows in ((kc, ks, kl), (vc, vs, vl)):
+        assert torch.equal(codes[at], c[:, 0])
+        assert torch.equal(steps[at], s[:, 0, 0])
+        torch.testing.assert_close(lows[at], low[:, 0, 0], rtol=0, atol=0, equal_nan=True)
+    k, v = _ops().kv4_read(pool, *where, dtype=torch.float32)
+    assert bool(torch.isnan(v[2:6]).all()) and bool(torch.isfinite(v[[0, 1, 6, 7, 8]]).all()) and bool((v[0] == 1.5).all())
+
+
+def test_write_leaves_pages_alone_where_a_layer_only_reads():
+    ops = _ops()
+    qkv = _rand((3, 4 * 64), 0, torch.bfloat16).to(DEV)
+    pool = ops.Kv4Pages.empty(2, 1, 8, 64, DEV)
+    pos, req, table = torch.arange(3, dtype=torch.int32, device=DEV), torch.zeros(3, dtype=torch.int32, device=DEV), torch.zeros((1, 1), dtype=torch.int32, device=DEV)
+    ops.rope_kv4_write(qkv, pos, req, table, torch.ones(32, device=DEV), pool, 2, 1, 64, 64, write_kv=False)
+    assert not bool(pool.pool.any())
+    ops.rope_kv4_write(qkv[:0], pos[:0], req[:0], table, torch.ones(32, device=DEV), pool, 2, 1, 64, 64)  # a step without tokens
+    assert not bool(pool.pool.any()) and ops.kv4_read(pool, pos[:0], req[:0], table)[0].shape == (0, 1, 64)
+
+
+# ------------------------------------------------------------------------------------------------ attention
+
+
+def _pool(pages, kv_heads, page, hd, seed, spread=1.0, held=None):
+    """Pages of quantised random keys and values, with a few large channels among the keys; places that ``held`` (bool [pages, page]) does not name
+    hold no numbers and the largest steps.  -> Kv4Pages, keys, values in 64 bits, the largest step of a value"""
+    gen = torch.Generator().manual_seed(seed)
+    k = torch.randn((pages, kv_heads, page, hd), generator=gen, dtype=torch.float64) * (1 + 4 * (torch.arange(hd) % 23 == 3))
+    v = torch.randn((pages, kv_heads, page, hd), generator=gen, dtype=torch.float64) * torch.exp(spread * torch.randn((pages, kv_heads, page, 1), generator=gen, dtype=torch.float64)) + 0.3
+    made, sides = [], []
+    for x in (k, v):
+        c, s, low = oracle.quantised(x)
+        sides.append(s * c + low)
+        if held is not None:
+            empty = ~held[:, None, :, None].expand_as(s)
+            s, low = torch.where(empty, 2.0**99, s), torch.where(empty, math.nan, low)
+        made += [c.to(torch.uint8).to(DEV), s[..., 0].bfloat16().to(DEV), low[..., 0].bfloat16().to(DEV)]
+    return _ops().Kv4Pages.from_codes(*made), sides[0], sides[1], float(oracle.quantised(v)[1].max())
+
+
+def tolerance(dtype, out, size, hd, keys, v_step, v_most):
+    """How far attention may be off, for |out| and the sizes at hand (``size``: the largest sum of |q| |k| scale of a visible pair).
+    A score is at most 2 hd + 4 roundings of 2^-24 of ``size`` off (plain products and sums in 32 bits); where codes are multiplied with 1,024 on top of them, which is taken off in the
+    first sum, so are 1,024 |q| of the step in the place of at most 15: at most 70 times as much, in hd / 8 + 2 roundings.  float32 takes the codes as they are.
+    The soft-max's weights are off by exp(2 delta) - 1 and the roundings of 2^x (2 units); bfloat16 rounds them to float16 on their way into the second product: 2^-11, and 2^-25 of the
+    largest for those below the normal range, times keys; sums over the keys add 2^-24 each, of all that is summed (values and codes times steps: at most v_most + 8 steps)."""
+    exact = dtype == torch.float32
+    delta = size * 2.0**-24 * ((2 * hd + 4) if exact else max(2 * hd + 4, 70 * (hd / 8 + 2)))
+    weight = math.expm1(2 * delta) + 2.0**-21 + (2.0**-22 if exact else 2.0**-11)
+    # (one part in float16 of a weight below 2^-14 of the largest is off by 2^-25; float32's second part by 2^-36 or less)
+    small = (2.0**-34 if exact else 2.0**-25) * min(keys, 2**14)
+    sums = min(keys, 4096) * 2.0**-24
+    return (v_most + 8 * v_step) * (weight + small + sums) + ROUND[dtype] * out.abs()
+
+
+ATTENTION = {
+    # name: lens, starts
+    "one key": ([1], [0]),
+    "singles": ([1, 1, 1, 1], [0, 30, 31, 257]),
+    "a long single": ([1], [2999]),
+    "portion": ([37], [0]),
+    "portions": ([2, 64, 33], [0, 5, 300]),
+    "mixed": ([1, 65, 1, 3], [63, 130, 500, 8]),
+}
+SHAPES = [(1, 1, 32, 8), (4, 2, 64, 8), (8, 2, 64, 16), (6, 1, 128, 16), (32, 8, 128, 32), (3, 3, 128, 64), (17, 1, 64, 16), (40, 2, 128, 16), (4, 2, 96, 16), (5, 5, 256, 8)]
+
+
+def _attend(case, heads, kv_heads, hd, page, dtype, window=0, seed=0, q_scale=1.0, spread=1.0):
+    from nanospec_amd.parts.attention import kv4_attention
+
+    lens, starts = ATTENTION[case] if isinstance(case, str) else case
+    tables, pages = oracle.scattered_tables([-(-(a + b) // page) for a, b in zip(lens, starts)], 2, seed)
+    held = torch.zeros(pages, page, dtype=torch.bool)
+    for r, (m, b) in enumerate(zip(lens, starts)):
+        for key in range(0, m + b, page):
+            held[int(tables[r, key // page]), : m + b - key] = True
+    pool, keys, values, v_step = _pool(pages, kv_heads, page, hd, seed, spread, held)
+    n = sum(lens)
+    q = (q_scale * _rand((n, heads * hd), seed + 7)).to(dtype)
+    wide = torch.full((n, heads * hd + 16), math.nan, dtype=dtype, device=DEV)  # q inside a wider row
+    wide[:, : heads * hd] = q.to(DEV)
+    if window:  # pages before every query's window have been given back: nobody may read them
+        for r, s in enumerate(starts):
+            tables[r, : max(0, s - window + 1) // page] = -1
+    ctx = oracle.batch_context(lens, starts, tables, DEV)
+    out = torch.full((n, heads * hd), 7.0, dtype=dtype, device=DEV)
+    scale = hd**-0.5
+    kv4_attention(ctx, wide, out, pool, ctx.block_tables[0], heads, kv_heads, hd, scale, window=window)
+    torch.cuda.synchronize()
+    want, size = oracle.attention(q.double().view(n, heads, hd), keys, values, lens, starts, tables, page, heads, kv_heads, scale, window)
+    tol = tolerance(dtype, want, size, hd, max(a + b for a, b in zip(lens, starts)), v_step, float(values.abs().max()))
+    return out.cpu().double().view(n, heads, hd), want, tol, (pool, ctx, wide, scale)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("case", list(ATTENTION))
+@pytest.mark.parametrize("heads,kv_heads,hd,page", SHAPES)
+def test_attention(case, heads, kv_heads, hd, page, dtype):
+    got, want, tol, _ = _attend(case, heads, kv_heads, hd, page, dtype, seed=heads + hd)
+    assert bool(((got - want).abs() <= tol).all()), float(((got - want).abs() / tol).max())
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("window", [1, 7, 64, 129])
+@pytest.mark.parametrize("heads,kv_heads,hd,page", [(8, 2, 64, 8), (4, 1, 128, 16), (2, 2, 96, 8)])
+def test_attention_window(heads, kv_heads, hd, page, window, dtype):
+    got, want, tol, _ = _attend("mixed", heads, kv_heads, hd, page, dtype, window=window, seed=window)
+    assert bool(((got - want).abs() <= tol).all())
