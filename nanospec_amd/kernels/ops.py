@@ -1124,6 +1124,134 @@ def attention_prompt_form(head_dim: int, page_size: int) -> int:
     return int(build.attn(head_dim, page_size).ns_attn_prompt_form())
 
 
+# ------------------------------------------------------------------------------------------------ products in 8-bit integers
+
+INT8_MAX_K = 32768
+INT8_K_MULTIPLE, INT8_K_MIN = 256, 512
+
+
+def int8_padded_k(k: int) -> int:
+    """The inner size that operands in 8 bits are laid out for: what lies beyond ``k`` is multiplied with zeros."""
+    return max(INT8_K_MIN, -(-k // INT8_K_MULTIPLE) * INT8_K_MULTIPLE)
+
+
+class Int8Weight:
+    """A weight matrix [N, K] in 8 bits: codes of -127 to 127 and a float32 scale for each output channel (a row), which stand for scale * code.  The codes are laid out once, in
+    pieces of 1 KiB that are operands of the 8-bit matrix instruction: wt[row tile][k / 64][lane = 16 g + r][16] = w[16 tile + r][64 piece + 16 g + ..], rows padded to a
+    multiple of 16 and k to ``int8_padded_k`` with zeros."""
+
+    def __init__(self, codes: torch.Tensor, scales: torch.Tensor) -> None:
+        if codes.dtype != torch.int8 or codes.dim() != 2 or min(codes.shape) < 1 or codes.shape[1] > INT8_MAX_K:
+            raise KernelRefused(f"Int8Weight takes int8 codes [N, K] with K up to {INT8_MAX_K}; got {codes.dtype} {tuple(codes.shape)}")
+        if scales.dtype != torch.float32 or scales.shape != codes.shape[:1] or scales.device != codes.device:
+            raise KernelRefused("Int8Weight takes a float32 scale for each row of the codes, on their device")
+        self.n, self.k = codes.shape
+        self.kp = int8_padded_k(self.k)
+        n_pad = -(-self.n // 16) * 16
+        if (n_pad, self.kp) != codes.shape:
+            padded = torch.zeros((n_pad, self.kp), dtype=torch.int8, device=codes.device)
+            padded[: self.n, : self.k] = codes
+        else:
+            padded = codes
+        self.data = padded.view(n_pad // 16, 16, self.kp // 64, 4, 16).permute(0, 2, 3, 1, 4).contiguous()
+        self.scales = torch.zeros(n_pad, dtype=torch.float32, device=codes.device)
+        self.scales[: self.n] = scales
+
+    @classmethod
+    def from_float(cls, w: torch.Tensor) -> "Int8Weight":
+        """The nearest: a row's scale is its largest magnitude / 127.  A row with an infinity or no number has the scale "no number"."""
+        if w.dim() != 2 or w.dtype not in (torch.float32, torch.bfloat16):
+            raise KernelRefused("Int8Weight.from_float takes a float32 or bfloat16 matrix")
+        codes = torch.empty(w.shape, dtype=torch.int8, device=w.device)
+        scales = torch.empty(w.shape[0], dtype=torch.float32, device=w.device)
+        rows = max(1, (1 << 28) // max(1, w.shape[1]))  # (portions: a row's values in 32-bit need not all be there at once)
+        for a in range(0, w.shape[0], rows):
+            x = w[a : a + rows].float()
+            most = x.abs().amax(1)
+            fine, some = torch.isfinite(most), torch.isfinite(most) & (most >= 2.0**-100)
+            inverse = torch.where(some, 127.0 / most, torch.zeros_like(most))
+            codes[a : a + rows] = torch.where(some[:, None], torch.round(x * inverse[:, None]).clamp(-127, 127), torch.zeros_like(x)).to(torch.int8)
+            scales[a : a + rows] = torch.where(some, most / 127, torch.where(fine, torch.zeros_like(most), torch.full_like(most, math.nan)))
+        return cls(codes, scales)
+
+    def codes(self) -> torch.Tensor:
+        """-> int8 [N, K]"""
+        n_pad = self.data.shape[0] * 16
+        return self.data.permute(0, 3, 1, 2, 4).reshape(n_pad, self.kp)[: self.n, : self.k]
+
+
+class Int8Rows:
+    """Activations in 8 bits: ``codes`` int8 [rows, ``int8_padded_k``] (what lies beyond ``k`` counts for nothing), ``scales`` float32 [rows], which stand for
+    scale * code.  Made by ``int8_rows``, ``rmsnorm_int8`` and ``silu_mul_int8``, taken by ``linear_int8``."""
+
+    def __init__(self, codes: torch.Tensor, scales: torch.Tensor, k: int) -> None:
+        self.codes, self.scales, self.k = codes, scales, k
+        self.shape = (codes.shape[0], k)
+
+
+def _int8_rows(x: torch.Tensor, k: int, src: int, take, what: str, resid=None, resid_out=None, weight=None, eps: float = 0.0) -> Int8Rows:
+    m, width = x.shape[0], 2 * k if src == 2 else k
+    if not 1 <= k <= INT8_MAX_K or x.shape[1] != width or (m > 1 and x.stride(0) < width) or (m and x.stride(1) != 1):
+        raise KernelRefused(f"{what}: rows of up to {INT8_MAX_K} values with unit stride along a row; got {tuple(x.shape)}")
+    take = take or (lambda shape, dtype: torch.empty(shape, dtype=dtype, device=x.device))
+    rows = Int8Rows(take((m, int8_padded_k(k)), torch.int8), take((m,), torch.float32), k)
+    _check(build.core().ns_int8_rows(_ptr(rows.codes), _ptr(rows.scales), _ptr(x), c_int(max(x.stride(0), width)), _ptr(resid), _ptr(resid_out), _ptr(weight), c_float(eps), c_int(m),
+                                     c_int(k), c_int(rows.codes.shape[1]), c_int(src), c_int(_dtype_code(x)), _stream()), what)
+    return rows
+
+
+def int8_rows(x: torch.Tensor, take=None) -> Int8Rows:
+    """Each row of ``x`` in 8 bits: scale = largest magnitude / 127 (a row of less than 2^-100 is zeros), code = the whole number next to x * (127 / largest magnitude), in 32-bit.  A row that
+    holds an infinity or no number has the scale "no number", and so have its products; other rows do not see it.  ``take`` (shape, dtype) gives the memory (``ctx.arena.take``)."""
+    _gpu(x)
+    if x.dim() != 2:
+        raise KernelRefused("int8_rows takes [rows, K]")
+    return _int8_rows(x, x.shape[1], 0, take, "int8_rows")
+
+
+def rmsnorm_int8(weight: torch.Tensor, eps: float, resid: torch.Tensor | None = None, x: torch.Tensor | None = None, resid_out: torch.Tensor | None = None, take=None) -> Int8Rows:
+    """``rmsnorm`` into 8 bits: weight * r * rsqrt(mean(r^2) + eps) with r = resid + x rounded to their type (or the one that is given), in 32-bit up to the codes.  ``resid_out``
+    (``resid`` itself, or another tensor like it): where r is stored."""
+    src = resid if resid is not None else x
+    if src is None:
+        raise KernelRefused("rmsnorm_int8 needs resid or x")
+    _gpu(weight, resid, x, resid_out)
+    dim = weight.numel()
+    for t in (resid, x, resid_out):
+        if t is not None and (t.dim() != 2 or t.shape[1] != dim or not t.is_contiguous() or t.dtype != weight.dtype or t.shape != src.shape):
+            raise KernelRefused(f"rmsnorm_int8: operands must be contiguous [*, {dim}] of the weight's dtype and one shape")
+    if weight.dim() != 1 or not weight.is_contiguous():
+        raise KernelRefused("rmsnorm_int8: the weight is one contiguous row")
+    first, second = (resid, None) if x is None else (x, resid)
+    return _int8_rows(first, dim, 1, take, "rmsnorm_int8", resid=second, resid_out=resid_out, weight=weight, eps=eps)
+
+
+def silu_mul_int8(gu: torch.Tensor, take=None) -> Int8Rows:
+    """``silu_mul`` into 8 bits: silu(gu[:, :I]) * gu[:, I:] for gu [rows, 2 I], in 32-bit up to the codes."""
+    _gpu(gu)
+    if gu.dim() != 2 or gu.shape[1] % 2:
+        raise KernelRefused("silu_mul_int8 takes [rows, 2 I]")
+    return _int8_rows(gu, gu.shape[1] // 2, 2, take, "silu_mul_int8")
+
+
+def linear_int8(x: Int8Rows, w: Int8Weight, out: torch.Tensor | None = None, dtype: torch.dtype = torch.bfloat16, take=None) -> torch.Tensor:
+    """x @ w.T of operands in 8 bits: sums exact in 32-bit integers, times the row's and the channel's scale in 32-bit, rounded once to ``out``'s type (without ``out``: ``dtype``).  ``take``
+    (shape, dtype) gives scratch (``ctx.arena.take``)."""
+    if not isinstance(x, Int8Rows) or not isinstance(w, Int8Weight):
+        raise KernelRefused("linear_int8 takes rows in 8 bits (int8_rows) and an Int8Weight")
+    _gpu(x.codes, w.data, out)
+    m = x.codes.shape[0]
+    if x.k != w.k or x.codes.shape[1] != w.kp or x.codes.dtype != torch.int8 or not x.codes.is_contiguous() or x.scales.shape != (m,) or x.scales.dtype != torch.float32:
+        raise KernelRefused(f"linear_int8: rows of {x.k}, a weight of {w.k}")
+    if out is None:
+        out = torch.empty((m, w.n), dtype=dtype, device=x.codes.device)
+    if out.shape != (m, w.n) or (m and out.stride(1) != 1) or (m > 1 and out.stride(0) < w.n):
+        raise KernelRefused(f"linear_int8: out must be [{m}, {w.n}] with unit stride along a row")
+    _check(build.core().ns_gemm_int8(_ptr(out), _ptr(x.codes), _ptr(x.scales), _ptr(w.data), _ptr(w.scales), c_int(m), c_int(w.n), c_int(w.kp), c_int(max(out.stride(0), w.n)),
+                                     c_int(_dtype_code(out)), _stream()), "linear_int8")
+    return out
+
+
 # ------------------------------------------------------------------------------------------------ keys and values in 4 bits
 
 KV4_TOKENS = 8  # tokens that lie together in a record of a 4-bit page (csrc/kv4.h says how); a page is a power of two of tokens, from 8

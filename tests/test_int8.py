@@ -1,0 +1,62 @@
+"""Operands in 8 bits on the CPU: the layout, and what is refused."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+from nanospec_amd.kernels import ops
+
+
+@pytest.mark.parametrize("n,k", [(1, 1), (16, 512), (37, 700), (48, 1024)])
+def test_layout(n, k):
+    codes = torch.randint(-127, 128, (n, k), dtype=torch.int8, generator=torch.Generator().manual_seed(n))
+    w = ops.Int8Weight(codes, torch.arange(n, dtype=torch.float32))
+    assert torch.equal(w.codes(), codes) and w.kp % 256 == 0 and w.kp >= max(512, k) and torch.equal(w.scales[:n], torch.arange(n, dtype=torch.float32))
+    flat = w.data.reshape(-1)
+    for row, col in ((0, 0), (n - 1, k - 1), (n // 2, k // 2), (n // 3, k // 3)):
+        at = ((row // 16) * (w.kp // 64) + col // 64) * 1024 + (16 * (col % 64 // 16) + row % 16) * 16 + col % 16
+        assert flat[at] == codes[row, col]
+    assert int(w.data.abs().long().sum()) == int(codes.abs().long().sum())  # zeros everywhere else
+
+
+def test_from_float_keeps_rows_apart():
+    w = torch.tensor([[1.0, -2.0, 0.5], [0.0, 0.0, 0.0], [float("inf"), 1.0, 0.0], [float("nan"), 1.0, 0.0], [2.0**-110, 0.0, 0.0]])
+    made = ops.Int8Weight.from_float(w)
+    assert made.codes()[0].tolist() == [64, -127, 32] and not bool(made.codes()[1:].any())
+    assert float(made.scales[0]) == 2 / 127 or abs(float(made.scales[0]) - 2 / 127) < 1e-9
+    assert made.scales[1] == 0 and made.scales[4] == 0 and bool(torch.isnan(made.scales[2:4]).all())
+
+
+@pytest.mark.parametrize("codes,scales", [(torch.zeros(4, 8), torch.zeros(4)), (torch.zeros(4, 8, dtype=torch.int8), torch.zeros(3)), (torch.zeros(4, 8, dtype=torch.int8), torch.zeros(4).double()),
+                                          (torch.zeros(4, dtype=torch.int8), torch.zeros(4)), (torch.zeros(1, 32769, dtype=torch.int8), torch.zeros(1)), (torch.zeros(0, 8, dtype=torch.int8), torch.zeros(0))])
+def test_weights_that_are_refused(codes, scales):
+    with pytest.raises(ops.KernelRefused):
+        ops.Int8Weight(codes, scales)
+
+
+def test_rows_that_are_refused(monkeypatch):
+    x = torch.zeros(3, 64)
+    for call in (lambda: ops.int8_rows(x), lambda: ops.silu_mul_int8(x), lambda: ops.rmsnorm_int8(torch.ones(64), 1e-5, x=x)):
+        with pytest.raises(ops.KernelRefused, match="GPU"):
+            call()
+    monkeypatch.setattr(ops, "_gpu", lambda *tensors: None)
+    one = torch.ones(64)
+    for call in (lambda: ops.int8_rows(x[0]), lambda: ops.int8_rows(x.t()), lambda: ops.int8_rows(torch.zeros(1, 32769)), lambda: ops.int8_rows(x.half()), lambda: ops.int8_rows(x[:, :0]),
+                 lambda: ops.int8_rows(x[:1].expand(3, 64)), lambda: ops.silu_mul_int8(torch.zeros(3, 63)), lambda: ops.rmsnorm_int8(one, 1e-5),
+                 lambda: ops.rmsnorm_int8(one, 1e-5, x=x, resid=torch.zeros(2, 64)), lambda: ops.rmsnorm_int8(one, 1e-5, x=x, resid=x.bfloat16()), lambda: ops.rmsnorm_int8(one[:32], 1e-5, x=x),
+                 lambda: ops.rmsnorm_int8(one, 1e-5, x=x, resid_out=torch.zeros(3, 128)[:, :64])):
+        with pytest.raises(ops.KernelRefused):
+            call()
+
+
+def test_products_that_are_refused(monkeypatch):
+    monkeypatch.setattr(ops, "_gpu", lambda *tensors: None)
+    w = ops.Int8Weight(torch.zeros((48, 600), dtype=torch.int8), torch.zeros(48))
+    rows = ops.Int8Rows(torch.zeros((3, 768), dtype=torch.int8), torch.zeros(3), 600)
+    for call in (lambda: ops.linear_int8(torch.zeros(3, 600), w), lambda: ops.linear_int8(rows, torch.zeros(48, 600)), lambda: ops.linear_int8(rows, w, out=torch.zeros(3, 47)),
+                 lambda: ops.linear_int8(rows, w, out=torch.zeros(48, 3).t()), lambda: ops.linear_int8(rows, w, dtype=torch.float16),
+                 lambda: ops.linear_int8(ops.Int8Rows(rows.codes, rows.scales, 601), w), lambda: ops.linear_int8(ops.Int8Rows(rows.codes, rows.scales[:2], 600), w),
+                 lambda: ops.linear_int8(ops.Int8Rows(rows.codes[:, :512], rows.scales, 600), w), lambda: ops.linear_int8(ops.Int8Rows(rows.codes.float(), rows.scales, 600), w)):
+        with pytest.raises(ops.KernelRefused):
+            call()

@@ -1,0 +1,179 @@
+"""Products in 8-bit integers: rows quantised (as they are, behind a norm, behind a gate) and multiplied, against their definition."""
+
+from __future__ import annotations
+
+import math
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+ROUND = {torch.bfloat16: 2.0**-8, torch.float32: 2.0**-24}  # a rounding is off by at most half a step, eps / 2 relative to the value
+
+
+def _ops():
+    from nanospec_amd.kernels import ops
+
+    return ops
+
+
+def _rand(shape, seed, dtype=torch.float32):
+    return torch.randn(shape, generator=torch.Generator().manual_seed(seed)).to(dtype)
+
+
+def _defined(x: torch.Tensor):
+    """float32 rows -> codes and scales by the definition's own 32-bit operations."""
+    most = x.abs().amax(1)
+    some = most >= 2.0**-100
+    inverse = torch.where(some, torch.full_like(most, 127.0) / most, 0.0)
+    codes = torch.round(x * inverse[:, None]).clamp(-127, 127)
+    return torch.where(some[:, None], codes, 0.0), torch.where(some, most / torch.full_like(most, 127.0), 0.0)
+
+
+ROWS = [(1, 1), (3, 8), (2, 513), (5, 2048), (7, 4096), (2, 14336), (1, 28672), (2, 32768), (3, 1001), (1, 32767), (4, 20000)]
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("m,k", ROWS)
+def test_rows(m, k, dtype):
+    """Codes and scales are the definition's, bit for bit, of contiguous rows and of rows inside wider ones, at addresses between 16 bytes too."""
+    ops = _ops()
+    x = _rand((m, k), m + k, dtype) * torch.exp(_rand((m, 1), 3)).to(dtype)
+    codes, scales = _defined(x.float())
+    for pad in (0, 8, 3):
+        wide = torch.full((m, k + 2 * pad), 50.0, dtype=dtype, device=DEV)
+        wide[:, pad : pad + k] = x.to(DEV)
+        rows = ops.int8_rows(wide[:, pad : pad + k])
+        assert torch.equal(rows.codes[:, :k].cpu().float(), codes) and torch.equal(rows.scales.cpu(), scales), pad
+
+
+def test_rows_that_are_zero_tiny_or_not_finite():
+    ops = _ops()
+    x = _rand((8, 640), 1)
+    x[0] = 0
+    x[1] *= 2.0**-110
+    x[2, 5], x[3, 639], x[4, 0] = math.inf, math.nan, -math.inf
+    x[5] *= 2.0**100
+    x[6] *= 2.0**-95
+    rows = ops.int8_rows(x.to(DEV))
+    good = [0, 1, 5, 6, 7]
+    codes, scales = _defined(x[good])
+    assert torch.equal(rows.codes[good, :640].cpu().float(), codes) and torch.equal(rows.scales[good].cpu(), scales)
+    assert bool(torch.isnan(rows.scales[2:5]).all()) and not bool(rows.codes[:2, :640].any()) and not bool(rows.codes[2:5, :640].any())
+    w = ops.Int8Weight.from_float(_rand((33, 640), 2).to(DEV))
+    y = ops.linear_int8(rows, w, dtype=torch.float32)
+    assert bool(torch.isnan(y[2:5]).all()) and bool(torch.isfinite(y[good]).all()) and not bool(y[:2].any())
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("m,k", [(1, 64), (5, 2048), (3, 1001), (2, 32768)])
+@pytest.mark.parametrize("form", ["resid and x", "resid", "x", "stored elsewhere"])
+def test_rows_behind_the_norm(m, k, dtype, form):
+    ops = _ops()
+    resid, x, weight, eps = _rand((m, k), 1, dtype) * 3, _rand((m, k), 2, dtype), (1 + 0.2 * _rand((k,), 3)).to(dtype), 1e-5
+    r = {"resid": resid, "x": x}.get(form, (resid.float() + x.float()).to(dtype))
+    keep = resid.to(DEV)
+    args = dict(resid=keep if form != "x" else None, x=x.to(DEV) if form != "resid" else None)
+    to = torch.full_like(keep, 9.0)
+    if form == "resid and x":
+        args["resid_out"] = keep
+    elif form == "stored elsewhere":
+        args["resid_out"] = to
+    rows = ops.rmsnorm_int8(weight.to(DEV), eps, **args)
+    if form == "resid and x":
+        assert torch.equal(keep.cpu(), r)
+    else:
+        assert torch.equal(keep.cpu(), resid) and torch.equal(to.cpu(), r if form == "stored elsewhere" else torch.full_like(r, 9.0))
+    y = r.double() * (r.double().square().mean(1, keepdim=True) + eps).rsqrt() * weight.double()
+    most = y.abs().amax(1)
+    # the mean of k squares (sums of a thread, a wave and a workgroup: at most 32 + 6 + 16 roundings of 2^-24 of it, halved by the root), 1 / sqrt to 2 units, two products
+    off = (27 + 4) * 2.0**-24 + 2.0**-22
+    assert bool(((rows.scales.cpu().double() - most / 127).abs() <= (off + 2.0**-23) * most / 127).all())
+    # a code is next to the value, or the one beside it where the value lies half way between the two
+    far = (rows.codes[:, :k].cpu().double() - y * (127 / most)[:, None]).abs()
+    assert float(far.max()) <= 0.5 + 127 * (2 * off + 2.0**-22)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("m,k", [(1, 64), (5, 8192), (3, 1001), (2, 28672), (1, 32768)])
+def test_rows_behind_the_gate(m, k, dtype):
+    ops = _ops()
+    gu = _rand((m, 2 * k), m + k, dtype) * 4
+    rows = ops.silu_mul_int8(gu.to(DEV))
+    g, u = gu.double().chunk(2, 1)
+    y = g * torch.sigmoid(g) * u
+    most = y.abs().amax(1)
+    off = 8 * 2.0**-24  # exp to 2 units, the sum, the quotient, the product, each 2^-24 of the value (the exponential's argument is exact)
+    assert bool(((rows.scales.cpu().double() - most / 127).abs() <= (off + 2.0**-23) * most / 127).all())
+    far = (rows.codes[:, :k].cpu().double() - y * (127 / most)[:, None]).abs()
+    assert float(far.max()) <= 0.5 + 127 * (2 * off + 2.0**-22)
+
+
+def _operands(m, n, k, seed):
+    gen = torch.Generator().manual_seed(seed)
+    cx = torch.randint(-127, 128, (m, k), generator=gen, dtype=torch.int8)
+    cw = torch.randint(-127, 128, (n, k), generator=gen, dtype=torch.int8)
+    xs, ws = torch.rand(m, generator=gen) + 0.5, torch.rand(n, generator=gen) + 0.5
+    return cx, xs, cw, ws
+
+
+def _rows(cx, xs):
+    """Rows in 8 bits whose padding holds what must not count."""
+    ops = _ops()
+    codes = torch.full((cx.shape[0], ops.int8_padded_k(cx.shape[1])), 113, dtype=torch.int8, device=DEV)
+    codes[:, : cx.shape[1]] = cx.to(DEV)
+    return ops.Int8Rows(codes, xs.to(DEV), cx.shape[1])
+
+
+PRODUCTS = [(1, 1, 1), (1, 2048, 2048), (16, 33, 512), (17, 20, 513), (3, 500, 14336), (33, 130, 4096), (64, 1000, 1100), (65, 4096, 768), (128, 257, 2304), (129, 100, 1024),
+            (255, 512, 512), (300, 1023, 3333), (520, 64, 8192), (1100, 2050, 640), (8, 7168, 4096), (61, 4096, 4096)]
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("m,n,k", PRODUCTS)
+def test_product(m, n, k, dtype):
+    """The sums are whole numbers below 2^31 and exact; two products with the scales and the conversion round three times in 32-bit, then once to the type.  Nothing beside the result
+    is written."""
+    ops = _ops()
+    cx, xs, cw, ws = _operands(m, n, k, m + n + k)
+    w = ops.Int8Weight(cw.to(DEV), ws.to(DEV))
+    assert torch.equal(w.codes().cpu(), cw)
+    room = torch.full((m + 1, n + 5), 7.0, dtype=dtype, device=DEV)
+    y = ops.linear_int8(_rows(cx, xs), w, out=room[:m, :n])
+    want = (cx.double().to(DEV) @ cw.double().to(DEV).T).cpu() * xs.double()[:, None] * ws.double()
+    assert bool(((y.cpu().double() - want).abs() <= (3 * 2.0**-24 * 1.001 + ROUND[dtype]) * want.abs()).all())
+    assert bool((room[m] == 7).all()) and bool((room[:, n:] == 7).all())
+    assert torch.equal(ops.linear_int8(_rows(cx, xs), w, dtype=dtype), y)
+
+
+def test_product_of_the_largest_sums():
+    """32,768 products of 127 * 127: 528,515,072, of either sign."""
+    ops = _ops()
+    k = 32768
+    cx = torch.full((130, k), 127, dtype=torch.int8)
+    cw = torch.full((70, k), 127, dtype=torch.int8)
+    cw[1::2] = -127
+    w = ops.Int8Weight(cw.to(DEV), torch.ones(70, device=DEV))
+    for m in (1, 40, 130):
+        y = ops.linear_int8(_rows(cx[:m], torch.ones(m)), w, dtype=torch.float32).cpu()
+        assert bool((y[:, ::2] == 127 * 127 * k).all()) and bool((y[:, 1::2] == -127 * 127 * k).all())
+
+
+def test_product_of_no_rows():
+    ops = _ops()
+    w = ops.Int8Weight.from_float(torch.randn(48, 64, device=DEV))
+    assert ops.linear_int8(ops.int8_rows(torch.randn(0, 64, device=DEV)), w).shape == (0, 48)
+
+
+@pytest.mark.parametrize("n,k", [(5, 7), (300, 4096), (64, 14336)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_weight_from_values(n, k, dtype):
+    ops = _ops()
+    w = _rand((n, k), n, dtype)
+    w[n // 2] = 0
+    made = ops.Int8Weight.from_float(w.to(DEV))
+    codes, scales = made.codes().cpu().double(), made.scales[:n].cpu().double()
+    most = w.double().abs().amax(1)
+    assert bool(((scales - most / 127).abs() <= 2.0**-23 * most).all())
+    assert bool(((codes * scales[:, None] - w.double()).abs() <= scales[:, None] * (0.5 + 127 * 2.0**-22)).all()) and not bool(codes[n // 2].any())
