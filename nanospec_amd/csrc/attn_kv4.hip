@@ -162,3 +162,48 @@ extern "C" int ns_attn_kv4_plain(void* out, void* part_o, void* part_l, const vo
     return NS_ERR_UNSUPPORTED;
   return ns_launch_status();
 }
+
+#include "attn_kv4_mfma.h"
+
+template <typename T, int HD, int PARTS>
+static int launch_tiles(const Kv4AttnParams& a, int rows, hipStream_t stream) {
+  const int group = a.heads / a.kv_heads;
+  if (rows) {
+    const long long items = (long long)a.n_tiles * a.kv_heads * ((group + 15) / 16);
+    if (items > 0x7fffffff) return NS_ERR_UNSUPPORTED;
+    attn_kv4_rows_kernel<T, HD, PARTS><<<dim3((unsigned)items, (unsigned)a.splits), 256, 0, stream>>>(a);
+  } else {
+    // two heads of a group share a wave's keys where there are two
+    const int heads = group > 1 ? 2 : 1;
+    const long long items = (long long)a.n_tiles * a.splits * a.kv_heads * ((group + heads - 1) / heads);
+    if (items > 0x7fffffff) return NS_ERR_UNSUPPORTED;
+    const unsigned grid = (unsigned)((items + 3) / 4);
+    if (heads == 2)
+      attn_kv4_tiles_kernel<T, HD, 4, PARTS><<<grid, 256, 0, stream>>>(a);
+    else
+      attn_kv4_tiles_kernel<T, HD, 2, PARTS><<<grid, 256, 0, stream>>>(a);
+  }
+  if (a.splits > 1) {
+    const long long cols = (long long)a.n_tiles * (rows ? 1 : KV4_TILE_TOKENS) * a.heads;
+    if (cols > 0x7fffffff) return NS_ERR_UNSUPPORTED;
+    attn_kv4_join_kernel<T><<<(unsigned)cols, 64, 0, stream>>>(a, rows ? 1 : KV4_TILE_TOKENS);
+  }
+  return ns_launch_status();
+}
+
+// Attention of the tokens that ``tiles`` [n_tiles][8] names: request, first token of the tile among the request's tokens of this step, row of the request's first token, tokens of the
+// request in this step, keys after it, three more.  rows 1: a tile is one token; 0: up to 32.  part_o: float32 [n_tiles * tokens of a tile * heads * splits * hd] and part_l
+// [n_tiles * tokens of a tile * heads * splits] with splits > 1.
+extern "C" int ns_attn_kv4(void* out, void* part_o, void* part_l, const void* q, int q_stride, const void* pool, const int* tiles, const int* block_table, int table_stride,
+                           int n_tiles, int heads, int kv_heads, int hd, int page, int rows, int splits, int window, float scale, int dtype, hipStream_t stream) {
+  if (n_tiles < 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads || page < KV4_TOKENS || (page & (page - 1)) || window < 0) return NS_ERR_BAD_ARG;
+  if (splits < 1 || splits > 64 || (splits > 1 && (!part_o || !part_l))) return NS_ERR_BAD_ARG;
+  if (hd != 64 && hd != 128) return NS_ERR_UNSUPPORTED;
+  if ((((uintptr_t)out | (uintptr_t)pool | (uintptr_t)part_o) & 15) != 0) return NS_ERR_UNSUPPORTED;
+  if (n_tiles == 0) return NS_OK;
+  const Kv4AttnParams a{out, (float*)part_o, (float*)part_l, q, (const uint8_t*)pool, tiles, nullptr, nullptr, block_table, q_stride, table_stride, n_tiles, heads, kv_heads,
+                        hd, page, splits, window, scale * 1.4426950408889634f};
+  if (dtype == NS_DTYPE_F32) return hd == 64 ? launch_tiles<float, 64, 2>(a, rows, stream) : launch_tiles<float, 128, 2>(a, rows, stream);
+  if (dtype == NS_DTYPE_BF16) return hd == 64 ? launch_tiles<bf16_t, 64, 1>(a, rows, stream) : launch_tiles<bf16_t, 128, 1>(a, rows, stream);
+  return NS_ERR_UNSUPPORTED;
+}

@@ -1401,6 +1401,33 @@ def _check_kv4_attn(q, out, pages: Kv4Pages, heads: int, kv_heads: int, head_dim
     return po, pl
 
 
+def kv4_tiles_take(head_dim: int) -> bool:
+    """The head sizes that ``attention_kv4`` is built for."""
+    return head_dim in (64, 128)
+
+
+def attention_kv4(q, out, pages: Kv4Pages, tiles, block_table, heads: int, kv_heads: int, head_dim: int, scale: float, rows: bool, window: int = 0, splits: int = 1,
+                  workspace: tuple[torch.Tensor, torch.Tensor] | None = None) -> torch.Tensor:
+    """Attention over 4-bit pages on the matrix cores, head sizes 64 and 128, bfloat16 and float32, of the tokens that ``tiles`` (int32 [n_tiles, 8], as for ``attention_mfma``) describe:
+    with ``rows`` single tokens, a tile each, otherwise portions in tiles of up to 32 tokens.  Tokens that no tile describes are left as they are.  ``splits`` > 1 cuts the keys of every tile into
+    that many ranges and needs ``workspace`` = float32 tensors of columns * splits * head_dim and columns * splits values, columns = tiles * (1 or 32) * heads."""
+    if not isinstance(pages, Kv4Pages):
+        raise KernelRefused("attention_kv4 takes 4-bit pages (Kv4Pages)")
+    if not kv4_tiles_take(head_dim):
+        raise KernelRefused(f"attention_kv4 takes head sizes 64 and 128, not {head_dim} (attention_kv4_plain takes it)")
+    _gpu(pages.pool, tiles, block_table)
+    _i32(tiles, "tiles")
+    _kv4_table(block_table, "attention_kv4")
+    if tiles.dim() != 2 or tiles.shape[1] != TILE_INTS:
+        raise KernelRefused(f"attention_kv4: tiles must be int32 [n_tiles, {TILE_INTS}]")
+    n_tiles = tiles.shape[0]
+    po, pl = _check_kv4_attn(q, out, pages, heads, kv_heads, head_dim, window, splits, workspace, n_tiles * (1 if rows else 32) * heads, "attention_kv4")
+    _check(build.core().ns_attn_kv4(_ptr(out), _ptr(po), _ptr(pl), _ptr(q), c_int(q.stride(0)), _ptr(pages.pool), _ptr(tiles), _ptr(block_table), c_int(block_table.stride(0)),
+                                    c_int(n_tiles), c_int(heads), c_int(kv_heads), c_int(head_dim), c_int(pages.page), c_int(1 if rows else 0), c_int(splits), c_int(window),
+                                    c_float(scale), c_int(_dtype_code(q)), _stream()), "attention_kv4")
+    return out
+
+
 def attention_kv4_plain(q, out, pages: Kv4Pages, token_req, positions, block_table, heads: int, kv_heads: int, head_dim: int, scale: float, window: int = 0, splits: int = 1,
                         workspace: tuple[torch.Tensor, torch.Tensor] | None = None) -> torch.Tensor:
     """Attention of every token over its request's 4-bit pages, in plain 32-bit arithmetic: bfloat16 and float32, any head size that such pages take.  ``q`` [tokens, >= heads *

@@ -29,6 +29,8 @@ LONG_ROW_KEYS = 8192  # rows that may reach this many keys get up to 32 ranges i
 F32_RANGE_KEYS = 128  # keys of a range of a single token's row in 32-bit: two tiles of 16 for each wave of its workgroup
 KV4_MAX_RANGES = 64  # of a row's keys in 4 bits, and the fewest keys of one
 KV4_RANGE_KEYS = 256
+KV4_PORTION_KEYS = 512  # the fewest keys of a range of a portion's
+KV4_GROUPS_PER_UNIT = 4  # workgroups of single tokens for each compute unit that ranges of keys are cut for
 QKV_JOIN_MAX_RANGES = 4  # 17 to 128 rows: the kernel that joins the ranges of the q/k/v product, rotates and writes the cache reads
 #                          every range, so more of them cost it what they gain the product
 
@@ -226,13 +228,33 @@ def f32_attention(ctx, q, out, cache, table, heads: int, kv_heads: int, head_dim
 
 
 def kv4_attention(ctx, q, out, pages, table, heads: int, kv_heads: int, head_dim: int, scale: float, window: int = 0) -> torch.Tensor:
-    """Attention of the batch's tokens over pages of 4 bits (``ops.Kv4Pages``)."""
-    n, take = q.shape[0], ctx.arena.take
-    longest = min(ctx.max_kv_len, window) if window else ctx.max_kv_len
-    # a workgroup a token, head and range of keys, until there are four for each compute unit
-    splits = max(1, min(KV4_MAX_RANGES, 4 * ops.compute_units(q.device) // max(1, n * heads), -(-longest // KV4_RANGE_KEYS)))
-    ws = (take((n * heads * splits * head_dim,), torch.float32), take((n * heads * splits,), torch.float32)) if splits > 1 else None
-    return ops.attention_kv4_plain(q, out, pages, ctx.token_req, ctx.positions, table, heads, kv_heads, head_dim, scale, window=window, splits=splits, workspace=ws)
+    """Attention of the batch's tokens over pages of 4 bits (``ops.Kv4Pages``): head sizes 64 and 128 on the matrix cores, portions and single tokens by their tiles, others in plain
+    32-bit arithmetic.  A batch without tiles has its tokens all in the latter."""
+    take, units, group = ctx.arena.take, ops.compute_units(q.device), heads // kv_heads
+    span = window or 1 << 30
+
+    def workspace(columns: int, splits: int):
+        return (take((columns * splits * head_dim,), torch.float32), take((columns * splits,), torch.float32)) if splits > 1 else None
+
+    if not ops.kv4_tiles_take(head_dim) or TilePlan.key not in ctx.plans:
+        # a workgroup a token, head and range of keys, until there are four for each compute unit
+        n, longest = q.shape[0], min(ctx.max_kv_len, span)
+        splits = max(1, min(KV4_MAX_RANGES, 4 * units // max(1, n * heads), -(-longest // KV4_RANGE_KEYS)))
+        return ops.attention_kv4_plain(q, out, pages, ctx.token_req, ctx.positions, table, heads, kv_heads, head_dim, scale, window=window, splits=splits,
+                                       workspace=workspace(n * heads, splits))
+    portions, singles = TilePlan.views(ctx)
+    if portions.shape[0]:
+        tiles, longest = portions.shape[0], min(ctx.max_chunk_kv, span + TilePlan.TOKENS)
+        waves = tiles * kv_heads * -(-group // (2 if group > 1 else 1))
+        splits = max(1, min(KV4_MAX_RANGES, 8 * units // waves, longest // KV4_PORTION_KEYS))
+        ops.attention_kv4(q, out, pages, portions, table, heads, kv_heads, head_dim, scale, rows=False, window=window, splits=splits,
+                          workspace=workspace(tiles * TilePlan.TOKENS * heads, splits))
+    if singles.shape[0]:
+        tiles, longest = singles.shape[0], min(ctx.max_kv_len, span)
+        groups = tiles * kv_heads * -(-group // 16)
+        splits = max(1, min(KV4_MAX_RANGES, KV4_GROUPS_PER_UNIT * units // groups, -(-longest // KV4_RANGE_KEYS)))
+        ops.attention_kv4(q, out, pages, singles, table, heads, kv_heads, head_dim, scale, rows=True, window=window, splits=splits, workspace=workspace(tiles * heads, splits))
+    return out
 
 
 class Attention:
