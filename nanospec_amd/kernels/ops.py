@@ -1136,9 +1136,8 @@ def int8_padded_k(k: int) -> int:
 
 
 class Int8Weight:
-    """A weight matrix [N, K] in 8 bits: codes of -127 to 127 and a float32 scale for each output channel (a row), which stand for scale * code.  The codes are laid out once, in
-    pieces of 1 KiB that are operands of the 8-bit matrix instruction: wt[row tile][k / 64][lane = 16 g + r][16] = w[16 tile + r][64 piece + 16 g + ..], rows padded to a
-    multiple of 16 and k to ``int8_padded_k`` with zeros."""
+    """A weight matrix [N, K] in 8 bits: codes of -127 to 127 and a float32 scale for each output channel (a row), which stand for scale * code.  The codes are laid out once
+    (``_int8_fragments``)."""
 
     def __init__(self, codes: torch.Tensor, scales: torch.Tensor) -> None:
         if codes.dtype != torch.int8 or codes.dim() != 2 or min(codes.shape) < 1 or codes.shape[1] > INT8_MAX_K:
@@ -1147,14 +1146,8 @@ class Int8Weight:
             raise KernelRefused("Int8Weight takes a float32 scale for each row of the codes, on their device")
         self.n, self.k = codes.shape
         self.kp = int8_padded_k(self.k)
-        n_pad = -(-self.n // 16) * 16
-        if (n_pad, self.kp) != codes.shape:
-            padded = torch.zeros((n_pad, self.kp), dtype=torch.int8, device=codes.device)
-            padded[: self.n, : self.k] = codes
-        else:
-            padded = codes
-        self.data = padded.view(n_pad // 16, 16, self.kp // 64, 4, 16).permute(0, 2, 3, 1, 4).contiguous()
-        self.scales = torch.zeros(n_pad, dtype=torch.float32, device=codes.device)
+        self.data = _int8_fragments(codes)
+        self.scales = torch.zeros(-(-self.n // 16) * 16, dtype=torch.float32, device=codes.device)
         self.scales[: self.n] = scales
 
     @classmethod
@@ -1176,17 +1169,44 @@ class Int8Weight:
 
     def codes(self) -> torch.Tensor:
         """-> int8 [N, K]"""
-        n_pad = self.data.shape[0] * 16
-        return self.data.permute(0, 3, 1, 2, 4).reshape(n_pad, self.kp)[: self.n, : self.k]
+        return _int8_plain(self.data, self.n, self.k)
+
+
+def _int8_fragments(codes: torch.Tensor) -> torch.Tensor:
+    """int8 [rows, K] -> [row blocks, k / 64, 4, 16, 16], padded with zeros to whole blocks of 16 rows and ``int8_padded_k``: pieces of 1 KiB that are operands of the 8-bit matrix
+    instruction, [block][piece][lane = 16 g + r][16] = codes[16 block + r][64 piece + 16 g + ..]."""
+    (rows, k), kp = codes.shape, int8_padded_k(codes.shape[1])
+    blocks = -(-rows // 16)
+    if (16 * blocks, kp) != (rows, k):
+        padded = torch.zeros((16 * blocks, kp), dtype=torch.int8, device=codes.device)
+        padded[:rows, :k] = codes
+        codes = padded
+    return codes.view(blocks, 16, kp // 64, 4, 16).permute(0, 2, 3, 1, 4).contiguous()
+
+
+def _int8_plain(data: torch.Tensor, rows: int, k: int) -> torch.Tensor:
+    """The way back."""
+    return data.permute(0, 3, 1, 2, 4).reshape(data.shape[0] * 16, data.shape[1] * 64)[:rows, :k]
 
 
 class Int8Rows:
-    """Activations in 8 bits: ``codes`` int8 [rows, ``int8_padded_k``] (what lies beyond ``k`` counts for nothing), ``scales`` float32 [rows], which stand for
-    scale * code.  Made by ``int8_rows``, ``rmsnorm_int8`` and ``silu_mul_int8``, taken by ``linear_int8``."""
+    """Activations in 8 bits: ``data`` int8 [row blocks, ``int8_padded_k`` / 64, 4, 16, 16] (laid out as an ``Int8Weight``; what lies in it beyond the rows and ``k`` counts for
+    nothing), ``scales`` float32 [rows], which stand for scale * code.  Made by ``int8_rows``, ``rmsnorm_int8`` and ``silu_mul_int8``, taken by ``linear_int8``."""
 
-    def __init__(self, codes: torch.Tensor, scales: torch.Tensor, k: int) -> None:
-        self.codes, self.scales, self.k = codes, scales, k
-        self.shape = (codes.shape[0], k)
+    def __init__(self, data: torch.Tensor, scales: torch.Tensor, k: int) -> None:
+        self.data, self.scales, self.k = data, scales, k
+        self.shape = (scales.shape[0], k)
+
+    @classmethod
+    def from_codes(cls, codes: torch.Tensor, scales: torch.Tensor) -> "Int8Rows":
+        """Codes int8 [rows, K] and a float32 scale for each row that were made elsewhere."""
+        if codes.dtype != torch.int8 or codes.dim() != 2 or not 1 <= codes.shape[1] <= INT8_MAX_K or scales.dtype != torch.float32 or scales.shape != codes.shape[:1]:
+            raise KernelRefused(f"Int8Rows.from_codes takes int8 [rows, K] with K up to {INT8_MAX_K} and a float32 scale for each row")
+        return cls(_int8_fragments(codes), scales.contiguous(), codes.shape[1])
+
+    def codes(self) -> torch.Tensor:
+        """-> int8 [rows, K]"""
+        return _int8_plain(self.data, *self.shape)
 
 
 def _int8_rows(x: torch.Tensor, k: int, src: int, take, what: str, resid=None, resid_out=None, weight=None, eps: float = 0.0) -> Int8Rows:
@@ -1194,9 +1214,9 @@ def _int8_rows(x: torch.Tensor, k: int, src: int, take, what: str, resid=None, r
     if not 1 <= k <= INT8_MAX_K or x.shape[1] != width or (m > 1 and x.stride(0) < width) or (m and x.stride(1) != 1):
         raise KernelRefused(f"{what}: rows of up to {INT8_MAX_K} values with unit stride along a row; got {tuple(x.shape)}")
     take = take or (lambda shape, dtype: torch.empty(shape, dtype=dtype, device=x.device))
-    rows = Int8Rows(take((m, int8_padded_k(k)), torch.int8), take((m,), torch.float32), k)
-    _check(build.core().ns_int8_rows(_ptr(rows.codes), _ptr(rows.scales), _ptr(x), c_int(max(x.stride(0), width)), _ptr(resid), _ptr(resid_out), _ptr(weight), c_float(eps), c_int(m),
-                                     c_int(k), c_int(rows.codes.shape[1]), c_int(src), c_int(_dtype_code(x)), _stream()), what)
+    rows = Int8Rows(take((-(-m // 16), int8_padded_k(k) // 64, 4, 16, 16), torch.int8), take((m,), torch.float32), k)
+    _check(build.core().ns_int8_rows(_ptr(rows.data), _ptr(rows.scales), _ptr(x), c_int(max(x.stride(0), width)), _ptr(resid), _ptr(resid_out), _ptr(weight), c_float(eps), c_int(m),
+                                     c_int(k), c_int(int8_padded_k(k)), c_int(src), c_int(_dtype_code(x)), _stream()), what)
     return rows
 
 
@@ -1234,21 +1254,61 @@ def silu_mul_int8(gu: torch.Tensor, take=None) -> Int8Rows:
     return _int8_rows(gu, gu.shape[1] // 2, 2, take, "silu_mul_int8")
 
 
+INT8_TILES = ((64, 64), (64, 128), (128, 64), (128, 128), (256, 128), (256, 256))  # rows of x by rows of the weight, as ``ns_gemm_int8_many`` numbers them
+INT8_FEW_WORK = 5e7  # blocks of 16 rows of x times columns times K
+INT8_TILE_US = (2.02, 3.43, 3.01, 5.42, 7.30, 10.13)  # of a tile for 1,024 of K, and once a tile
+INT8_TILE_ONCE_US = (0.06, 0.16, 0.47, 0.15, 1.53, 4.09)
+
+
+@functools.lru_cache(maxsize=1 << 14)
+def int8_plan(m: int, n: int, k: int, units: int) -> tuple[int, int] | None:
+    """(tile, ranges of K) of a product of m rows and n columns in tiles, or None where the kernel for few rows is the faster one.
+
+    That one reads the weight once for every 16 rows, so it is taken up to 16 rows and as long as what it reads fits the caches.  us, it and the best tiles: 32 rows of 4,096 x 4,096 6.8 and 9.7, 48 8.5 and
+    10.1, 64 13.0 and 10.9; of 6,144 x 4,096 32 10.1 and 11.0, 48 15.0 and 12.2; of 2,048 x 2,048 128 6.4 and 7.6; of 16,384 x 2,048 16 8.3 and 9.0, 24 13.1 and 9.4.
+    The tiles are chosen by what they take, in us: 3.8, and for every round of as many tiles as there are units a tile's time, but no less than the weight at 5.2 TB/s; ranges of K 2.0 more, and their sums
+    at 2.5 TB/s.  Over 198 products (16 to 2,048 rows, 1,000 x 1,111 to 8,192 x 28,672) the choice takes 1.02 times as long as the best of all tiles and ranges, 1.27 at worst (1,500 rows of 12,288 x 3,000)."""
+    if m <= 16 or -(-m // 16) * n * k <= INT8_FEW_WORK:
+        return None
+    kp, best = int8_padded_k(k), None
+    for form, (bm, bn) in enumerate(INT8_TILES):
+        tiles = -(-m // bm) * -(-n // bn)
+        for ranges in (1, 2, 3, 4, 6, 8):
+            if ranges > 1 and kp < ranges * INT8_K_MIN:
+                break
+            us = max(3.8 + -(-tiles * ranges // units) * (INT8_TILE_US[form] * kp / (1024 * ranges) + INT8_TILE_ONCE_US[form]), 3.8 + n * kp / 5.2e6)
+            us += 2.0 + ranges * m * n * 4 / 2.5e6 if ranges > 1 else 0.0
+            if best is None or us < best[0]:
+                best = us, form, ranges
+    return best[1], best[2]
+
+
 def linear_int8(x: Int8Rows, w: Int8Weight, out: torch.Tensor | None = None, dtype: torch.dtype = torch.bfloat16, take=None) -> torch.Tensor:
     """x @ w.T of operands in 8 bits: sums exact in 32-bit integers, times the row's and the channel's scale in 32-bit, rounded once to ``out``'s type (without ``out``: ``dtype``).  ``take``
     (shape, dtype) gives scratch (``ctx.arena.take``)."""
     if not isinstance(x, Int8Rows) or not isinstance(w, Int8Weight):
         raise KernelRefused("linear_int8 takes rows in 8 bits (int8_rows) and an Int8Weight")
-    _gpu(x.codes, w.data, out)
-    m = x.codes.shape[0]
-    if x.k != w.k or x.codes.shape[1] != w.kp or x.codes.dtype != torch.int8 or not x.codes.is_contiguous() or x.scales.shape != (m,) or x.scales.dtype != torch.float32:
+    _gpu(x.data, w.data, out)
+    m = x.scales.shape[0]
+    if x.k != w.k or x.data.shape != (-(-m // 16), w.kp // 64, 4, 16, 16) or x.data.dtype != torch.int8 or not x.data.is_contiguous() or x.scales.shape != (m,) or x.scales.dtype != torch.float32:
         raise KernelRefused(f"linear_int8: rows of {x.k}, a weight of {w.k}")
     if out is None:
-        out = torch.empty((m, w.n), dtype=dtype, device=x.codes.device)
+        out = torch.empty((m, w.n), dtype=dtype, device=x.data.device)
     if out.shape != (m, w.n) or (m and out.stride(1) != 1) or (m > 1 and out.stride(0) < w.n):
         raise KernelRefused(f"linear_int8: out must be [{m}, {w.n}] with unit stride along a row")
-    _check(build.core().ns_gemm_int8(_ptr(out), _ptr(x.codes), _ptr(x.scales), _ptr(w.data), _ptr(w.scales), c_int(m), c_int(w.n), c_int(w.kp), c_int(max(out.stride(0), w.n)),
-                                     c_int(_dtype_code(out)), _stream()), "linear_int8")
+    code = _dtype_code(out)
+    lib, common = build.core(), (c_int(m), c_int(w.n), c_int(w.kp), c_int(max(out.stride(0), w.n)))
+    operands = (_ptr(x.data), _ptr(x.scales), _ptr(w.data), _ptr(w.scales))
+    plan = int8_plan(m, w.n, w.k, compute_units(out.device))
+    if plan is None:
+        _check(lib.ns_gemm_int8(_ptr(out), *operands, *common, c_int(code), _stream()), "linear_int8")
+        return out
+    form, ranges = plan
+    parts = None
+    if ranges > 1:
+        shape = (ranges * m * (-(-w.n // 4) * 4),)
+        parts = take(shape, torch.int32) if take is not None else torch.empty(shape, dtype=torch.int32, device=out.device)
+    _check(lib.ns_gemm_int8_many(_ptr(out), _ptr(parts), *operands, *common, c_int(form), c_int(ranges), c_int(code), _stream()), "linear_int8")
     return out
 
 

@@ -53,10 +53,26 @@ def test_rows_that_are_refused(monkeypatch):
 def test_products_that_are_refused(monkeypatch):
     monkeypatch.setattr(ops, "_gpu", lambda *tensors: None)
     w = ops.Int8Weight(torch.zeros((48, 600), dtype=torch.int8), torch.zeros(48))
-    rows = ops.Int8Rows(torch.zeros((3, 768), dtype=torch.int8), torch.zeros(3), 600)
+    rows = ops.Int8Rows.from_codes(torch.zeros((3, 600), dtype=torch.int8), torch.zeros(3))
     for call in (lambda: ops.linear_int8(torch.zeros(3, 600), w), lambda: ops.linear_int8(rows, torch.zeros(48, 600)), lambda: ops.linear_int8(rows, w, out=torch.zeros(3, 47)),
                  lambda: ops.linear_int8(rows, w, out=torch.zeros(48, 3).t()), lambda: ops.linear_int8(rows, w, dtype=torch.float16),
-                 lambda: ops.linear_int8(ops.Int8Rows(rows.codes, rows.scales, 601), w), lambda: ops.linear_int8(ops.Int8Rows(rows.codes, rows.scales[:2], 600), w),
-                 lambda: ops.linear_int8(ops.Int8Rows(rows.codes[:, :512], rows.scales, 600), w), lambda: ops.linear_int8(ops.Int8Rows(rows.codes.float(), rows.scales, 600), w)):
+                 lambda: ops.linear_int8(ops.Int8Rows(rows.data, rows.scales, 601), w), lambda: ops.linear_int8(ops.Int8Rows(rows.data, torch.zeros(17), 600), w),
+                 lambda: ops.linear_int8(ops.Int8Rows(rows.data[:, :8], rows.scales, 600), w), lambda: ops.linear_int8(ops.Int8Rows(rows.data.float(), rows.scales, 600), w),
+                 lambda: ops.Int8Rows.from_codes(torch.zeros(3, 600), torch.zeros(3)), lambda: ops.Int8Rows.from_codes(torch.zeros((3, 600), dtype=torch.int8), torch.zeros(2))):
         with pytest.raises(ops.KernelRefused):
             call()
+
+
+def test_plan():
+    """Few rows, or little to read, go by 16 rows; ranges of K are as long as a tile takes at least; a plan stands for every size."""
+    assert ops.int8_plan(1, 28672, 4096, 256) is None and ops.int8_plan(16, 28672, 4096, 256) is None and ops.int8_plan(32, 4096, 4096, 256) is None
+    assert ops.int8_plan(17, 28672, 4096, 256) is not None and ops.int8_plan(64, 4096, 4096, 256) is not None
+    for m in (17, 100, 999, 4096, 70000):
+        for n in (1, 1000, 4096, 128256):
+            for k in (1, 513, 4096, 32768):
+                plan = ops.int8_plan(m, n, k, 256)
+                if plan is not None:
+                    form, ranges = plan
+                    assert 0 <= form < len(ops.INT8_TILES) and ops.int8_padded_k(k) >= ranges * ops.INT8_K_MIN
+                    tiles = -(-m // ops.INT8_TILES[form][0]) * -(-n // ops.INT8_TILES[form][1])
+                    assert tiles * ranges <= 1 << 22

@@ -45,7 +45,7 @@ def test_rows(m, k, dtype):
         wide = torch.full((m, k + 2 * pad), 50.0, dtype=dtype, device=DEV)
         wide[:, pad : pad + k] = x.to(DEV)
         rows = ops.int8_rows(wide[:, pad : pad + k])
-        assert torch.equal(rows.codes[:, :k].cpu().float(), codes) and torch.equal(rows.scales.cpu(), scales), pad
+        assert torch.equal(rows.codes().cpu().float(), codes) and torch.equal(rows.scales.cpu(), scales), pad
 
 
 def test_rows_that_are_zero_tiny_or_not_finite():
@@ -59,8 +59,8 @@ def test_rows_that_are_zero_tiny_or_not_finite():
     rows = ops.int8_rows(x.to(DEV))
     good = [0, 1, 5, 6, 7]
     codes, scales = _defined(x[good])
-    assert torch.equal(rows.codes[good, :640].cpu().float(), codes) and torch.equal(rows.scales[good].cpu(), scales)
-    assert bool(torch.isnan(rows.scales[2:5]).all()) and not bool(rows.codes[:2, :640].any()) and not bool(rows.codes[2:5, :640].any())
+    assert torch.equal(rows.codes()[good].cpu().float(), codes) and torch.equal(rows.scales[good].cpu(), scales)
+    assert bool(torch.isnan(rows.scales[2:5]).all()) and not bool(rows.codes()[:2].any()) and not bool(rows.codes()[2:5].any())
     w = ops.Int8Weight.from_float(_rand((33, 640), 2).to(DEV))
     y = ops.linear_int8(rows, w, dtype=torch.float32)
     assert bool(torch.isnan(y[2:5]).all()) and bool(torch.isfinite(y[good]).all()) and not bool(y[:2].any())
@@ -91,7 +91,7 @@ def test_rows_behind_the_norm(m, k, dtype, form):
     off = (27 + 4) * 2.0**-24 + 2.0**-22
     assert bool(((rows.scales.cpu().double() - most / 127).abs() <= (off + 2.0**-23) * most / 127).all())
     # a code is next to the value, or the one beside it where the value lies half way between the two
-    far = (rows.codes[:, :k].cpu().double() - y * (127 / most)[:, None]).abs()
+    far = (rows.codes().cpu().double() - y * (127 / most)[:, None]).abs()
     assert float(far.max()) <= 0.5 + 127 * (2 * off + 2.0**-22)
 
 
@@ -106,7 +106,7 @@ def test_rows_behind_the_gate(m, k, dtype):
     most = y.abs().amax(1)
     off = 8 * 2.0**-24  # exp to 2 units, the sum, the quotient, the product, each 2^-24 of the value (the exponential's argument is exact)
     assert bool(((rows.scales.cpu().double() - most / 127).abs() <= (off + 2.0**-23) * most / 127).all())
-    far = (rows.codes[:, :k].cpu().double() - y * (127 / most)[:, None]).abs()
+    far = (rows.codes().cpu().double() - y * (127 / most)[:, None]).abs()
     assert float(far.max()) <= 0.5 + 127 * (2 * off + 2.0**-22)
 
 
@@ -119,11 +119,13 @@ def _operands(m, n, k, seed):
 
 
 def _rows(cx, xs):
-    """Rows in 8 bits whose padding holds what must not count."""
+    """Rows in 8 bits whose padding, beyond their values and behind the last row, holds what must not count."""
     ops = _ops()
-    codes = torch.full((cx.shape[0], ops.int8_padded_k(cx.shape[1])), 113, dtype=torch.int8, device=DEV)
-    codes[:, : cx.shape[1]] = cx.to(DEV)
-    return ops.Int8Rows(codes, xs.to(DEV), cx.shape[1])
+    m, k = cx.shape
+    codes = torch.full((-(-m // 16) * 16, ops.int8_padded_k(k)), 113, dtype=torch.int8)
+    codes[:m, :k] = cx
+    rows = ops.Int8Rows.from_codes(codes.to(DEV), torch.ones(codes.shape[0], device=DEV))
+    return ops.Int8Rows(rows.data, xs.to(DEV), k)
 
 
 PRODUCTS = [(1, 1, 1), (1, 2048, 2048), (16, 33, 512), (17, 20, 513), (3, 500, 14336), (33, 130, 4096), (64, 1000, 1100), (65, 4096, 768), (128, 257, 2304), (129, 100, 1024),
@@ -145,6 +147,28 @@ def test_product(m, n, k, dtype):
     assert bool(((y.cpu().double() - want).abs() <= (3 * 2.0**-24 * 1.001 + ROUND[dtype]) * want.abs()).all())
     assert bool((room[m] == 7).all()) and bool((room[:, n:] == 7).all())
     assert torch.equal(ops.linear_int8(_rows(cx, xs), w, dtype=dtype), y)
+
+
+@pytest.mark.parametrize("form", range(6))
+@pytest.mark.parametrize("m,n,k,ranges", [(1, 4, 512, 1), (17, 65, 768, 1), (130, 260, 1280, 2), (300, 516, 2304, 4), (257, 130, 4096, 8), (520, 1027, 1024, 2), (1300, 400, 512, 1)])
+def test_product_in_every_tile(m, n, k, ranges, form):
+    """Tiles and ranges that the plan would not choose: the same whole numbers, times the scales, at sizes off every edge."""
+    import ctypes
+
+    from nanospec_amd.kernels import build
+
+    ops = _ops()
+    cx, xs, cw, ws = _operands(m, n, k, m + k)
+    w, x = ops.Int8Weight(cw.to(DEV), ws.to(DEV)), _rows(cx, xs)
+    out = torch.full((m + 1, n + 3), 7.0, device=DEV)
+    parts = torch.full((ranges * m * (n + 3),), -5, dtype=torch.int32, device=DEV)
+    i = ctypes.c_int
+    status = build.core().ns_gemm_int8_many(ops._ptr(out), ops._ptr(parts), ops._ptr(x.data), ops._ptr(x.scales), ops._ptr(w.data), ops._ptr(w.scales), i(m), i(n), i(w.kp), i(n + 3),
+                                            i(form), i(ranges), i(ops.F32), ops._stream())
+    assert status == 0
+    want = (cx.double() @ cw.double().T) * xs.double()[:, None] * ws.double()
+    assert bool(((out[:m, :n].cpu().double() - want).abs() <= 4 * 2.0**-24 * 1.001 * want.abs()).all())
+    assert bool((out[m] == 7).all()) and bool((out[:, n:] == 7).all())
 
 
 def test_product_of_the_largest_sums():
