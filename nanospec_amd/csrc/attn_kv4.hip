@@ -13,8 +13,9 @@ struct Kv4AttnParams {
   const void* q;    // row t at q + t * q_stride, head h at + h * hd
   const uint8_t* pool;
   const int *tiles, *token_req, *positions, *block_table;
-  int q_stride, table_stride, n_tiles, heads, kv_heads, hd, page, splits, window;
+  int q_stride, table_stride, n_tiles, heads, kv_heads, hd, page, splits, window, groups;  // groups: workgroups that share single tokens' keys
   float scale_log2;  // softmax scale * log2(e)
+  int wide;          // every query begins at a multiple of 16 bytes
 };
 
 // ------------------------------------------------------------------------------------------------------------------------------------
@@ -123,13 +124,34 @@ __global__ __launch_bounds__(64) void attn_kv4_join_kernel(const Kv4AttnParams a
     if (token >= info[3]) return;
     row = info[2] + token;
   }
+  const float* from = a.part_o + col * a.splits * a.hd;
+  // the first eight results are asked for before it is known which count
+  float x[4][8];
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+#pragma unroll
+    for (int s = 0; s < 8; ++s) x[i][s] = lane + 64 * i < a.hd && s < a.splits ? from[(size_t)s * a.hd + lane + 64 * i] : 0.f;
   const float ls = lane < a.splits ? a.part_l[col * a.splits + lane] : -INFINITY;
+  // (results are there from the first on; where there is none the row has been written whole)
+  const int used = __popcll(__ballot(ls != -INFINITY));
+  if (used == 0) return;
   const float top = wave_max(ls), base = top == -INFINITY ? 0.f : top;
   const float weight = exp2f(ls - base), total = wave_sum(weight);
-  for (int c = lane; c < a.hd; c += NS_WAVE) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int c = lane + 64 * i;
+    if (64 * i >= a.hd) break;
     float o = 0.f;
-    for (int s = 0; s < a.splits; ++s) o += a.part_o[(col * a.splits + s) * a.hd + c] * __shfl(weight, s, NS_WAVE);
-    ((T*)a.out)[(row * a.heads + head) * a.hd + c] = from_f<T>(o / total);
+#pragma unroll
+    for (int s = 0; s < 8; ++s) o += s < used ? x[i][s] * __shfl(weight, s, NS_WAVE) : 0.f;
+    for (int s0 = 8; s0 < used; s0 += 8) {  // eight results' loads on their way at a time
+      float more[8];
+#pragma unroll
+      for (int s = 0; s < 8; ++s) more[s] = c < a.hd ? from[(size_t)min(s0 + s, used - 1) * a.hd + c] : 0.f;
+#pragma unroll
+      for (int s = 0; s < 8; ++s) o += s0 + s < used ? more[s] * __shfl(weight, (s0 + s) & 63, NS_WAVE) : 0.f;
+    }
+    if (c < a.hd) ((T*)a.out)[(row * a.heads + head) * a.hd + c] = from_f<T>(o / total);
   }
 }
 
@@ -153,7 +175,7 @@ extern "C" int ns_attn_kv4_plain(void* out, void* part_o, void* part_l, const vo
   if (splits < 1 || splits > 64 || (splits > 1 && (!part_o || !part_l)) || (long long)tokens * heads > 0x7fffffff) return NS_ERR_BAD_ARG;
   if (tokens == 0) return NS_OK;
   const Kv4AttnParams a{out, (float*)part_o, (float*)part_l, q, (const uint8_t*)pool, nullptr, token_req, positions, block_table, q_stride, table_stride, 0, heads, kv_heads,
-                        hd, page, splits, window, scale * 1.4426950408889634f};
+                        hd, page, splits, window, 0, scale * 1.4426950408889634f, 0};
   if (dtype == NS_DTYPE_F32)
     launch_plain<float>(a, tokens, stream);
   else if (dtype == NS_DTYPE_BF16)
@@ -166,22 +188,19 @@ extern "C" int ns_attn_kv4_plain(void* out, void* part_o, void* part_l, const vo
 #include "attn_kv4_mfma.h"
 
 template <typename T, int HD, int PARTS>
-static int launch_tiles(const Kv4AttnParams& a, int rows, hipStream_t stream) {
+static int launch_tiles(const Kv4AttnParams& a, int rows, int wave_tokens, hipStream_t stream) {
   const int group = a.heads / a.kv_heads;
   if (rows) {
-    const long long items = (long long)a.n_tiles * a.kv_heads * ((group + 15) / 16);
-    if (items > 0x7fffffff) return NS_ERR_UNSUPPORTED;
-    attn_kv4_rows_kernel<T, HD, PARTS><<<dim3((unsigned)items, (unsigned)a.splits), 256, 0, stream>>>(a);
+    if (a.n_tiles > 65535) return NS_ERR_UNSUPPORTED;
+    attn_kv4_rows_kernel<T, HD, PARTS><<<dim3((unsigned)(a.kv_heads * ((group + 15) / 16)), (unsigned)a.n_tiles, (unsigned)a.splits), KV4_ROW_WAVES * NS_WAVE, 0, stream>>>(a);
   } else {
-    // two heads of a group share a wave's keys where there are two
-    const int heads = group > 1 ? 2 : 1;
-    const long long items = (long long)a.n_tiles * a.splits * a.kv_heads * ((group + heads - 1) / heads);
-    if (items > 0x7fffffff) return NS_ERR_UNSUPPORTED;
+    const long long items = (long long)a.n_tiles * a.splits * a.heads * (KV4_TILE_TOKENS / wave_tokens);
+    if (items > 0x7fffffff - 4) return NS_ERR_UNSUPPORTED;
     const unsigned grid = (unsigned)((items + 3) / 4);
-    if (heads == 2)
-      attn_kv4_tiles_kernel<T, HD, 4, PARTS><<<grid, 256, 0, stream>>>(a);
-    else
-      attn_kv4_tiles_kernel<T, HD, 2, PARTS><<<grid, 256, 0, stream>>>(a);
+    if constexpr (PARTS == 1) {
+      if (wave_tokens == 32) attn_kv4_tiles_kernel<T, HD, 2, PARTS><<<grid, 256, 0, stream>>>(a);
+    }
+    if (wave_tokens == 16) attn_kv4_tiles_kernel<T, HD, 1, PARTS><<<grid, 256, 0, stream>>>(a);
   }
   if (a.splits > 1) {
     const long long cols = (long long)a.n_tiles * (rows ? 1 : KV4_TILE_TOKENS) * a.heads;
@@ -192,18 +211,20 @@ static int launch_tiles(const Kv4AttnParams& a, int rows, hipStream_t stream) {
 }
 
 // Attention of the tokens that ``tiles`` [n_tiles][8] names: request, first token of the tile among the request's tokens of this step, row of the request's first token, tokens of the
-// request in this step, keys after it, three more.  rows 1: a tile is one token; 0: up to 32.  part_o: float32 [n_tiles * tokens of a tile * heads * splits * hd] and part_l
+// request in this step, keys after it, one more, of single tokens the blocks of 32 keys of all of them, one more.  rows 1: a tile is one token; 0: up to 32, of which a wave takes wave_tokens (16; with bfloat16 also 32).  part_o: float32 [n_tiles * tokens of a tile * heads * splits * hd] and part_l
 // [n_tiles * tokens of a tile * heads * splits] with splits > 1.
 extern "C" int ns_attn_kv4(void* out, void* part_o, void* part_l, const void* q, int q_stride, const void* pool, const int* tiles, const int* block_table, int table_stride,
-                           int n_tiles, int heads, int kv_heads, int hd, int page, int rows, int splits, int window, float scale, int dtype, hipStream_t stream) {
+                           int n_tiles, int heads, int kv_heads, int hd, int page, int rows, int wave_tokens, int splits, int groups, int window, float scale, int dtype, hipStream_t stream) {
   if (n_tiles < 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads || page < KV4_TOKENS || (page & (page - 1)) || window < 0) return NS_ERR_BAD_ARG;
-  if (splits < 1 || splits > 64 || (splits > 1 && (!part_o || !part_l))) return NS_ERR_BAD_ARG;
+  if (splits < 1 || splits > 64 || (splits > 1 && (!part_o || !part_l)) || groups < 1) return NS_ERR_BAD_ARG;
+  if (!rows && wave_tokens != 16 && (wave_tokens != 32 || dtype == NS_DTYPE_F32)) return NS_ERR_BAD_ARG;
   if (hd != 64 && hd != 128) return NS_ERR_UNSUPPORTED;
   if ((((uintptr_t)out | (uintptr_t)pool | (uintptr_t)part_o) & 15) != 0) return NS_ERR_UNSUPPORTED;
   if (n_tiles == 0) return NS_OK;
   const Kv4AttnParams a{out, (float*)part_o, (float*)part_l, q, (const uint8_t*)pool, tiles, nullptr, nullptr, block_table, q_stride, table_stride, n_tiles, heads, kv_heads,
-                        hd, page, splits, window, scale * 1.4426950408889634f};
-  if (dtype == NS_DTYPE_F32) return hd == 64 ? launch_tiles<float, 64, 2>(a, rows, stream) : launch_tiles<float, 128, 2>(a, rows, stream);
-  if (dtype == NS_DTYPE_BF16) return hd == 64 ? launch_tiles<bf16_t, 64, 1>(a, rows, stream) : launch_tiles<bf16_t, 128, 1>(a, rows, stream);
+                        hd, page, splits, window, groups, scale * 1.4426950408889634f,
+                        ((uintptr_t)q & 15) == 0 && q_stride % (dtype == NS_DTYPE_F32 ? 4 : 8) == 0};
+  if (dtype == NS_DTYPE_F32) return hd == 64 ? launch_tiles<float, 64, 2>(a, rows, wave_tokens, stream) : launch_tiles<float, 128, 2>(a, rows, wave_tokens, stream);
+  if (dtype == NS_DTYPE_BF16) return hd == 64 ? launch_tiles<bf16_t, 64, 1>(a, rows, wave_tokens, stream) : launch_tiles<bf16_t, 128, 1>(a, rows, wave_tokens, stream);
   return NS_ERR_UNSUPPORTED;
 }

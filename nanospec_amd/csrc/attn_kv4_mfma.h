@@ -7,12 +7,11 @@
 // the 32, so that lane (col, t) holds the weights of keys 8 t .. 8 t + 7, one octet, whose values and marks it reads in whole records.
 // Nothing passes through LDS on the way (a wave's operands are 4.25 bits a value, from L2): the waves need no barriers.
 //
-// From codes to operands.  Float16 of 1,024 + u has u in its lowest four bits, and of 1,024 + 16 u in the next four: a mask and an or make two
-// codes at a time, and the queries' channels at the second kind of place carry a factor of 1/16, exactly.  The 1,024s are taken off in the first
-// sum: it starts at -1,024 times the sum of the queries.  That rounds at 2^-24 of 1,024 |q|, 2^-14 of a step of the key, less than bfloat16
-// queries hold; float32 (PARTS 2) and the values, whose sums over many keys that may cancel, take it off before (codes of -8 .. 7, exactly).
+// From codes to operands.  A code in the lowest four bits of a float16, all others zero, is that many 2^-24, a number below the normal range, which the matrix instruction multiplies
+// exactly (in the next four bits: times 16).  A mask makes two codes of a dword operands, and nothing has to be taken off: the products are 2^-24 (2^-20) times the sums of whole
+// numbers that are meant.  The queries' channels that meet codes times 16 carry a factor of 1/16, exactly; the outputs' channels that do are multiplied by it at the end.
 //   s = step (q . u) + low sum(q):      two operations a score, as both are a key's
-//   out = sum p step (u - 8) + sum p (low + 8 step):   p step is the weight in the second product, the rest a sum of numbers
+//   out = sum p step u + sum p low:     p step is the weight in the second product, the rest a sum of numbers
 // Queries are float16 on their way in, scaled by a power of two of their own so that the largest lies at 256: what is 2^-22 of it is exact.  Weights are
 // rounded to float16 (2^-12 of themselves).  PARTS 2: queries and weights as the sum of two float16 values each, two products for one.
 //
@@ -30,22 +29,13 @@ typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 #define KV4_TILE_INTS 8
 #define KV4_TILE_TOKENS 32  // of a portion's tile
 #define KV4_SLACK 8.f
+#define KV4_ROW_WAVES 4
+#define KV4_RANGE_BLOCKS 8  // of 32 keys: the fewest of a range of a single token's keys
 
 __device__ __forceinline__ f16x8 as_f16x8(uint32_t a, uint32_t b, uint32_t c, uint32_t d) { return __builtin_bit_cast(f16x8, u32x4{a, b, c, d}); }
-// two codes of a dword as 1,024 + u, and as 1,024 + 16 u
-// (one instruction: the compiler makes two of it, as an instruction may name one constant only, and the other has to be in a register of its own)
-__device__ __forceinline__ uint32_t and_or(uint32_t w, uint32_t mask, uint32_t set) {
-  uint32_t r;
-  asm("v_and_or_b32 %0, %1, %2, %3" : "=v"(r) : "v"(w), "s"(mask), "v"(set));
-  return r;
-}
-__device__ __forceinline__ uint32_t kv4_ones(uint32_t w) { return and_or(w, 0x000f000fu, 0x64006400u); }
-__device__ __forceinline__ uint32_t kv4_sixteens(uint32_t w) { return and_or(w, 0x00f000f0u, 0x64006400u); }
-// the same less 1,024 and 8 (128): u - 8, 16 (u - 8)
-__device__ __forceinline__ uint32_t kv4_centred(uint32_t w, bool sixteens) {
-  const _Float16 off = sixteens ? (_Float16)-1152.f : (_Float16)-1032.f;
-  return __builtin_bit_cast(uint32_t, __builtin_bit_cast(f16x2, w) + f16x2{off, off});
-}
+// two codes of a dword as 2^-24 u, and as 2^-20 u
+__device__ __forceinline__ uint32_t kv4_ones(uint32_t w) { return w & 0x000f000fu; }
+__device__ __forceinline__ uint32_t kv4_sixteens(uint32_t w) { return w & 0x00f000f0u; }
 __device__ __forceinline__ float quarters_max(float v) {
   v = fmaxf(v, __shfl_xor(v, 16, NS_WAVE));
   return fmaxf(v, __shfl_xor(v, 32, NS_WAVE));
@@ -69,7 +59,7 @@ struct Kv4Wave {
   static constexpr int NG = HD / 32, NB = HD / 64;
   static constexpr int REC = 8 * HD + 64;
   f16x8 q[CT][PARTS][NG];
-  float qsum[CT], unscale[CT];  // sum of the scaled queries; scale * log2(e) and the queries' own scale taken off
+  float qsum[CT], unscale[CT];  // sum of the scaled queries, times 2^-24 as the products are; what a score is multiplied with: the scale, log2(e), the queries' own scale and the 2^-24 taken off
   float R[CT], l[CT], z[CT];
   f32x4v o[CT][NB][4];
   int lane, col, t;
@@ -87,22 +77,41 @@ struct Kv4Wave {
     }
   }
 
-  // this lane's column of tile c: its query's channels (nullptr: a column of zeros)
-  __device__ __forceinline__ void query(int c, const T* from, float scale_log2) {
+  // this lane's column of tile c: its query's channels (nullptr: a column of zeros).  ``wide``: they lie at a multiple of 16 bytes.
+  __device__ __forceinline__ void query(int c, const T* from, float scale_log2, bool wide) {
     float x[NG][8], most = 0.f;
+    if (!from) {
+#pragma unroll
+      for (int g = 0; g < NG; ++g)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[g][e] = 0.f;
+    } else if (wide) {
+      constexpr int V = 16 / sizeof(T);
+      typedef T vec_t __attribute__((ext_vector_type(V)));
+#pragma unroll
+      for (int g = 0; g < NG; ++g)
+#pragma unroll
+        for (int i = 0; i < 8 / V; ++i) {
+          const vec_t v = *reinterpret_cast<const vec_t*>(from + 32 * g + 8 * t + V * i);
+#pragma unroll
+          for (int e = 0; e < V; ++e) x[g][V * i + e] = to_f((T)v[e]);
+        }
+    } else {
+#pragma unroll
+      for (int g = 0; g < NG; ++g)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[g][e] = to_f(from[32 * g + 8 * t + e]);
+    }
 #pragma unroll
     for (int g = 0; g < NG; ++g)
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        x[g][e] = from ? to_f(from[32 * g + 8 * t + e]) : 0.f;
-        most = fmaxf(most, fabsf(x[g][e]));
-      }
+      for (int e = 0; e < 8; ++e) most = fmaxf(most, fabsf(x[g][e]));
     most = quarters_max(most);
     // 2^(8 - exponent): exact; nothing to scale in zeros and where the largest is infinite (the products are then no numbers by themselves)
     const int ex = (int)(__float_as_uint(most) >> 23);
     const int up = ex == 0 || ex == 255 ? 127 : min(max(127 + 127 + 8 - ex, 1), 254);
     const float by = __uint_as_float((uint32_t)up << 23);
-    unscale[c] = scale_log2 * __uint_as_float((uint32_t)max(1, 254 - up) << 23);
+    unscale[c] = scale_log2 * 0x1p24f * __uint_as_float((uint32_t)max(1, 254 - up) << 23);
     float sum = 0.f;
 #pragma unroll
     for (int g = 0; g < NG; ++g) {
@@ -113,38 +122,40 @@ struct Kv4Wave {
         const float y = x[g][e] * by, s = e & 2 ? y * 0.0625f : y;
         hi[e] = (_Float16)s;
         lo[e] = (_Float16)(s - (float)hi[e]);
-        // what is taken off, and what a lowest value meets, are the queries as they are multiplied
+        // what a lowest value meets are the queries as they are multiplied
         sum += PARTS == 1 ? (e & 2 ? 16.f * (float)hi[e] : (float)hi[e]) : y;
       }
       q[c][0][g] = hi;
       if constexpr (PARTS == 2) q[c][1][g] = lo;
     }
-    qsum[c] = quarters_sum(sum);
-  }
-  // -1,024 times the sum of what the first product multiplies (channels with a factor of 1/16 count as such)
-  __device__ __forceinline__ float start(int c) const {
-    float s = 0.f;
-#pragma unroll
-    for (int g = 0; g < NG; ++g)
-#pragma unroll
-      for (int e = 0; e < 8; ++e) s += (float)q[c][0][g][e];
-    return -1024.f * quarters_sum(s);
+    qsum[c] = quarters_sum(sum) * 0x1p-24f;
   }
 
-  // records of the octet of this lane's key (a row of the first product) and of its octet of values, of the 32 keys from ``k0`` on
+  // The records of a block's four octets, in records from the pool's start, found through the scalar unit; a lane picks those of the octet of its key (a row of the first product) and of
+  // its octet of values.  Octets outside low .. high are their neighbours: nobody sees those keys, and they may have no page.
+  struct Octets {
+    int r[4];
+  };
   struct At {
     const uint8_t *k, *v;
   };
-  // ``low``, ``high``: the first and the last octet that may be read (outside them their neighbours are: nobody sees those keys)
-  __device__ __forceinline__ void pages_of(int k0, int low, int high, const int* table, int shift, int& pk, int& pv) const {
-    const int ok = min(max(k0 / 8 + col / 4, low), high), ov = min(max(k0 / 8 + t, low), high);
-    pk = table[ok >> shift];
-    pv = table[ov >> shift];
+  __device__ __forceinline__ Octets octets(int block, int low, int high, const int* table, int kv_heads, int kvh, int shift) const {
+    typedef const __attribute__((address_space(4))) int* scalar_ints;  // (this kernel does not write the table)
+    const scalar_ints ids = (scalar_ints)(unsigned long long)table;
+    Octets o;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int oct = min(max(4 * block + j, low), high);
+      o.r[j] = ((ids[oct >> shift] * kv_heads + kvh) << shift) | (oct & ((1 << shift) - 1));
+    }
+    return o;
   }
-  __device__ __forceinline__ At at(int k0, int low, int high, int pk, int pv, const uint8_t* pool, int kv_heads, int kvh, int shift) const {
-    const int ok = min(max(k0 / 8 + col / 4, low), high), ov = min(max(k0 / 8 + t, low), high), mask = (1 << shift) - 1;
-    return {pool + ((((size_t)pk * kv_heads + kvh) << shift) + (ok & mask)) * REC + (col % 4) * (HD / 2) + t * (HD / 8),
-            pool + ((((size_t)pv * kv_heads + kvh) << shift) + (ov & mask)) * REC};
+  static __device__ __forceinline__ int pick(const Octets& o, int j) {
+    const int a = j & 1 ? o.r[1] : o.r[0], b = j & 1 ? o.r[3] : o.r[2];
+    return j & 2 ? b : a;
+  }
+  __device__ __forceinline__ At at(const Octets& o, const uint8_t* pool) const {
+    return {pool + (uint32_t)pick(o, col / 4) * (uint64_t)REC + ((col % 4) * (HD / 2) + t * (HD / 8)), pool + (uint32_t)pick(o, t) * (uint64_t)REC};
   }
   __device__ __forceinline__ void load_keys(Kv4Block<HD>& b, const At& p) const {
 #pragma unroll
@@ -169,7 +180,7 @@ struct Kv4Wave {
 
   // The 32 keys from k0 on.  ``mask``: some column may not see all of them.  What has been used of the block is loaded anew, from ``then``, at once: a load has most
   // of a block's time to arrive, and there is one set of registers for them.
-  __device__ __forceinline__ void block(Kv4Block<HD>& b, int k0, bool mask, const float* cinit, const At& then) {
+  __device__ __forceinline__ void block(Kv4Block<HD>& b, int k0, bool mask, const At& then) {
     // keys as operands
     f16x8 ka[2][NG];
 #pragma unroll
@@ -177,23 +188,21 @@ struct Kv4Wave {
 #pragma unroll
       for (int g = 0; g < NG; ++g) {
         const uint32_t w = b.k[a][g], w8 = w >> 8;
-        uint32_t r0 = kv4_ones(w), r1 = kv4_sixteens(w), r2 = kv4_ones(w8), r3 = kv4_sixteens(w8);
-        if constexpr (PARTS == 2) r0 = kv4_centred(r0, false), r1 = kv4_centred(r1, true), r2 = kv4_centred(r2, false), r3 = kv4_centred(r3, true);
-        ka[a][g] = as_f16x8(r0, r1, r2, r3);
+        ka[a][g] = as_f16x8(kv4_ones(w), kv4_sixteens(w), kv4_ones(w8), kv4_sixteens(w8));
       }
     load_keys(b, then);
     __builtin_amdgcn_sched_barrier(0);
     f16x8 p[CT][PARTS];
-    float k_step[8], k_low[8], v_step[8], v_mid[8];
+    float k_step[8], k_low[8], v_step[8], v_low[8];
     uint32_t v_mark[8], most_of = 0;
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
       const uint32_t km = b.km[e / 4][e % 4], vm = b.vm[e / 4][e % 4];
       k_step[e] = kv4_step(km);
-      k_low[e] = PARTS == 1 ? kv4_low(km) : fmaf(8.f, k_step[e], kv4_low(km));
+      k_low[e] = kv4_low(km);
       v_mark[e] = vm;
       v_step[e] = kv4_step(vm);
-      v_mid[e] = fmaf(8.f, v_step[e], kv4_low(vm));
+      v_low[e] = kv4_low(vm);
       most_of = max(most_of, vm);
     }
     load_marks(b.km, then, 0);
@@ -203,8 +212,7 @@ struct Kv4Wave {
       f32x4v d[2];
 #pragma unroll
       for (int a = 0; a < 2; ++a) {
-        const float from = PARTS == 1 ? cinit[c] : 0.f;
-        d[a] = f32x4v{from, from, from, from};
+        d[a] = f32x4v{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int g = 0; g < NG; ++g)
 #pragma unroll
@@ -213,7 +221,7 @@ struct Kv4Wave {
       float s[8], top = -INFINITY;
       uint32_t most = most_of;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) s[e] = fmaf(k_step[e], d[e / 4][e % 4], k_low[e] * qsum[c]) * unscale[c];
+      for (int e = 0; e < 8; ++e) s[e] = fmaf(k_step[e], d[e / 4][e % 4], k_low[e] * qsum[c]);
       if (mask) {
         most = 0;
 #pragma unroll
@@ -227,7 +235,7 @@ struct Kv4Wave {
 #pragma unroll
       for (int e = 0; e < 8; ++e) top = fmaxf(top, s[e]);
       // the exponent above the largest step, at least -64 (smaller ones lose what float16 does not hold of them)
-      const float reach = top + fmaxf((float)(int)(most >> 23) - 126.f, -64.f);
+      const float reach = top * unscale[c] + fmaxf((float)(int)(most >> 23) - 126.f, -64.f);
       if (__any(reach > R[c] + KV4_SLACK)) {
         const float want = quarters_max(reach), next = want > R[c] + KV4_SLACK ? want : R[c], base = next == -INFINITY ? 0.f : next;
         const float shrink = __builtin_amdgcn_exp2f(R[c] - base);
@@ -243,15 +251,15 @@ struct Kv4Wave {
       float w[8];
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        w[e] = __builtin_amdgcn_exp2f(s[e] - base);
+        w[e] = __builtin_amdgcn_exp2f(fmaf(s[e], unscale[c], -base));
         l[c] += w[e];
       }
       if (mask) {  // (what a column does not see may be no number)
 #pragma unroll
-        for (int e = 0; e < 8; ++e) z[c] += s[e] != -INFINITY ? w[e] * v_mid[e] : 0.f;
+        for (int e = 0; e < 8; ++e) z[c] += s[e] != -INFINITY ? w[e] * v_low[e] : 0.f;
       } else {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) z[c] = fmaf(w[e], v_mid[e], z[c]);
+        for (int e = 0; e < 8; ++e) z[c] = fmaf(w[e], v_low[e], z[c]);
       }
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
@@ -271,7 +279,7 @@ struct Kv4Wave {
 #pragma unroll
         for (int x = 0; x < 4; ++x) {
           const uint32_t y = i >= 2 ? w[x] >> 8 : w[x];
-          r[x] = kv4_centred(i & 1 ? kv4_sixteens(y) : kv4_ones(y), i & 1);
+          r[x] = i & 1 ? kv4_sixteens(y) : kv4_ones(y);
         }
         const f16x8 va = as_f16x8(r[0], r[1], r[2], r[3]);
 #pragma unroll
@@ -288,19 +296,14 @@ struct Kv4Wave {
   __device__ __forceinline__ void walk(int b0, int b1, int by, int whole0, int whole1, int low, int high, const int* table, const uint8_t* pool, int kv_heads, int kvh,
                                        int shift) {
     if (b0 >= b1) return;
-    float cinit[CT];
-#pragma unroll
-    for (int c = 0; c < CT; ++c) cinit[c] = PARTS == 1 ? start(c) : 0.f;
-    Kv4Block<HD> now;
-    int pk, pv;
-    pages_of(32 * b0, low, high, table, shift, pk, pv);
-    const At first = at(32 * b0, low, high, pk, pv, pool, kv_heads, kvh, shift);
-    pages_of(32 * (b0 + by), low, high, table, shift, pk, pv);
-    load_keys(now, first), load_marks(now.km, first, 0), load_marks(now.vm, first, 1), load_values(now, first);
+    Kv4Block<HD> held;
+    const At to = at(octets(b0, low, high, table, kv_heads, kvh, shift), pool);
+    load_keys(held, to), load_marks(held.km, to, 0), load_marks(held.vm, to, 1), load_values(held, to);
+    Octets next = octets(b0 + by, low, high, table, kv_heads, kvh, shift);  // (ids a block ahead of the loads)
     for (int b = b0; b < b1; b += by) {
-      const At then = at(32 * (b + by), low, high, pk, pv, pool, kv_heads, kvh, shift);
-      pages_of(32 * (b + 2 * by), low, high, table, shift, pk, pv);
-      block(now, 32 * b, b < whole0 || b >= whole1, cinit, then);
+      const At then = at(next, pool);
+      next = octets(b + 2 * by, low, high, table, kv_heads, kvh, shift);
+      block(held, 32 * b, b < whole0 || b >= whole1, then);
     }
   }
 
@@ -310,78 +313,108 @@ struct Kv4Wave {
     low = quarters_sum(z[c]);
     return total == 0.f ? -INFINITY : R[c] + __log2f(total);
   }
-  __device__ __forceinline__ float sum_of(int c, int n, int e) const { return (e & 1 ? 0.0625f : 1.f) * o[c][n][e % 4][e / 4]; }
+  __device__ __forceinline__ float sum_of(int c, int n, int e) const { return (e & 1 ? 0x1p20f : 0x1p24f) * o[c][n][e % 4][e / 4]; }
 };
 
-// Single tokens: a workgroup a (token, key/value head, 16 query heads of its group, range of keys), whose four waves take blocks of 32 keys in turn and meet in LDS.
+// Single tokens: a workgroup a (token, key/value head, 16 query heads of its group, range of keys), whose waves take blocks of 32 keys in turn and meet in LDS.  Ranges are even and as many
+// as give ``a.groups`` workgroups over all tokens: a row twice as long as others has twice as many.
+// Bound by memory where the rows are long and many (61 rows of 200 to 12,000 keys, 8 key/value heads of 128 channels: 94 us, 4.2 TB/s; 64 rows of 6,000: 5.3), by one workgroup's
+// chain of loads where they are few (a row of 1,100: 8.7 us).  Two blocks on their way at a time were slower everywhere (their registers cost a wave a SIMD), eight waves a workgroup too but
+// for eight (row, head)s of 32,000 keys (19 for 24 us).
 template <typename T, int HD, int PARTS>
-__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(PARTS == 2 ? 2 : 3))) void attn_kv4_rows_kernel(const Kv4AttnParams a) {
+__global__ __launch_bounds__(KV4_ROW_WAVES * 64) __attribute__((amdgpu_waves_per_eu(2))) void attn_kv4_rows_kernel(const Kv4AttnParams a) {
   typedef Kv4Wave<T, HD, 1, PARTS> Wave;
-  __shared__ float outs[4][16][HD + 4];
-  __shared__ float weights[4][16];
+  constexpr int WAVES = KV4_ROW_WAVES;
+  __shared__ float outs[WAVES][16][HD + 4];
+  __shared__ float weights[WAVES][16];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / NS_WAVE);
   const int group = a.heads / a.kv_heads, hblks = (group + 15) / 16, ny = a.kv_heads * hblks;
-  const int y = blockIdx.x % ny, tile = blockIdx.x / ny, split = blockIdx.y, kvh = y / hblks, head0 = kvh * group + y % hblks * 16;
+  const int y = blockIdx.x, tile = blockIdx.y, split = blockIdx.z, kvh = hblks == 1 ? y : y / hblks, head0 = kvh * group + (y - kvh * hblks) * 16;
   const int heads = min(16, (kvh + 1) * group - head0);
   const int* info = a.tiles + (size_t)tile * KV4_TILE_INTS;
-  const int req = info[0], t0 = info[1], row = info[2] + t0, n = info[3], kv = info[4];
+  const int req = info[0], t0 = info[1], row = info[2] + t0, n = info[3], kv = info[4], all = info[6];
   if (t0 >= n) return;
   const int pos = kv - n + t0, first = a.window ? max(0, pos - a.window + 1) : 0, shift = 31 - __clz(a.page) - 3;
-  const int b0 = first / 32, blocks = pos / 32 + 1 - b0, share = (blocks + a.splits - 1) / a.splits;
+  const int b0 = first / 32, blocks = pos / 32 + 1 - b0;
+  // (quotients by reciprocals: a share that is one block too long does no harm, and the same for all of a row's ranges)
+  const float every = (float)ny * (a.window ? fminf((float)all, (float)a.n_tiles * (float)(a.window / 32 + 2)) : (float)all);
+  const float wanted = fmaxf((float)KV4_RANGE_BLOCKS, every * __builtin_amdgcn_rcpf((float)a.groups)), ranges = fminf((float)a.splits, ceilf((float)blocks * __builtin_amdgcn_rcpf(wanted)));
+  const int share = __builtin_amdgcn_readfirstlane((int)((float)blocks * __builtin_amdgcn_rcpf(fmaxf(ranges, 1.f))) + 1);
+  if (split * share >= blocks) {
+    if ((int)threadIdx.x < heads) a.part_l[((size_t)tile * a.heads + head0 + threadIdx.x) * a.splits + split] = -INFINITY;
+    return;
+  }
+  const bool whole = share >= blocks;
   const int from = b0 + split * share, to = min(b0 + blocks, from + share);
   Wave w;
   w.init();
   w.kpos[0] = pos, w.kfirst[0] = first;
-  w.query(0, w.col < heads ? (const T*)a.q + (size_t)row * a.q_stride + (head0 + w.col) * HD : nullptr, a.scale_log2);
-  w.walk(from + wave, to, 4, (first + 31) / 32, (pos + 1) / 32, first / 8, pos / 8, a.block_table + (size_t)req * a.table_stride, a.pool, a.kv_heads, kvh, shift);
+  w.query(0, w.col < heads ? (const T*)a.q + (size_t)row * a.q_stride + (head0 + w.col) * HD : nullptr, a.scale_log2, a.wide);
+  w.walk(from + wave, to, WAVES, (first + 31) / 32, (pos + 1) / 32, first / 8, pos / 8, a.block_table + (size_t)req * a.table_stride, a.pool, a.kv_heads, kvh, shift);
   float total, low;
   const float weight = w.weight(0, total, low), inv = total == 0.f ? 0.f : 1.f / total;
   if (w.t == 0) weights[wave][w.col] = weight;
+  if (w.col < heads) {
 #pragma unroll
-  for (int nb = 0; nb < Wave::NB; ++nb)
+    for (int nb = 0; nb < Wave::NB; ++nb)
 #pragma unroll
-    for (int e = 0; e < 16; ++e) outs[wave][w.col][64 * nb + 16 * w.t + e] = (w.sum_of(0, nb, e) + low) * inv;
+      for (int e = 0; e < 16; e += 4) {
+        f32x4v x;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[i] = (w.sum_of(0, nb, e + i) + low) * inv;
+        *reinterpret_cast<f32x4v*>(&outs[wave][w.col][64 * nb + 16 * w.t + e]) = x;
+      }
+  }
   __syncthreads();
-  for (int i = threadIdx.x; i < heads * HD; i += 256) {
-    const int c = i / HD, ch = i % HD;
+  const size_t pc0 = ((size_t)tile * a.heads + head0) * a.splits;
+  for (int i = threadIdx.x; i < heads * (HD / 4); i += WAVES * 64) {
+    const int c = i / (HD / 4), ch = i % (HD / 4) * 4;
     float top = -INFINITY;
 #pragma unroll
-    for (int v = 0; v < 4; ++v) top = fmaxf(top, weights[v][c]);
+    for (int v = 0; v < WAVES; ++v) top = fmaxf(top, weights[v][c]);
     const float base = top == -INFINITY ? 0.f : top;
-    float sum = 0.f, all = 0.f;
+    f32x4v sum = {0.f, 0.f, 0.f, 0.f};
+    float every_weight = 0.f;
 #pragma unroll
-    for (int v = 0; v < 4; ++v) {
-      const float x = exp2f(weights[v][c] - base);
-      all += x;
-      sum += x == 0.f ? 0.f : x * outs[v][c][ch];
+    for (int v = 0; v < WAVES; ++v) {
+      const float x = __builtin_amdgcn_exp2f(weights[v][c] - base);
+      every_weight += x;
+      if (x != 0.f) sum += x * *reinterpret_cast<const f32x4v*>(&outs[v][c][ch]);
     }
-    const float r = all == 0.f ? 0.f : sum / all;
-    if (a.splits == 1) {
-      ((T*)a.out)[((size_t)row * a.heads + head0 + c) * HD + ch] = from_f<T>(r);
+    const float by = every_weight == 0.f ? 0.f : 1.f / every_weight;
+    const size_t pc = pc0 + (size_t)c * a.splits + split;
+    if (whole) {
+      typedef T vec_t __attribute__((ext_vector_type(4)));
+      vec_t r;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) r[e] = from_f<T>(sum[e] * by);
+      *reinterpret_cast<vec_t*>((T*)a.out + ((size_t)row * a.heads + head0 + c) * HD + ch) = r;
+      if (a.splits > 1 && ch == 0) a.part_l[pc] = -INFINITY;  // (the second kernel finds nothing to join and leaves the row alone)
     } else {
-      const size_t pc = ((size_t)tile * a.heads + head0 + c) * a.splits + split;
-      a.part_o[pc * HD + ch] = r;
-      if (ch == 0) a.part_l[pc] = all == 0.f ? -INFINITY : base + log2f(all);
+      *reinterpret_cast<f32x4v*>(a.part_o + pc * HD + ch) = sum * by;
+      if (ch == 0) a.part_l[pc] = every_weight == 0.f ? -INFINITY : base + __log2f(every_weight);
     }
   }
 }
 
-// Portions: a wave 32 tokens of CT / 2 heads of a group, four waves a workgroup that share nothing but their place.
+// Portions: a wave 16 CT tokens of a head, four waves a workgroup that share nothing but their place.
+// Bound by vector instructions: a block of 32 keys and 32 columns of 128 channels has 32 matrix instructions (512 cycles) and about 290 others (1,350), of which 112 make operands of the
+// codes and 16 are exponentials.  2,048 tokens at 16,000 keys: 776 us, 736 TFLOP/s; 2,048 at none 69 us.  Four tiles of columns a wave (each operand made for twice as many) leave one wave a
+// SIMD and nothing to fill its waits: 1,203 and 149 us.
 template <typename T, int HD, int CT, int PARTS>
-__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(CT == 2 && !(PARTS == 2 && HD == 128) ? 2 : 1))) void attn_kv4_tiles_kernel(const Kv4AttnParams a) {
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void attn_kv4_tiles_kernel(const Kv4AttnParams a) {
   typedef Kv4Wave<T, HD, CT, PARTS> Wave;
-  constexpr int HEADS = CT / 2;
+  constexpr int TOKENS = 16 * CT, PIECES = KV4_TILE_TOKENS / TOKENS;  // of a wave; of a tile
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / NS_WAVE);
-  const int group = a.heads / a.kv_heads, hblks = (group + HEADS - 1) / HEADS, ny = a.kv_heads * hblks;
   // (late tiles see the most keys: they begin first)
-  const long long item = (long long)blockIdx.x * 4 + wave, per = (long long)ny * a.splits;
-  const int tile = a.n_tiles - 1 - (int)(item / per), rest = (int)(item % per), split = rest / ny, y = rest % ny;
+  const int item = blockIdx.x * 4 + wave, columns = a.heads * PIECES, tile = a.n_tiles - 1 - item / (columns * a.splits), rest = item % (columns * a.splits);
+  const int split = rest / columns, head = rest % columns / PIECES, piece = rest % PIECES;
   if (tile < 0) return;
-  const int kvh = y / hblks, head0 = kvh * group + y % hblks * HEADS, heads = min(HEADS, (kvh + 1) * group - head0);
+  const int kvh = head / (a.heads / a.kv_heads);
   const int* info = a.tiles + (size_t)tile * KV4_TILE_INTS;
-  const int req = info[0], t0 = info[1], row0 = info[2], n = info[3], kv = info[4];
+  const int req = info[0], t0 = info[1] + piece * TOKENS, row0 = info[2], n = info[3], kv = info[4];
   if (t0 >= n) return;
-  const int tokens = min(KV4_TILE_TOKENS, n - t0), pos0 = kv - n + t0, last = pos0 + tokens - 1, shift = 31 - __clz(a.page) - 3;
+  const int tokens = min(TOKENS, n - t0), pos0 = kv - n + t0, last = pos0 + tokens - 1, shift = 31 - __clz(a.page) - 3;
   const int first = a.window ? max(0, pos0 - a.window + 1) : 0, first_of_last = a.window ? max(0, last - a.window + 1) : 0;
   const int b0 = first / 32, blocks = last / 32 + 1 - b0, share = (blocks + a.splits - 1) / a.splits;
   const int from = b0 + split * share, to = min(b0 + blocks, from + share);
@@ -389,18 +422,18 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(CT == 2 && 
   w.init();
 #pragma unroll
   for (int c = 0; c < CT; ++c) {
-    const int token = min(16 * (c % 2) + w.col, tokens - 1);  // (beyond the last: the last once more, not written)
+    const int token = min(16 * c + w.col, tokens - 1);  // (beyond the last: the last once more, not written)
     w.kpos[c] = pos0 + token;
     w.kfirst[c] = a.window ? max(0, pos0 + token - a.window + 1) : 0;
-    w.query(c, c / 2 < heads ? (const T*)a.q + (size_t)(row0 + t0 + token) * a.q_stride + (head0 + c / 2) * HD : nullptr, a.scale_log2);
+    w.query(c, (const T*)a.q + (size_t)(row0 + t0 + token) * a.q_stride + head * HD, a.scale_log2, a.wide);
   }
   w.walk(from, to, 1, (first_of_last + 31) / 32, (pos0 + 1) / 32, first / 8, last / 8, a.block_table + (size_t)req * a.table_stride, a.pool, a.kv_heads, kvh, shift);
 #pragma unroll
   for (int c = 0; c < CT; ++c) {
     float total, low;
     const float weight = w.weight(c, total, low), inv = total == 0.f ? 0.f : 1.f / total;
-    const int token = 16 * (c % 2) + w.col, head = head0 + c / 2;
-    if (token >= tokens || c / 2 >= heads) continue;
+    const int token = 16 * c + w.col;
+    if (token >= tokens) continue;
     if (a.splits == 1) {
       T* to_ = (T*)a.out + ((size_t)(row0 + t0 + token) * a.heads + head) * HD;
 #pragma unroll
@@ -416,7 +449,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(CT == 2 && 
         }
       }
     } else {
-      const size_t pc = (((size_t)tile * KV4_TILE_TOKENS + token) * a.heads + head) * a.splits + split;
+      const size_t pc = (((size_t)tile * KV4_TILE_TOKENS + piece * TOKENS + token) * a.heads + head) * a.splits + split;
 #pragma unroll
       for (int nb = 0; nb < Wave::NB; ++nb)
 #pragma unroll

@@ -1467,10 +1467,11 @@ def kv4_tiles_take(head_dim: int) -> bool:
 
 
 def attention_kv4(q, out, pages: Kv4Pages, tiles, block_table, heads: int, kv_heads: int, head_dim: int, scale: float, rows: bool, window: int = 0, splits: int = 1,
-                  workspace: tuple[torch.Tensor, torch.Tensor] | None = None) -> torch.Tensor:
+                  workspace: tuple[torch.Tensor, torch.Tensor] | None = None, groups: int = 1, wave_tokens: int = 16) -> torch.Tensor:
     """Attention over 4-bit pages on the matrix cores, head sizes 64 and 128, bfloat16 and float32, of the tokens that ``tiles`` (int32 [n_tiles, 8], as for ``attention_mfma``) describe:
     with ``rows`` single tokens, a tile each, otherwise portions in tiles of up to 32 tokens.  Tokens that no tile describes are left as they are.  ``splits`` > 1 cuts the keys of every tile into
-    that many ranges and needs ``workspace`` = float32 tensors of columns * splits * head_dim and columns * splits values, columns = tiles * (1 or 32) * heads."""
+    that many ranges and needs ``workspace`` = float32 tensors of columns * splits * head_dim and columns * splits values, columns = tiles * (1 or 32) * heads.  Single tokens
+    use as many of their ranges as make about ``groups`` workgroups of all tokens' keys.  A wave takes ``wave_tokens`` of a portion's tile, 16 or, of bfloat16, 32."""
     if not isinstance(pages, Kv4Pages):
         raise KernelRefused("attention_kv4 takes 4-bit pages (Kv4Pages)")
     if not kv4_tiles_take(head_dim):
@@ -1480,11 +1481,15 @@ def attention_kv4(q, out, pages: Kv4Pages, tiles, block_table, heads: int, kv_he
     _kv4_table(block_table, "attention_kv4")
     if tiles.dim() != 2 or tiles.shape[1] != TILE_INTS:
         raise KernelRefused(f"attention_kv4: tiles must be int32 [n_tiles, {TILE_INTS}]")
+    if groups < 1 or pages.pool.numel() // pages.pool.shape[3] >= 1 << 31:
+        raise KernelRefused("attention_kv4: at least one workgroup, and fewer than 2^31 records in the pool")
+    if wave_tokens not in (16, 32) or (wave_tokens == 32 and q.dtype == torch.float32):
+        raise KernelRefused("attention_kv4: a wave takes 16 tokens, of bfloat16 also 32")
     n_tiles = tiles.shape[0]
     po, pl = _check_kv4_attn(q, out, pages, heads, kv_heads, head_dim, window, splits, workspace, n_tiles * (1 if rows else 32) * heads, "attention_kv4")
     _check(build.core().ns_attn_kv4(_ptr(out), _ptr(po), _ptr(pl), _ptr(q), c_int(q.stride(0)), _ptr(pages.pool), _ptr(tiles), _ptr(block_table), c_int(block_table.stride(0)),
-                                    c_int(n_tiles), c_int(heads), c_int(kv_heads), c_int(head_dim), c_int(pages.page), c_int(1 if rows else 0), c_int(splits), c_int(window),
-                                    c_float(scale), c_int(_dtype_code(q)), _stream()), "attention_kv4")
+                                    c_int(n_tiles), c_int(heads), c_int(kv_heads), c_int(head_dim), c_int(pages.page), c_int(1 if rows else 0), c_int(wave_tokens), c_int(splits),
+                                    c_int(groups), c_int(window), c_float(scale), c_int(_dtype_code(q)), _stream()), "attention_kv4")
     return out
 
 

@@ -27,10 +27,18 @@ PORTION_SINGLE_SET_BLOCKS = 128  # 32-key blocks of the longest row from which a
 DECODE_WAVES_PER_UNIT = 4  # decode rows' keys are cut into ranges until about this many waves per compute unit are at work
 LONG_ROW_KEYS = 8192  # rows that may reach this many keys get up to 32 ranges instead of 16
 F32_RANGE_KEYS = 128  # keys of a range of a single token's row in 32-bit: two tiles of 16 for each wave of its workgroup
-KV4_MAX_RANGES = 64  # of a row's keys in 4 bits, and the fewest keys of one
-KV4_RANGE_KEYS = 256
-KV4_PORTION_KEYS = 512  # the fewest keys of a range of a portion's
-KV4_GROUPS_PER_UNIT = 4  # workgroups of single tokens for each compute unit that ranges of keys are cut for
+# Attention over keys and values in 4 bits (us, 32 heads on 8 of 128 channels unless said otherwise)
+KV4_MAX_RANGES = 64  # of a row's keys
+KV4_RANGE_KEYS = 256  # the fewest keys of a single token's: with fewer a workgroup's beginning and end are longer than its blocks
+# The fewest keys of a range of a portion's, and the most where there are ranges at all (their lengths differ with the tiles': 666 tokens at 20,000 keys 480 in 2 ranges, 396 in 4, 372 in 5,
+# 371 in 8).  Ranges cost what joining their results takes: 2,048 tokens 69 in one range, 103 in two; 100 tokens at 1,000 keys 28 and, in 8, 19.
+KV4_PORTION_KEYS = 128, 4096
+# The keys up to which a wave takes 16 tokens of a portion (three or four waves a SIMD, which hide each other's waits and end evenly) instead of 32 (two, each key made an operand once for
+# both halves).  2,048 tokens 69 and 81, 100 at 1,000 keys 19 and 23; 512 at 8,000 133 and 118, 2,048 at 16,000 888 and 778.
+KV4_NARROW_KEYS = 4096
+# Workgroups of four waves that single tokens' keys are cut for, for each compute unit.  Of 1, 2, 3 and 4: 8 rows of 4,000 keys 18.2, 17.6, 20.6, 21.4; 61 of 200 to 12,000 89, 93, 95, 90;
+# 2 of 100,000 (64 heads) 64, 62, 67, 70; one of 32,000 20, 24, 24, 24; 64 of 6,000 (64 channels) 67, 62, 62, 65.
+KV4_GROUPS_PER_UNIT = 2
 QKV_JOIN_MAX_RANGES = 4  # 17 to 128 rows: the kernel that joins the ranges of the q/k/v product, rotates and writes the cache reads
 #                          every range, so more of them cost it what they gain the product
 
@@ -41,8 +49,8 @@ class TilePlan:
     A tile is ``ops.TILE_INTS`` ints: request, first token of the tile among the request's tokens of this step, row of the
     request's first token, tokens of the request in this step, keys after this step, for one-token tiles the keys that
     all of them read in this step over all layers (by which the kernel chooses its loads: what cannot stay cached until
-    the next step is read past the caches); for portion tiles the number of their portion in the seventh int, and in the eighth,
-    whichever tile it stands in, as the p-th one of them the number of portion p's first tile (-1 behind the last portion that brings
+    the next step is read past the caches), and in the seventh int the blocks of 32 keys of all one-token tiles; for portion tiles the number of their portion in the seventh int, and in the eighth,
+    whichever of these tiles it stands in, as the p-th one of them the number of portion p's first tile (-1 behind the last portion that brings
     tokens).  shape = (portion tiles, one-token tiles); a region of a fixed shape may hold more portion tiles than the batch needs: the
     rest bring no tokens and the kernel skips them."""
 
@@ -80,6 +88,7 @@ class TilePlan:
             k = len(req)
             d[:k, 0], d[:k, 2], d[:k, 3], d[:k, 4] = req, indptr[req], 1, kv[req]
             d[:k, 5] = min(int(kv[req].sum()) * facts.kv_layers, 2**31 - 1)
+            d[:, 6] = ((kv[req] + 31) // 32).sum()
             out[ops.TILE_INTS * tc : ops.TILE_INTS * (tc + td)] = d.reshape(-1)
 
     @staticmethod
@@ -245,15 +254,20 @@ def kv4_attention(ctx, q, out, pages, table, heads: int, kv_heads: int, head_dim
     portions, singles = TilePlan.views(ctx)
     if portions.shape[0]:
         tiles, longest = portions.shape[0], min(ctx.max_chunk_kv, span + TilePlan.TOKENS)
-        waves = tiles * kv_heads * -(-group // (2 if group > 1 else 1))
-        splits = max(1, min(KV4_MAX_RANGES, 8 * units // waves, longest // KV4_PORTION_KEYS))
-        ops.attention_kv4(q, out, pages, portions, table, heads, kv_heads, head_dim, scale, rows=False, window=window, splits=splits,
+        wave_tokens = 16 if q.dtype == torch.float32 or longest <= KV4_NARROW_KEYS else TilePlan.TOKENS
+        # ranges until there are eight waves for each compute unit, if there are not without
+        waves, least, most = tiles * heads * (TilePlan.TOKENS // wave_tokens), *KV4_PORTION_KEYS
+        splits = 1 if waves >= 8 * units else max(1, min(KV4_MAX_RANGES, max(-(-8 * units // waves), -(-longest // most)), longest // least))
+        ops.attention_kv4(q, out, pages, portions, table, heads, kv_heads, head_dim, scale, rows=False, window=window, splits=splits, wave_tokens=wave_tokens,
                           workspace=workspace(tiles * TilePlan.TOKENS * heads, splits))
     if singles.shape[0]:
         tiles, longest = singles.shape[0], min(ctx.max_kv_len, span)
-        groups = tiles * kv_heads * -(-group // 16)
-        splits = max(1, min(KV4_MAX_RANGES, KV4_GROUPS_PER_UNIT * units // groups, -(-longest // KV4_RANGE_KEYS)))
-        ops.attention_kv4(q, out, pages, singles, table, heads, kv_heads, head_dim, scale, rows=True, window=window, splits=splits, workspace=workspace(tiles * heads, splits))
+        # the kernel cuts each row by the keys that all of them have, so that it comes to about ``groups`` workgroups; here is said how often it may at most
+        items = tiles * kv_heads * -(-group // 16)
+        groups = KV4_GROUPS_PER_UNIT * units
+        splits = max(1, min(KV4_MAX_RANGES, 2 + 4 * groups // items, -(-longest // KV4_RANGE_KEYS)))
+        ops.attention_kv4(q, out, pages, singles, table, heads, kv_heads, head_dim, scale, rows=True, window=window, splits=splits, groups=groups,
+                          workspace=workspace(tiles * heads, splits))
     return out
 
 
