@@ -32,6 +32,8 @@ def main(argv=None) -> int:
     ap.add_argument("--max-running", type=int, default=None)
     ap.add_argument("--max-step-tokens", type=int, default=None, help="token budget of a step (prompts are cut into portions)")
     ap.add_argument("--prefill-chunk", type=int, default=None)
+    ap.add_argument("--products", default="model", choices=["model", "int8"], help="products of the layers in the model's precision or in 8-bit integers")
+    ap.add_argument("--kv-format", default="model", choices=["model", "int4"], help="keys and values in the model's precision or in 4 bits")
     ap.add_argument("--no-graphs", action="store_true", help="do not replay captured graphs for decode steps")
     a = ap.parse_args(argv)
 
@@ -46,12 +48,12 @@ def main(argv=None) -> int:
     from .engine import Engine, EngineConfig
     from .loader import load_model
 
-    model = load_model(a.model, dtype=a.dtype)
+    model = load_model(a.model, dtype=a.dtype, products=a.products)
     params = [SamplingParams(a.max_tokens, a.temperature, a.top_k, a.top_p, None if a.seed is None else a.seed + i, a.logprobs)
               for i in range(len(prompts))]
     blocks = a.num_blocks or sum(-(-(len(p) + a.max_tokens) // a.block_size) for p in prompts) + 1
     eng = Engine(model, EngineConfig(blocks, a.block_size, a.max_admit, a.max_running, cuda_graphs=not a.no_graphs,
-                                     max_step_tokens=a.max_step_tokens, prefill_chunk=a.prefill_chunk))
+                                     max_step_tokens=a.max_step_tokens, prefill_chunk=a.prefill_chunk, kv_format=a.kv_format))
     reqs = [eng.add(p, s) for p, s in zip(prompts, params)]
     while eng.sched.has_work:
         eng.step()

@@ -5,7 +5,8 @@ A run-order entry of the model with a ``PagedNeed`` gets one layer of its group'
                                                         kv/cache.py:16-19; here a head's part of a page is contiguous)
     V [entries, pages, kv_heads, value_dim, page]      (transposed per page for the attention kernels; value_dim is
                                                         head_dim unless the mixer says otherwise)
-Both start as zeros: slots that are masked out are still read (reference: kv/cache.py:18).  A page id
+or, with ``kv_format="int4"``, one of its pages of 4 bits [entries, pages, kv_heads, page / 8, record] (``kernels.ops.Kv4Pages``).
+All start as zeros: slots that are masked out are still read (reference: kv/cache.py:18).  A page id
 means the same page in every entry of its group.  An entry with a ``StateNeed`` gets a tensor
 [slots, *shape]; an entry that reads another entry's cache gets that entry's view.
 """
@@ -16,11 +17,12 @@ from dataclasses import dataclass
 
 import torch
 
-from ..kernels.ops import SlotTensors
+from ..kernels.ops import Kv4Pages, SlotTensors, kv4_read, kv4_takes
 from ..parts.needs import PagedNeed, StateNeed, each_need
 from .manager import GroupSpec
 
 
+KV_FORMATS = ("model", "int4")  # keys and values in the model's precision, or in 4 bits with a step and a lowest value for each token and head
 STEPS_SHARE = 0.1  # of the device's memory that is to be left for the steps beside weights, pages and states
 
 
@@ -29,6 +31,12 @@ class PagedView:
     group: int
     k: torch.Tensor
     v: torch.Tensor
+
+
+@dataclass
+class Int4View:
+    group: int
+    pages: Kv4Pages
 
 
 @dataclass
@@ -59,8 +67,30 @@ def plan_groups(cache_needs: list) -> tuple[list[GroupSpec], list[PagedNeed], li
     return specs, needs, of_entry
 
 
+def check_int4(model, page_size: int) -> None:
+    """Whether every entry of the model's run order that keeps or reads keys and values does so in 4 bits too, with pages of ``page_size`` tokens."""
+    for i, (need, call) in enumerate(zip(model.cache_needs, model.spec.run_order)):
+        if call.cache_from is not None:
+            need = model.cache_needs[call.cache_from]
+            if not getattr(getattr(model.layers[call.layer], "mixer", None), "takes_int4_cache", False):
+                raise ValueError(f"entry {i} of the run order reads another entry's keys and values and does not do so in 4 bits")
+        for single in each_need(need):
+            if isinstance(single, PagedNeed) and not single.int4:
+                raise ValueError(f"entry {i} of the run order does not keep its keys and values in 4 bits: that is built for soft-max attention over rotated keys with values of the keys' size, "
+                                 "without gates, sinks, caps, biases or norms of its own")
+            if isinstance(single, PagedNeed) and not kv4_takes(single.head_dim, page_size):
+                raise ValueError(f"keys and values in 4 bits take heads of a multiple of 32 channels up to 256 and pages of a power of two of tokens from 8, not {single.head_dim} channels and "
+                                 f"pages of {page_size}")
+
+
 class CacheStorage:
-    def __init__(self, model, num_pages: list[int], page_size: int, num_slots: int, dtype, device) -> None:
+    def __init__(self, model, num_pages: list[int], page_size: int, num_slots: int, dtype, device, kv_format: str = "model") -> None:
+        if kv_format not in KV_FORMATS:
+            raise ValueError(f"kv_format={kv_format!r}: use one of {KV_FORMATS}")
+        self.kv_format = kv_format
+        if kv_format == "int4":
+            check_int4(model, page_size)
+            model.serve_int4_cache()
         # what a model keeps only to be faster makes room: where the pages do not fit beside it, or leave little for the steps
         give_back = getattr(model, "give_back_second_copies", lambda: False)
         short = False
@@ -70,6 +100,7 @@ class CacheStorage:
             short = True
         if short:  # (behind the handler, whose traceback holds what had been allocated)
             self.__dict__.clear()
+            self.kv_format = kv_format
             give_back()
             self._allocate(model, num_pages, page_size, num_slots, dtype, device)
         elif dtype == torch.float32 and torch.device(device).type == "cuda":  # (no other models have such copies)
@@ -83,10 +114,13 @@ class CacheStorage:
         flat = [(single, i) for i, (need, call) in enumerate(zip(model.cache_needs, model.spec.run_order)) if call.cache_from is None
                 for single in each_need(need)]
         counts = [sum(1 for single, _ in flat if isinstance(single, PagedNeed) and needs.index(single) == i) for i in range(len(needs))]
-        self.k = [torch.zeros((counts[i], num_pages[i], n.kv_heads, page_size, n.head_dim), dtype=dtype, device=device)
-                  for i, n in enumerate(needs)]
-        self.v = [torch.zeros((counts[i], num_pages[i], n.kv_heads, n.v_dim, page_size), dtype=dtype, device=device)
-                  for i, n in enumerate(needs)]
+        int4 = self.kv_format == "int4"
+        self.k = [] if int4 else [torch.zeros((counts[i], num_pages[i], n.kv_heads, page_size, n.head_dim), dtype=dtype, device=device)
+                                  for i, n in enumerate(needs)]
+        self.v = [] if int4 else [torch.zeros((counts[i], num_pages[i], n.kv_heads, n.v_dim, page_size), dtype=dtype, device=device)
+                                  for i, n in enumerate(needs)]
+        self.int4 = [torch.zeros((counts[i], *Kv4Pages.shape(num_pages[i], n.kv_heads, page_size, n.head_dim)), dtype=torch.uint8, device=device)
+                     for i, n in enumerate(needs)] if int4 else []
         self.states: list[torch.Tensor] = []
         self.views: list = []
         taken = [0] * len(needs)
@@ -95,7 +129,7 @@ class CacheStorage:
                 return tuple(view_of(single) for single in need)
             if isinstance(need, PagedNeed):
                 g = needs.index(need)
-                view = PagedView(g, self.k[g][taken[g]], self.v[g][taken[g]])
+                view = Int4View(g, Kv4Pages(self.int4[g][taken[g]], need.head_dim)) if int4 else PagedView(g, self.k[g][taken[g]], self.v[g][taken[g]])
                 taken[g] += 1
                 return view
             if isinstance(need, StateNeed):
@@ -123,5 +157,18 @@ class CacheStorage:
         for t in self.states:
             t[slot].zero_()
 
+    def kept(self, entry: int, positions: torch.Tensor, token_req: torch.Tensor, block_table: torch.Tensor):
+        """-> (keys, values) [tokens, kv_heads, size], float32, of the tokens at ``positions`` of requests ``token_req`` as run-order entry ``entry`` keeps them (keys as the scores meet them);
+        ``block_table`` int32 [requests, pages] of the entry's group.  For looking at a cache: on the current stream, into new tensors."""
+        view = self.views[entry]
+        if isinstance(view, Int4View):
+            return kv4_read(view.pages, positions, token_req, block_table, dtype=torch.float32)
+        if not isinstance(view, PagedView):
+            raise ValueError(f"entry {entry} of the run order keeps no keys and values in pages of its own")
+        page, at = block_table[token_req.long(), positions.long() // self.page_size].long(), positions.long() % self.page_size
+        return view.k[page, :, at].float(), view.v[page, :, :, at].float()
+
     def bytes_per_token(self) -> int:
+        if self.kv_format == "int4":  # (records of eight tokens)
+            return sum(t.shape[0] * t.shape[2] * t.shape[4] // 8 for t in self.int4)
         return sum((k[:, 0, :, 0].numel() + v[:, 0, :, :, 0].numel()) * k.element_size() for k, v in zip(self.k, self.v))

@@ -34,6 +34,7 @@ class EngineConfig:
     prefill_chunk: int | None = None  # longest portion of one prompt in a step
     on_exhaustion: str = "reserve"  # "reserve" | "preempt": see engine/scheduler.py
     max_seq_len: int | None = None  # longest request that is accepted; None = what the model's positions and the pool allow
+    kv_format: str = "model"  # "model": keys and values in the model's precision; "int4": in 4 bits (cache/storage.py)
     lookahead: bool = True  # enqueue the next decode step before waiting for this one's tokens
 
 
@@ -47,7 +48,7 @@ class Engine:
         max_running = config.max_running if config.max_running is not None else 256
         num_slots = max_running + 1  # one for the pad rows of captured graphs
         self.cache = CacheManager(specs, config.num_blocks, config.block_size, num_slots)
-        self.storage = CacheStorage(model, [config.num_blocks] * len(specs), config.block_size, num_slots, self.dtype, self.device)
+        self.storage = CacheStorage(model, [config.num_blocks] * len(specs), config.block_size, num_slots, self.dtype, self.device, config.kv_format)
         # the longest request: what the caller says and the model's positions allow (the pool bounds it too; the scheduler
         # refuses what can never fit it).  Block tables are only ever as wide as the live requests need: the runner's
         # captured steps grow with them.

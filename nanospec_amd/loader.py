@@ -35,18 +35,18 @@ def _require_gpu(device) -> torch.device:
     return device
 
 
-def load_model(model, device="cuda", dtype=torch.bfloat16, layouts: str = "auto") -> DecoderModel:
-    """``model``: a folder with config.json and safetensors files.  ``layouts``: see ``DecoderModel.load``."""
+def load_model(model, device="cuda", dtype=torch.bfloat16, layouts: str = "auto", products: str = "model") -> DecoderModel:
+    """``model``: a folder with config.json and safetensors files.  ``layouts``, ``products``: see ``DecoderModel.load``."""
     folder = Path(model)
     if not folder.is_dir():
         raise FileNotFoundError(f"{model} is not a model folder (no network access is attempted)")
     config, spec = load_config(folder)
     device = _require_gpu(device)
-    return DecoderModel(spec, config).load(SafetensorsSource(folder), as_dtype(dtype), device, layouts)
+    return DecoderModel(spec, config).load(SafetensorsSource(folder), as_dtype(dtype), device, layouts, products)
 
 
 def random_model(config, seed: int = 0, device="cuda", dtype=torch.bfloat16, on_device: bool = False,
-                 layouts: str = "auto") -> DecoderModel:
+                 layouts: str = "auto", products: str = "model") -> DecoderModel:
     """A model with seeded random weights, without a folder.  ``on_device`` draws the numbers on the GPU
     (large models; the numbers then differ from the CPU draw of the same seed, the law does not)."""
     device = _require_gpu(device)
@@ -55,7 +55,7 @@ def random_model(config, seed: int = 0, device="cuda", dtype=torch.bfloat16, on_
     net = DecoderModel(spec, config)
     skip = {spec.head_name} if spec.tie_head else set()
     if not on_device:
-        return net.load(DictSource(random_tensors(net.wanted(), seed, dtype, skip=skip), "<random>"), dtype, device, layouts)
+        return net.load(DictSource(random_tensors(net.wanted(), seed, dtype, skip=skip), "<random>"), dtype, device, layouts, products)
 
     class _Lazy:
         """Draws each tensor on the device when it is asked for, so that no second copy is ever held."""
@@ -77,4 +77,4 @@ def random_model(config, seed: int = 0, device="cuda", dtype=torch.bfloat16, on_
             shape, role = self.wanted[name]
             return draw(shape, role, self.gen, dtype, dtype)
 
-    return net.load(_Lazy(net.wanted()), dtype, device, layouts)
+    return net.load(_Lazy(net.wanted()), dtype, device, layouts, products)

@@ -18,7 +18,7 @@ import torch
 
 from ..kernels import ops
 from . import registry
-from .linear import LinearWeight
+from .linear import Int8Linear, LinearWeight
 from .needs import PagedNeed
 
 # How the matrix-core attention kernel is launched, from the counts of a step's batch and the size of the GPU
@@ -275,6 +275,8 @@ class Attention:
     graph_safe = True
     ends_in_residual = True  # forward takes residual=IntoResidual
     takes_layouts = True  # load takes which copies of its matrices to keep
+    takes_products = True  # ... and what its products run in
+    reads_int8 = False  # forward takes ops.Int8Rows
 
     def __init__(self, spec, prefix: str) -> None:
         if spec.heads % spec.kv_heads:
@@ -351,9 +353,10 @@ class Attention:
                                                    + 0.2 * torch.randn(shape, generator=gen, dtype=torch.float32, device=gen.device))
         return out
 
-    def load(self, get, dtype, device, layouts: str = "both") -> None:
+    def load(self, get, dtype, device, layouts: str = "both", products: str = "model") -> None:
         s = self.spec
         plain = layouts == "both"
+        int8 = products == "int8"
         q, k, v, o = self._names
         rows = s.heads * s.head_dim + (s.kv_heads * (s.head_dim + (0 if s.value_is_key else s.v_dim)) if s.own_kv else 0)
         self.gate_at = rows  # the output gate's logits, if the layer has a gate, are the last columns of the first product
@@ -390,8 +393,14 @@ class Attention:
         if s.general:
             # the general path: one product for what the layer projects, then norm / cache write and attention as kernels
             self.wqkv_rope = None
-            self.wqkv = LinearWeight(wqkv, keep_plain=plain)
-            self.wo = LinearWeight(get(o).to(device=device, dtype=dtype).contiguous(), keep_plain=plain)
+            self.wqkv = Int8Linear(wqkv) if int8 else LinearWeight(wqkv, keep_plain=plain)
+            self.wo = Int8Linear(get(o).to(device=device, dtype=dtype)) if int8 else LinearWeight(get(o).to(device=device, dtype=dtype).contiguous(), keep_plain=plain)
+            return
+        self.reads_int8 = int8
+        if int8:
+            self.wqkv_rope = None
+            self.wqkv = self.wqkv_int4 = Int8Linear(wqkv)
+            self.wo = Int8Linear(get(o).to(device=device, dtype=dtype))
             return
         # for few rows the stacked matrix is streamed by a kernel that rotates and writes the cache in its epilogue; it
         # wants the rows tiled in an order of its own
@@ -402,12 +411,23 @@ class Attention:
         # (without the plain layout the stacked matrix is also kept tiled in its own row order, for more than 16 rows)
         self.wqkv = LinearWeight(wqkv, keep_plain=plain, tiled=self.wqkv_rope is None or not plain)
         self.wo = LinearWeight(get(o).to(device=device, dtype=dtype).contiguous(), keep_plain=plain)
+        self.wqkv_int4 = None
+
+    @property
+    def takes_int4_cache(self) -> bool:
+        return not self.spec.general and self.spec.head_dim % 32 == 0
+
+    def serve_int4_cache(self) -> None:
+        """A stacked product that leaves q, k and v as they are: with 4-bit pages the rotation and the write are a kernel of their own, also for few rows.  (The copy that the kernel with
+        both in its epilogue streams has its rows in that kernel's order.)"""
+        if self.takes_int4_cache and self.wqkv_int4 is None:
+            self.wqkv_int4 = self.wqkv if self.wqkv_rope is None or self.wqkv.plain is None else LinearWeight(self.wqkv.plain)
 
     def cache_need(self):
         s = self.spec
         if not s.own_kv:
             return None  # it reads the cache of the run-order entry that its LayerCall names
-        return PagedNeed(s.kv_heads, s.head_dim, s.window, 0 if s.v_dim == s.head_dim else s.v_dim)
+        return PagedNeed(s.kv_heads, s.head_dim, s.window, 0 if s.v_dim == s.head_dim else s.v_dim, int4=self.takes_int4_cache)
 
     def batch_plans(self) -> list:
         """What this mixer asks the batch builder to put on the device each step (``engine.context``)."""
@@ -429,11 +449,19 @@ class Attention:
         pos = self.position
         if pos.max_positions is not None and ctx.max_position >= pos.max_positions:
             raise ValueError(f"position {ctx.max_position} is beyond the model's {pos.max_positions} positions")
-        qkv = ctx.arena.take((n, self.wqkv.n), x.dtype)
+        dtype = self.wqkv.dtype if isinstance(x, ops.Int8Rows) else x.dtype
+        qkv = ctx.arena.take((n, self.wqkv.n), dtype)
         table = ctx.block_tables[cache.group]
+        int4 = getattr(cache, "pages", None)
         if s.general:
+            if int4 is not None:
+                raise ops.KernelRefused("this layer does not read keys and values in 4 bits")
             return self._forward_general(ctx, x, cache, owns_cache, out, residual, qkv, table, add_out_bias)
-        if self.wqkv_rope is not None and n <= 16 and ops.tiled_takes(x.x if isinstance(x, ops.PreNormed) else x, s.hidden):
+        if int4 is not None:
+            self.wqkv_int4(x, out=qkv, arena=ctx.arena, plain_copy=not ctx.captured)
+            ops.rope_kv4_write(qkv, ctx.positions, ctx.token_req, table, pos.inv_freq, int4, s.heads, s.kv_heads, s.head_dim, pos.rotary_dim,
+                               write_kv=owns_cache, **self._form)
+        elif self.wqkv_rope is not None and n <= 16 and ops.tiled_takes(x.x if isinstance(x, ops.PreNormed) else x, s.hidden):
             ops.linear_qkv_rope(x, self.wqkv_rope, qkv, ctx.positions, ctx.token_req, table, pos.inv_freq, cache.k, cache.v,
                                 s.heads, s.kv_heads, s.head_dim, pos.rotary_dim, write_kv=owns_cache, **self._form)
         elif (self.wqkv_rope is not None and n <= ops.WIDE_TALL_ROWS and not isinstance(x, ops.PreNormed) and ops.tiled_takes(x[:1], s.hidden)
@@ -450,15 +478,17 @@ class Attention:
             self.wqkv(x, out=qkv, arena=ctx.arena, plain_copy=not ctx.captured)
             ops.rope_kv_write(qkv, ctx.positions, ctx.token_req, table, pos.inv_freq, cache.k, cache.v, s.heads, s.kv_heads,
                               s.head_dim, pos.rotary_dim, write_kv=owns_cache, **self._form)
-        att = ctx.arena.take((n, s.heads * s.head_dim), x.dtype)
-        page = cache.k.shape[2]
-        if ops.mfma_attention_takes(x.dtype, s.head_dim, page):
+        att = ctx.arena.take((n, s.heads * s.head_dim), dtype)
+        page = cache.k.shape[2] if int4 is None else int4.page
+        if int4 is not None:
+            kv4_attention(ctx, qkv, att, int4, table, s.heads, s.kv_heads, s.head_dim, s.softmax_scale, window=s.window)
+        elif ops.mfma_attention_takes(dtype, s.head_dim, page):
             group = s.heads // s.kv_heads
             for plan in launch_plans(ctx, group, s.kv_heads, s.head_dim):
                 ops.attention_mfma(qkv, att, cache.k, cache.v, plan.tiles, table, s.heads, s.kv_heads, s.head_dim,
                                    s.softmax_scale, window=s.window, hp=plan.hp, splits=plan.splits, workspace=plan.workspace,
                                    qt=plan.qt, coop=plan.coop)
-        elif TilePlan.key in ctx.plans and ops.f32_attention_takes(x.dtype, s.head_dim, s.head_dim, page):
+        elif TilePlan.key in ctx.plans and ops.f32_attention_takes(dtype, s.head_dim, s.head_dim, page):
             f32_attention(ctx, qkv, att, cache, table, s.heads, s.kv_heads, s.head_dim, s.softmax_scale, window=s.window)
         else:
             ops.attention_generic(qkv, att, cache.k, cache.v, ctx.token_req, ctx.positions, table, s.heads, s.kv_heads,

@@ -12,6 +12,17 @@ from ..kernels import ops
 from . import registry
 from .linear import IntoResidual
 
+
+def load_parts(parts, get, dtype, device, layouts: str, products: str) -> None:
+    for p in parts:
+        if getattr(p, "takes_products", False):
+            p.load(get, dtype, device, layouts, products)
+        elif getattr(p, "takes_layouts", False):
+            p.load(get, dtype, device, layouts)
+        else:
+            p.load(get, dtype, device)
+
+
 class PreNormBlock:
     def __init__(self, spec, prefix: str | None = None) -> None:
         p = spec.prefix if prefix is None else prefix
@@ -33,14 +44,10 @@ class PreNormBlock:
             out.update(p.wanted())
         return out
 
-    def load(self, get, dtype, device, layouts: str = "both") -> None:
-        for p in self.parts:
-            if getattr(p, "takes_layouts", False):
-                p.load(get, dtype, device, layouts)
-            else:
-                p.load(get, dtype, device)
+    def load(self, get, dtype, device, layouts: str = "both", products: str = "model") -> None:
+        load_parts(self.parts, get, dtype, device, layouts, products)
 
-    takes_layouts = True
+    takes_layouts = takes_products = True
 
     def cache_need(self):
         return self.mixer.cache_need()
@@ -76,11 +83,15 @@ class PreNormBlock:
         ends = lambda part: link and getattr(part, "ends_in_residual", False)
         lp = lambda norm: link and norm is not None and getattr(norm, "links_products", False) and norm.weight.dtype == resid.dtype
         buf = lambda: ctx.arena.take(resid.shape, resid.dtype)
+        # a norm whose result goes straight into 8 bits, for parts whose products read those
+        int8 = lambda norm, part, x: getattr(part, "reads_int8", False) and getattr(norm, "makes_int8", False) and (x is None or isinstance(x, torch.Tensor))
 
         # first norm and mixer
         whole = (ops.PreNormed, ops.Added)  # forms in which resid already holds the sum
         if isinstance(delta, whole):
             h = delta if isinstance(delta, ops.PreNormed) and takes(self.mixer) else self.mixer_norm.forward(ctx, resid=resid, out=buf())
+        elif int8(self.mixer_norm, self.mixer, delta):
+            h = self.mixer_norm.int8(ctx, resid, x=delta, write_resid=delta is not None)
         else:
             h = self.mixer_norm.forward(ctx, resid=resid, x=delta, write_resid=delta is not None, out=buf())
         if ends(self.mixer) and lp(self.ffn_norm):
@@ -91,6 +102,8 @@ class PreNormBlock:
         # second norm and feed-forward
         if isinstance(a, whole):
             h2 = a if isinstance(a, ops.PreNormed) and takes(self.ffn) else self.ffn_norm.forward(ctx, resid=resid, out=buf())
+        elif int8(self.ffn_norm, self.ffn, a):
+            h2 = self.ffn_norm.int8(ctx, resid, x=a, write_resid=True)
         else:
             h2 = self.ffn_norm.forward(ctx, resid=resid, x=a, write_resid=True, out=buf())
         if ends(self.ffn) and lp(next_norm) and next_sums is not None:
@@ -179,14 +192,10 @@ class StreamBlock:
         """How many buffers the block can leave unwritten outputs in (``forward``'s ``delta_out``)."""
         return 2 if self.parallel and self.ffn is not None and self.extra is None else 1
 
-    takes_layouts = True
+    takes_layouts = takes_products = True
 
-    def load(self, get, dtype, device, layouts: str = "both") -> None:
-        for p in self.parts:
-            if getattr(p, "takes_layouts", False):
-                p.load(get, dtype, device, layouts)
-            else:
-                p.load(get, dtype, device)
+    def load(self, get, dtype, device, layouts: str = "both", products: str = "model") -> None:
+        load_parts(self.parts, get, dtype, device, layouts, products)
         S, m = self.copies, float(self.spec.mult)
         self.dtype = dtype
         self._hc = []

@@ -28,6 +28,9 @@ from ..kernels import ops
 # hand-written kernels: slower prompts, half the memory.  Of a float32 matrix the plain copy is always there and, with "both", one in
 # two parts that its products of many rows read (``ops.SplitWeight``).
 LAYOUTS = ("both", "tiled")
+# What the products of a model's layers run in (``DecoderModel.load(..., products=)``; parts that say ``takes_products`` are told at load time): the model's precision, or 8-bit integers
+# (``Int8Linear``).  The head, norms, attention and what passes between the parts stay as they are.
+PRODUCTS = ("model", "int8")
 
 
 STREAM_ROWS = 16  # up to here the streaming kernel beats the library at the shapes measured
@@ -319,6 +322,52 @@ class LinearWeight:
             else:
                 ops.linear_wide(x[s:e], self.tiled, out=out[s:e], out_f32=out_f32, workspace=ws, ksplit=ksplit, nt=nt)
         return out
+
+
+class Int8Linear:
+    """x @ W^T in 8-bit integers, beside ``LinearWeight``: the weight's rows and x's rows are whole numbers of -127 to 127 with a 32-bit scale each (``ops.Int8Weight``), sums exact, the
+    result in the model's precision.  ``x`` may come in 8 bits already (``ops.Int8Rows``, from the norm or the activation in front); otherwise a kernel quantises it.  Only the 8-bit
+    weight is kept."""
+
+    def __init__(self, w: torch.Tensor) -> None:
+        self.n, self.k = w.shape
+        self.dtype = w.dtype
+        self.weight = ops.Int8Weight.from_float(w)
+
+    def links_norms(self, rows: int) -> bool:
+        return False
+
+    def into_residual(self, x, link: IntoResidual, arena=None, plain_copy: bool = False):
+        return self(x, out=link.x_next, arena=arena)  # (the norm's kernel adds it)
+
+    def __call__(self, x, out: torch.Tensor | None = None, out_f32: bool = False, arena=None, plain_copy: bool = False, act: str | None = None) -> torch.Tensor:
+        rows = x
+        take = arena.take if arena is not None else None
+        if isinstance(x, torch.Tensor):
+            if x.dtype != self.dtype:
+                raise ops.KernelRefused(f"linear: input is {x.dtype}, the weight {self.dtype}")
+            rows = ops.int8_rows(x, take=take)
+        if out is None:
+            dtype = torch.float32 if out_f32 else self.dtype
+            out = take((rows.shape[0], self.n), dtype) if take is not None else None
+        elif out_f32 and out.dtype != torch.float32:
+            raise ops.KernelRefused("linear: a 32-bit result goes into a float32 tensor")
+        out = ops.linear_int8(rows, self.weight, out=out, dtype=torch.float32 if out_f32 else self.dtype, take=take)
+        return out if act is None else ops.activation(out, act)
+
+
+class Int8Gated:
+    """``GatedWeights`` in 8-bit integers: one product of the stacked matrices, then silu(gate) * up straight into 8 bits for the product behind it."""
+
+    def __init__(self, gate: torch.Tensor, up: torch.Tensor) -> None:
+        self.inter, self.k = gate.shape
+        self.product = Int8Linear(torch.cat([gate, up]))
+
+    def links_norms(self, rows: int) -> bool:
+        return False
+
+    def __call__(self, ctx, x) -> "ops.Int8Rows":
+        return ops.silu_mul_int8(self.product(x, arena=ctx.arena), take=ctx.arena.take)
 
 
 class GatedWeights:

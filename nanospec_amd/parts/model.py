@@ -11,7 +11,7 @@ import torch
 from ..kernels import ops
 from ..weights import source as wsource
 from . import registry
-from .linear import LAYOUTS, LinearWeight, drop_copies_of_little_use, second_copies
+from .linear import LAYOUTS, PRODUCTS, LinearWeight, drop_copies_of_little_use, second_copies
 from .needs import PagedNeed, StateNeed
 
 
@@ -100,12 +100,20 @@ class DecoderModel:
     def wanted(self) -> dict:
         return wanted_tensors(self.spec, self.layers)
 
-    def load(self, source, dtype: torch.dtype, device, layouts: str = "auto") -> "DecoderModel":
+    def load(self, source, dtype: torch.dtype, device, layouts: str = "auto", products: str = "model") -> "DecoderModel":
         """Check the source against what the model wants (one error that lists everything wrong), then read
         each tensor once.  A head that is absent is the embedding table if the configuration ties them
         (reference: model/loader.py:62-70).  ``layouts``: "both" keeps every matrix in two layouts
-        (``parts.linear.LAYOUTS``), "tiled" only in one (in bfloat16 the re-laid one), "auto" chooses by the memory that is free."""
+        (``parts.linear.LAYOUTS``), "tiled" only in one (in bfloat16 the re-laid one), "auto" chooses by the memory that is free.
+        ``products`` "int8": the layers' products run in 8-bit integers (``parts.linear.PRODUCTS``), and their matrices are kept in 8 bits alone."""
         spec = self.spec
+        if products not in PRODUCTS:
+            raise ValueError(f"products={products!r}: use one of {PRODUCTS}")
+        if products == "int8":
+            for layer in self.layers:
+                for part in (layer, getattr(layer, "mixer", None), getattr(layer, "ffn", None)):
+                    if part is not None and not getattr(part, "takes_products", False):
+                        raise ValueError(f"products in 8-bit integers are not built for {type(part).__name__}")
         full = self.wanted()
         wanted = {k: v[0] for k, v in full.items()}
         wsource.check(source, wanted, optional={spec.head_name} if spec.tie_head else frozenset(), unread_prefixes=spec.unread_prefixes)
@@ -122,7 +130,7 @@ class DecoderModel:
             if layouts == "tiled":
                 slower = "copy matrices into plain rows first and are slower" if dtype == torch.bfloat16 else "run on the 32-bit matrix instructions and take twice as long"
                 print(f"[nanospec_amd] {linear / 2**30:.0f} GiB of matrices, {free / 2**30:.0f} GiB free: keeping one layout; steps of many tokens {slower}", file=sys.stderr, flush=True)
-        self.layouts = layouts
+        self.layouts, self.products = layouts, products
         get = source.get
         self.embed = get(spec.embed_name).to(device=device, dtype=dtype).contiguous()
         if spec.head_name in source.names():
@@ -130,7 +138,9 @@ class DecoderModel:
         else:
             self.head = LinearWeight(self.embed, keep_plain=False)  # the embedding table is the head
         for layer in self.layers:
-            if getattr(layer, "takes_layouts", False):
+            if getattr(layer, "takes_products", False):
+                layer.load(get, dtype, device, layouts, products)
+            elif getattr(layer, "takes_layouts", False):
                 layer.load(get, dtype, device, layouts)
             else:
                 layer.load(get, dtype, device)
@@ -149,6 +159,15 @@ class DecoderModel:
         # matrices, random draws) is finished before anyone can read it
         torch.cuda.synchronize(self.device)
         return self
+
+    def serve_int4_cache(self) -> None:
+        """The layers are about to be handed keys and values in 4 bits (``cache.storage``)."""
+        for layer in self.layers:
+            for part in getattr(layer, "parts", ()):
+                for one in (part, *getattr(part, "sides", ())):
+                    if hasattr(one, "serve_int4_cache"):
+                        one.serve_int4_cache()
+        torch.cuda.synchronize(self.device)
 
     def give_back_second_copies(self) -> bool:
         """For whoever needs the memory (``cache.storage``): the second copies of float32 matrices, which only make products of many rows faster, are given back.  Not once a runner has been made for

@@ -3,7 +3,7 @@ tuple of these for a mixer made of several (it is then handed a tuple of views i
 
 from __future__ import annotations
 
-from dataclasses import dataclass
+from dataclasses import dataclass, field
 
 import torch
 
@@ -16,6 +16,7 @@ class PagedNeed:
     head_dim: int
     window: int = 0  # 0 = every earlier token stays
     value_dim: int = 0  # size of a value head if it is not ``head_dim``
+    int4: bool = field(default=False, compare=False)  # the mixer also works on pages of 4 bits (``kernels.ops.Kv4Pages``)
 
     @property
     def v_dim(self) -> int:

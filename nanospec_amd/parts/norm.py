@@ -20,6 +20,7 @@ class RMSNorm:
         # a weight kept as the factor minus one: the factor is 1 + w, which the kernels form in 32-bit from the stored value (1 + w
         # rounded to bfloat16 would lose most of w)
         self.offset = 1.0 if getattr(spec, "unit_offset", False) else 0.0
+        self.makes_int8 = not self.offset
         if self.offset:
             self.links_products = False  # the products that fold a norm in multiply by the stored weight
 
@@ -33,6 +34,10 @@ class RMSNorm:
         if self.offset:
             raise ops.KernelRefused("a norm whose weight is kept as the factor minus one reads a 32-bit stream (blocks of kind 'streams')")
         return ops.rmsnorm(self.weight, self.spec.eps, resid=resid, x=x, rows=rows, write_resid=write_resid, out=out)
+
+    def int8(self, ctx, resid, x=None, write_resid=False) -> "ops.Int8Rows":
+        """``forward``, its result in 8 bits for the product behind it: quantised from 32-bit in the same pass."""
+        return ops.rmsnorm_int8(self.weight, self.spec.eps, resid=resid, x=x, resid_out=resid if write_resid else None, take=ctx.arena.take)
 
     def read_streams(self, ctx, streams: torch.Tensor, coeff: torch.Tensor, rows=None, out=None, sum_out=None, pending=None,
                      store: bool = True) -> torch.Tensor:

@@ -35,11 +35,18 @@ Optional:
                                                   smallest limit of a model's layers)
   any part     takes_layouts = True: load(get, dtype, device, layouts) with layouts "both" | "tiled"
                                                   (which copies of a bfloat16 matrix to keep, ``parts.linear.LAYOUTS``)
+  block, mixer, ffn
+               takes_products = True: load(get, dtype, device, layouts, products) with products "model" | "int8"
+                                                  (what its products run in, ``parts.linear.PRODUCTS``)
+  mixer        takes_int4_cache: bool; serve_int4_cache() is called before it is handed a cache in 4 bits
+                                                  (``cache.storage.Int4View``), which its ``PagedNeed`` says it takes
 
 Optional, for parts whose products can do the work of the RMS norms around them (``parts.linear.IntoResidual``):
   norm         links_products = True, weight, spec.eps
   mixer, ffn   ends_in_residual = True: forward(..., residual=IntoResidual) -> PreNormed | PartialSums | Added | tensor;
                links_norms(rows) -> bool: x may be a PreNormed
+  norm         makes_int8 = True: int8(ctx, resid, x=None, write_resid=False) -> ``ops.Int8Rows``
+  mixer, ffn   reads_int8: bool                   x may be those
   block        links_blocks = True; entry_norm (the norm that reads the block's input);
                forward(..., next_norm=None, next_sums=None, next_carry=None) -> None or one of those three
 """

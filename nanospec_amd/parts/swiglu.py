@@ -2,7 +2,8 @@
 Gate and up matrices are stacked at load time so that one pass over the input serves both.  With biases
 (``SwiGLUSpec.bias``) gate and up add theirs in the streaming product's epilogue for up to 16 rows, and for more rows are one
 product of the stacked matrix and a kernel that adds the biases and applies the activation; the down-projection's bias is
-added behind it, or left to the block (``out_bias``)."""
+added behind it, or left to the block (``out_bias``).  Without biases the products may run in 8-bit integers
+(``products="int8"``): both inputs are quantised by the kernel in front, the norm's or the activation's."""
 
 from __future__ import annotations
 
@@ -10,13 +11,15 @@ import torch
 
 from ..kernels import ops
 from . import registry
-from .linear import GatedWeights, LinearWeight
+from .linear import GatedWeights, Int8Gated, Int8Linear, LinearWeight
 
 
 class SwiGLU:
     graph_safe = True
     ends_in_residual = True  # forward takes residual=IntoResidual
     takes_layouts = True  # load takes which copies of its matrices to keep
+    takes_products = True  # ... and what its products run in
+    reads_int8 = False  # forward takes ops.Int8Rows
 
     def __init__(self, spec, prefix: str) -> None:
         self.spec, self.prefix = spec, prefix
@@ -41,11 +44,17 @@ class SwiGLU:
                         d + s.bias_suffix: ((s.hidden,), "bias")})
         return out
 
-    def load(self, get, dtype, device, layouts: str = "both") -> None:
+    def load(self, get, dtype, device, layouts: str = "both", products: str = "model") -> None:
         s = self.spec
         plain = layouts == "both"
         g, u, d = self._names
         to = lambda name: get(name).to(device=device, dtype=dtype)
+        self.reads_int8 = products == "int8"
+        if self.reads_int8:
+            if self.biased:
+                raise ValueError("a feed-forward with biases has no products in 8-bit integers")
+            self.gate_up, self.down = Int8Gated(to(g), to(u)), Int8Linear(to(d))
+            return
         if self.biased:
             self.gate_up = GatedWeights(to(g), to(u), keep_plain=plain, bias=(to(g + s.bias_suffix), to(u + s.bias_suffix)))
             self.out_bias = to(d + s.bias_suffix).contiguous()
@@ -64,7 +73,7 @@ class SwiGLU:
             y = self.down(act, out=out if out is not None else ctx.arena.take((n, self.spec.hidden), x.dtype), arena=ctx.arena,
                           plain_copy=not ctx.captured)
             return ops.add_bias(y, self.out_bias) if add_out_bias else y
-        act = self.gate_up(ctx, x, out=ctx.arena.take((x.shape[0], self.spec.intermediate), x.dtype))
+        act = self.gate_up(ctx, x) if self.reads_int8 else self.gate_up(ctx, x, out=ctx.arena.take((x.shape[0], self.spec.intermediate), x.dtype))
         if residual is not None:
             return self.down.into_residual(act, residual, arena=ctx.arena, plain_copy=not ctx.captured)
         return self.down(act, out=out, arena=ctx.arena, plain_copy=not ctx.captured)

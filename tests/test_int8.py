@@ -76,3 +76,19 @@ def test_plan():
                     assert 0 <= form < len(ops.INT8_TILES) and ops.int8_padded_k(k) >= ranges * ops.INT8_K_MIN
                     tiles = -(-m // ops.INT8_TILES[form][0]) * -(-n // ops.INT8_TILES[form][1])
                     assert tiles * ranges <= 1 << 22
+
+
+def test_models_refuse_products_that_are_not_built():
+    """Before anything is read or moved."""
+    from types import SimpleNamespace
+
+    from nanospec_amd.config import LlamaConfig
+    from nanospec_amd.parts import DecoderModel
+    from tiny import TINY
+
+    net = DecoderModel(LlamaConfig.from_hf(TINY["A"]["cfg"]).model_spec())
+    with pytest.raises(ValueError, match="products="):
+        net.load(None, torch.float32, "cpu", products="int4")
+    net.layers[1].ffn = SimpleNamespace()
+    with pytest.raises(ValueError, match="not built for SimpleNamespace"):
+        net.load(None, torch.float32, "cpu", products="int8")

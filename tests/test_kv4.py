@@ -102,3 +102,42 @@ def test_attention_refuses(monkeypatch, change):
 def test_tensors_on_the_cpu_are_refused():
     with pytest.raises(ops.KernelRefused, match="GPU"):
         ops.kv4_read(ops.Kv4Pages.empty(1, 1, 8, 32, "cpu"), torch.zeros(1, dtype=torch.int32), torch.zeros(1, dtype=torch.int32), torch.zeros((1, 1), dtype=torch.int32))
+
+
+# ------------------------------------------------------------------------------------------------ which models and engines take them
+
+
+def _model(needs, cache_from=None, mixers=None):
+    from types import SimpleNamespace
+
+    cache_from = cache_from or [None] * len(needs)
+    order = [SimpleNamespace(cache_from=c, layer=i) for i, c in enumerate(cache_from)]
+    layers = [SimpleNamespace(mixer=m) for m in (mixers or [None] * len(needs))]
+    return SimpleNamespace(cache_needs=needs, spec=SimpleNamespace(run_order=order), layers=layers, serve_int4_cache=lambda: None)
+
+
+def test_caches_in_4_bits_refuse_what_is_not_built():
+    from types import SimpleNamespace
+
+    from nanospec_amd.cache.storage import CacheStorage
+    from nanospec_amd.parts.needs import PagedNeed
+
+    fits, other = PagedNeed(2, 64, int4=True), PagedNeed(2, 64)
+    assert fits == other and hash(fits) == hash(other)  # (groups of pages are what they were)
+    make = lambda model, page=16, kv_format="int4": CacheStorage(model, [4] * len({n for n in model.cache_needs if n is not None}), page, 2, torch.float32, "cpu", kv_format)
+    with pytest.raises(ValueError, match="kv_format"):
+        make(_model([fits]), kv_format="int8")
+    with pytest.raises(ValueError, match="does not keep its keys and values in 4 bits"):
+        make(_model([fits, other]))
+    with pytest.raises(ValueError, match="multiple of 32 channels"):
+        make(_model([PagedNeed(2, 80, int4=True)]))
+    for page in (4, 12):
+        with pytest.raises(ValueError, match="power of two of tokens from 8"):
+            make(_model([fits]), page)
+    reads = SimpleNamespace(takes_int4_cache=True)
+    with pytest.raises(ValueError, match="reads another entry"):
+        make(_model([fits, None], [None, 0], [reads, SimpleNamespace()]))
+    storage = make(_model([fits, None, None], [None, 0, None], [reads, reads, None]))
+    assert storage.views[1] is storage.views[0] and storage.views[2] is None and storage.views[0].pages.pool.shape == (4, 2, 2, 8 * 64 + 64)
+    with pytest.raises(ValueError, match="keeps no keys and values"):
+        storage.kept(2, None, None, None)
