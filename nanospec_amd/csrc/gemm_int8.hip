@@ -385,6 +385,8 @@ __global__ __launch_bounds__(Q::WAVES * NS_WAVE) __attribute__((amdgpu_waves_per
   }
 }
 
+#define INT8_JOIN_ROWS 65535  // a row of workgroups each
+
 template <typename T>
 __global__ __launch_bounds__(256) void gemm_int8_join_kernel(const Int8ManyParams a) {
   const Int8Params& p = a.p;
@@ -400,7 +402,7 @@ static int launch_int8_many(Int8ManyParams a, hipStream_t stream) {
   const Int8Params& p = a.p;
   a.m_tiles = (p.M + Q::BM - 1) / Q::BM, a.n_tiles = (p.N + Q::BN - 1) / Q::BN;
   const long long items = (long long)a.m_tiles * a.n_tiles * p.ranges;
-  if (p.KP / 256 / p.ranges * 4 < Q::ST || items > (1 << 22) || p.M > 65535) return NS_ERR_UNSUPPORTED;
+  if (p.KP / 256 / p.ranges * 4 < Q::ST || items > (1 << 22) || (p.ranges > 1 && p.M > INT8_JOIN_ROWS)) return NS_ERR_UNSUPPORTED;
   const unsigned grid = (unsigned)((items + 7) / 8 * 8);
   if (p.ranges == 1) {
     gemm_int8_many_kernel<Q, T, false><<<grid, Q::WAVES * NS_WAVE, 0, stream>>>(a);

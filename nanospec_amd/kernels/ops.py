@@ -1255,6 +1255,7 @@ def silu_mul_int8(gu: torch.Tensor, take=None) -> Int8Rows:
 
 
 INT8_TILES = ((64, 64), (64, 128), (128, 64), (128, 128), (256, 128), (256, 256))  # rows of x by rows of the weight, as ``ns_gemm_int8_many`` numbers them
+INT8_JOIN_ROWS = 65535  # that ranges of K are joined for
 INT8_FEW_WORK = 5e7  # blocks of 16 rows of x times columns times K
 INT8_TILE_US = (2.02, 3.43, 3.01, 5.42, 7.30, 10.13)  # of a tile for 1,024 of K, and once a tile
 INT8_TILE_ONCE_US = (0.06, 0.16, 0.47, 0.15, 1.53, 4.09)
@@ -1274,7 +1275,7 @@ def int8_plan(m: int, n: int, k: int, units: int) -> tuple[int, int] | None:
     for form, (bm, bn) in enumerate(INT8_TILES):
         tiles = -(-m // bm) * -(-n // bn)
         for ranges in (1, 2, 3, 4, 6, 8):
-            if ranges > 1 and kp < ranges * INT8_K_MIN:
+            if ranges > 1 and (kp < ranges * INT8_K_MIN or m > INT8_JOIN_ROWS):
                 break
             us = max(3.8 + -(-tiles * ranges // units) * (INT8_TILE_US[form] * kp / (1024 * ranges) + INT8_TILE_ONCE_US[form]), 3.8 + n * kp / 5.2e6)
             us += 2.0 + ranges * m * n * 4 / 2.5e6 if ranges > 1 else 0.0

@@ -92,3 +92,10 @@ def test_models_refuse_products_that_are_not_built():
     net.layers[1].ffn = SimpleNamespace()
     with pytest.raises(ValueError, match="not built for SimpleNamespace"):
         net.load(None, torch.float32, "cpu", products="int8")
+
+
+def test_plans_of_more_rows_than_are_joined():
+    for m in (65535, 65536, 200_000):
+        for n, k in ((17, 32768), (64, 8192), (4096, 4096)):
+            plan = ops.int8_plan(m, n, k, 256)
+            assert plan is not None and (plan[1] == 1 or m <= ops.INT8_JOIN_ROWS)

@@ -201,3 +201,13 @@ def test_weight_from_values(n, k, dtype):
     most = w.double().abs().amax(1)
     assert bool(((scales - most / 127).abs() <= 2.0**-23 * most).all())
     assert bool(((codes * scales[:, None] - w.double()).abs() <= scales[:, None] * (0.5 + 127 * 2.0**-22)).all()) and not bool(codes[n // 2].any())
+
+
+@pytest.mark.parametrize("m,n,k", [(65536, 130, 600), (70001, 200, 520), (1_048_600, 17, 64)])
+def test_product_of_more_rows_than_a_grid_has_of_them(m, n, k):
+    """Rows beyond 65,535, in tiles and, of a small weight, 16 at a time up to the rows that that kernel's grid has; sums below 2^24 are exact in 32-bit too."""
+    ops = _ops()
+    codes = torch.randint(-127, 128, (m, k), generator=torch.Generator().manual_seed(1), dtype=torch.int8).to(DEV)
+    w = torch.randint(-127, 128, (n, k), generator=torch.Generator().manual_seed(2), dtype=torch.int8).to(DEV)
+    y = ops.linear_int8(ops.Int8Rows.from_codes(codes, torch.ones(m, device=DEV)), ops.Int8Weight(w, torch.ones(n, device=DEV)), dtype=torch.float32)
+    assert torch.equal(y, codes.float() @ w.float().T)
