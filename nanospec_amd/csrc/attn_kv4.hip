@@ -188,19 +188,23 @@ extern "C" int ns_attn_kv4_plain(void* out, void* part_o, void* part_l, const vo
 #include "attn_kv4_mfma.h"
 
 template <typename T, int HD, int PARTS>
-static int launch_tiles(const Kv4AttnParams& a, int rows, int wave_tokens, hipStream_t stream) {
+static int launch_tiles(const Kv4AttnParams& a, int rows, int form, hipStream_t stream) {
   const int group = a.heads / a.kv_heads;
   if (rows) {
     if (a.n_tiles > 65535) return NS_ERR_UNSUPPORTED;
-    attn_kv4_rows_kernel<T, HD, PARTS><<<dim3((unsigned)(a.kv_heads * ((group + 15) / 16)), (unsigned)a.n_tiles, (unsigned)a.splits), KV4_ROW_WAVES * NS_WAVE, 0, stream>>>(a);
+    const dim3 grid((unsigned)(a.kv_heads * ((group + 15) / 16)), (unsigned)a.n_tiles, (unsigned)a.splits);
+    if (form == 8)
+      attn_kv4_rows_kernel<T, HD, PARTS, 8><<<grid, 512, 0, stream>>>(a);
+    else
+      attn_kv4_rows_kernel<T, HD, PARTS, 4><<<grid, 256, 0, stream>>>(a);
   } else {
-    const long long items = (long long)a.n_tiles * a.splits * a.heads * (KV4_TILE_TOKENS / wave_tokens);
+    const long long items = (long long)a.n_tiles * a.splits * a.heads * (KV4_TILE_TOKENS / form);
     if (items > 0x7fffffff - 4) return NS_ERR_UNSUPPORTED;
     const unsigned grid = (unsigned)((items + 3) / 4);
     if constexpr (PARTS == 1) {
-      if (wave_tokens == 32) attn_kv4_tiles_kernel<T, HD, 2, PARTS><<<grid, 256, 0, stream>>>(a);
+      if (form == 32) attn_kv4_tiles_kernel<T, HD, 2, PARTS><<<grid, 256, 0, stream>>>(a);
     }
-    if (wave_tokens == 16) attn_kv4_tiles_kernel<T, HD, 1, PARTS><<<grid, 256, 0, stream>>>(a);
+    if (form == 16) attn_kv4_tiles_kernel<T, HD, 1, PARTS><<<grid, 256, 0, stream>>>(a);
   }
   if (a.splits > 1) {
     const long long cols = (long long)a.n_tiles * (rows ? 1 : KV4_TILE_TOKENS) * a.heads;
@@ -211,20 +215,21 @@ static int launch_tiles(const Kv4AttnParams& a, int rows, int wave_tokens, hipSt
 }
 
 // Attention of the tokens that ``tiles`` [n_tiles][8] names: request, first token of the tile among the request's tokens of this step, row of the request's first token, tokens of the
-// request in this step, keys after it, one more, of single tokens the blocks of 32 keys of all of them, one more.  rows 1: a tile is one token; 0: up to 32, of which a wave takes wave_tokens (16; with bfloat16 also 32).  part_o: float32 [n_tiles * tokens of a tile * heads * splits * hd] and part_l
+// request in this step, keys after it, one more, of single tokens the blocks of 32 keys of all of them, one more.  rows 1: a tile is one token, and a workgroup has ``form`` waves (4, 8); 0: up to 32 tokens, of which a
+// wave takes ``form`` (16; with bfloat16 also 32).  part_o: float32 [n_tiles * tokens of a tile * heads * splits * hd] and part_l
 // [n_tiles * tokens of a tile * heads * splits] with splits > 1.
 extern "C" int ns_attn_kv4(void* out, void* part_o, void* part_l, const void* q, int q_stride, const void* pool, const int* tiles, const int* block_table, int table_stride,
-                           int n_tiles, int heads, int kv_heads, int hd, int page, int rows, int wave_tokens, int splits, int groups, int window, float scale, int dtype, hipStream_t stream) {
+                           int n_tiles, int heads, int kv_heads, int hd, int page, int rows, int form, int splits, int groups, int window, float scale, int dtype, hipStream_t stream) {
   if (n_tiles < 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads || page < KV4_TOKENS || (page & (page - 1)) || window < 0) return NS_ERR_BAD_ARG;
   if (splits < 1 || splits > 64 || (splits > 1 && (!part_o || !part_l)) || groups < 1) return NS_ERR_BAD_ARG;
-  if (!rows && wave_tokens != 16 && (wave_tokens != 32 || dtype == NS_DTYPE_F32)) return NS_ERR_BAD_ARG;
+  if (rows ? form != 4 && form != 8 : form != 16 && (form != 32 || dtype == NS_DTYPE_F32)) return NS_ERR_BAD_ARG;
   if (hd != 64 && hd != 128) return NS_ERR_UNSUPPORTED;
   if ((((uintptr_t)out | (uintptr_t)pool | (uintptr_t)part_o) & 15) != 0) return NS_ERR_UNSUPPORTED;
   if (n_tiles == 0) return NS_OK;
   const Kv4AttnParams a{out, (float*)part_o, (float*)part_l, q, (const uint8_t*)pool, tiles, nullptr, nullptr, block_table, q_stride, table_stride, n_tiles, heads, kv_heads,
                         hd, page, splits, window, groups, scale * 1.4426950408889634f,
                         ((uintptr_t)q & 15) == 0 && q_stride % (dtype == NS_DTYPE_F32 ? 4 : 8) == 0};
-  if (dtype == NS_DTYPE_F32) return hd == 64 ? launch_tiles<float, 64, 2>(a, rows, wave_tokens, stream) : launch_tiles<float, 128, 2>(a, rows, wave_tokens, stream);
-  if (dtype == NS_DTYPE_BF16) return hd == 64 ? launch_tiles<bf16_t, 64, 1>(a, rows, wave_tokens, stream) : launch_tiles<bf16_t, 128, 1>(a, rows, wave_tokens, stream);
+  if (dtype == NS_DTYPE_F32) return hd == 64 ? launch_tiles<float, 64, 2>(a, rows, form, stream) : launch_tiles<float, 128, 2>(a, rows, form, stream);
+  if (dtype == NS_DTYPE_BF16) return hd == 64 ? launch_tiles<bf16_t, 64, 1>(a, rows, form, stream) : launch_tiles<bf16_t, 128, 1>(a, rows, form, stream);
   return NS_ERR_UNSUPPORTED;
 }

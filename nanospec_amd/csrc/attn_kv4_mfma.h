@@ -29,7 +29,6 @@ typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 #define KV4_TILE_INTS 8
 #define KV4_TILE_TOKENS 32  // of a portion's tile
 #define KV4_SLACK 8.f
-#define KV4_ROW_WAVES 4
 #define KV4_RANGE_BLOCKS 8  // of 32 keys: the fewest of a range of a single token's keys
 
 __device__ __forceinline__ f16x8 as_f16x8(uint32_t a, uint32_t b, uint32_t c, uint32_t d) { return __builtin_bit_cast(f16x8, u32x4{a, b, c, d}); }
@@ -319,12 +318,10 @@ struct Kv4Wave {
 // Single tokens: a workgroup a (token, key/value head, 16 query heads of its group, range of keys), whose waves take blocks of 32 keys in turn and meet in LDS.  Ranges are even and as many
 // as give ``a.groups`` workgroups over all tokens: a row twice as long as others has twice as many.
 // Bound by memory where the rows are long and many (61 rows of 200 to 12,000 keys, 8 key/value heads of 128 channels: 94 us, 4.2 TB/s; 64 rows of 6,000: 5.3), by one workgroup's
-// chain of loads where they are few (a row of 1,100: 8.7 us).  Two blocks on their way at a time were slower everywhere (their registers cost a wave a SIMD), eight waves a workgroup too but
-// for eight (row, head)s of 32,000 keys (19 for 24 us).
-template <typename T, int HD, int PARTS>
-__global__ __launch_bounds__(KV4_ROW_WAVES * 64) __attribute__((amdgpu_waves_per_eu(2))) void attn_kv4_rows_kernel(const Kv4AttnParams a) {
+// chain of loads where they are few (a row of 1,000, in eight waves: 9.3 us).  Two blocks on their way at a time were slower everywhere (their registers cost a wave a SIMD).
+template <typename T, int HD, int PARTS, int WAVES>
+__global__ __launch_bounds__(WAVES * 64) __attribute__((amdgpu_waves_per_eu(2))) void attn_kv4_rows_kernel(const Kv4AttnParams a) {
   typedef Kv4Wave<T, HD, 1, PARTS> Wave;
-  constexpr int WAVES = KV4_ROW_WAVES;
   __shared__ float outs[WAVES][16][HD + 4];
   __shared__ float weights[WAVES][16];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / NS_WAVE);

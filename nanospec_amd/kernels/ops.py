@@ -74,6 +74,27 @@ def compute_units(device) -> int:
     return _units[index]
 
 
+def _units_of(t: torch.Tensor) -> int:
+    """``compute_units`` of a GPU tensor's device."""
+    return _units.get(t.get_device()) or compute_units(t.device)
+
+
+_KINDS = {"p": c_void_p, "i": c_int, "f": c_float}
+
+
+@functools.lru_cache(maxsize=None)
+def _entry(name: str, kinds: str):
+    """A C entry that takes plain integers and floats: ``kinds`` names its arguments, p an address, i an int, f a float.  (Twenty arguments wrapped one by one take a call 3 us, which a step
+    that is launched kernel by kernel waits for.)"""
+    fn = getattr(build.core(), name)
+    fn.argtypes = [_KINDS[k] for k in kinds]
+    return fn
+
+
+def _address(t) -> int:
+    return 0 if t is None else t.data_ptr()
+
+
 def _i32(t: torch.Tensor, name: str) -> torch.Tensor:
     if t.dtype != torch.int32 or not t.is_contiguous():
         raise KernelRefused(f"{name} must be a contiguous int32 tensor")
@@ -1210,13 +1231,18 @@ class Int8Rows:
 
 
 def _int8_rows(x: torch.Tensor, k: int, src: int, take, what: str, resid=None, resid_out=None, weight=None, eps: float = 0.0) -> Int8Rows:
-    m, width = x.shape[0], 2 * k if src == 2 else k
-    if not 1 <= k <= INT8_MAX_K or x.shape[1] != width or (m > 1 and x.stride(0) < width) or (m and x.stride(1) != 1):
+    m, width = x.shape
+    stride, step = x.stride()
+    if not 1 <= k <= INT8_MAX_K or width != (2 * k if src == 2 else k) or (m > 1 and stride < width) or (m and step != 1):
         raise KernelRefused(f"{what}: rows of up to {INT8_MAX_K} values with unit stride along a row; got {tuple(x.shape)}")
-    take = take or (lambda shape, dtype: torch.empty(shape, dtype=dtype, device=x.device))
-    rows = Int8Rows(take((-(-m // 16), int8_padded_k(k) // 64, 4, 16, 16), torch.int8), take((m,), torch.float32), k)
-    _check(build.core().ns_int8_rows(_ptr(rows.data), _ptr(rows.scales), _ptr(x), c_int(max(x.stride(0), width)), _ptr(resid), _ptr(resid_out), _ptr(weight), c_float(eps), c_int(m),
-                                     c_int(k), c_int(int8_padded_k(k)), c_int(src), c_int(_dtype_code(x)), _stream()), what)
+    kp, code = int8_padded_k(k), _dtype_code(x)
+    shape = (-(-m // 16), kp // 64, 4, 16, 16)
+    if take is None:
+        rows = Int8Rows(torch.empty(shape, dtype=torch.int8, device=x.device), torch.empty(m, dtype=torch.float32, device=x.device), k)
+    else:
+        rows = Int8Rows(take(shape, torch.int8), take((m,), torch.float32), k)
+    _check(_entry("ns_int8_rows", "pppipppfiiiiip")(rows.data.data_ptr(), rows.scales.data_ptr(), x.data_ptr(), max(stride, width), _address(resid), _address(resid_out), _address(weight), eps,
+                                                   m, k, kp, src, code, _stream()), what)
     return rows
 
 
@@ -1289,27 +1315,28 @@ def linear_int8(x: Int8Rows, w: Int8Weight, out: torch.Tensor | None = None, dty
     (shape, dtype) gives scratch (``ctx.arena.take``)."""
     if not isinstance(x, Int8Rows) or not isinstance(w, Int8Weight):
         raise KernelRefused("linear_int8 takes rows in 8 bits (int8_rows) and an Int8Weight")
-    _gpu(x.data, w.data, out)
-    m = x.scales.shape[0]
-    if x.k != w.k or x.data.shape != (-(-m // 16), w.kp // 64, 4, 16, 16) or x.data.dtype != torch.int8 or not x.data.is_contiguous() or x.scales.shape != (m,) or x.scales.dtype != torch.float32:
+    data, scales = x.data, x.scales
+    _gpu(data, scales, w.data, out)
+    m, n = scales.shape[0], w.n
+    if x.k != w.k or data.shape != (-(-m // 16), w.kp // 64, 4, 16, 16) or data.dtype != torch.int8 or not data.is_contiguous() or scales.dim() != 1 or scales.dtype != torch.float32:
         raise KernelRefused(f"linear_int8: rows of {x.k}, a weight of {w.k}")
     if out is None:
-        out = torch.empty((m, w.n), dtype=dtype, device=x.data.device)
-    if out.shape != (m, w.n) or (m and out.stride(1) != 1) or (m > 1 and out.stride(0) < w.n):
-        raise KernelRefused(f"linear_int8: out must be [{m}, {w.n}] with unit stride along a row")
+        out = torch.empty((m, n), dtype=dtype, device=data.device)
+    stride, step = out.stride() if out.dim() == 2 else (0, 0)
+    if out.shape != (m, n) or (m and step != 1) or (m > 1 and stride < n):
+        raise KernelRefused(f"linear_int8: out must be [{m}, {n}] with unit stride along a row")
     code = _dtype_code(out)
-    lib, common = build.core(), (c_int(m), c_int(w.n), c_int(w.kp), c_int(max(out.stride(0), w.n)))
-    operands = (_ptr(x.data), _ptr(x.scales), _ptr(w.data), _ptr(w.scales))
-    plan = int8_plan(m, w.n, w.k, compute_units(out.device))
+    operands = (data.data_ptr(), scales.data_ptr(), w.data.data_ptr(), w.scales.data_ptr(), m, n, w.kp, max(stride, n))
+    plan = int8_plan(m, n, w.k, _units_of(out))
     if plan is None:
-        _check(lib.ns_gemm_int8(_ptr(out), *operands, *common, c_int(code), _stream()), "linear_int8")
+        _check(_entry("ns_gemm_int8", "pppppiiiiip")(out.data_ptr(), *operands, code, _stream()), "linear_int8")
         return out
     form, ranges = plan
     parts = None
     if ranges > 1:
-        shape = (ranges * m * (-(-w.n // 4) * 4),)
+        shape = (ranges * m * (-(-n // 4) * 4),)
         parts = take(shape, torch.int32) if take is not None else torch.empty(shape, dtype=torch.int32, device=out.device)
-    _check(lib.ns_gemm_int8_many(_ptr(out), _ptr(parts), *operands, *common, c_int(form), c_int(ranges), c_int(code), _stream()), "linear_int8")
+    _check(_entry("ns_gemm_int8_many", "ppppppiiiiiiip")(out.data_ptr(), _address(parts), *operands, form, ranges, code, _stream()), "linear_int8")
     return out
 
 
@@ -1340,6 +1367,7 @@ class Kv4Pages:
             raise KernelRefused("4-bit pages begin at a multiple of 16 bytes")
         self.pool, self.head_dim = pool, head_dim
         self.pages, self.kv_heads, self.page = pool.shape[0], pool.shape[1], pool.shape[2] * KV4_TOKENS
+        self.records = pool.shape[0] * pool.shape[1] * pool.shape[2]
 
     @staticmethod
     def shape(pages: int, kv_heads: int, page: int, head_dim: int) -> tuple[int, int, int, int]:
@@ -1423,29 +1451,30 @@ def rope_kv4_write(qkv: torch.Tensor, positions: torch.Tensor, token_req: torch.
     if rotary_dim % 2 or not 0 <= rotary_dim <= head_dim or inv_freq.dtype != torch.float32 or not inv_freq.is_contiguous() or inv_freq.numel() < rotary_dim // 2:
         raise KernelRefused("rope_kv4_write: the rotary part is an even number of a head's channels, inv_freq holds rotary_dim/2 float32 values")
     to = qkv if q_out is None else q_out
-    _check(build.core().ns_rope_kv4_write(_ptr(qkv), c_int(qkv.stride(0)), _ptr(to), c_int(to.stride(0)), _ptr(positions), _ptr(token_req), _ptr(block_table),
-                                          c_int(block_table.stride(0)), _ptr(inv_freq), _ptr(pages.pool), c_int(n), c_int(heads), c_int(kv_heads), c_int(head_dim),
-                                          c_int(rotary_dim), c_int(1 if interleaved else 0), c_float(factor), c_int(pages.page), c_int(1 if write_kv else 0),
-                                          c_int(_dtype_code(qkv)), _stream()), "rope_kv4_write")
+    _check(_entry("ns_rope_kv4_write", "pipipppippiiiiiifiiip")(qkv.data_ptr(), qkv.stride(0), to.data_ptr(), to.stride(0), positions.data_ptr(), token_req.data_ptr(),
+                                                              block_table.data_ptr(), block_table.stride(0), inv_freq.data_ptr(), pages.pool.data_ptr(), n, heads, kv_heads, head_dim,
+                                                              rotary_dim, 1 if interleaved else 0, factor, pages.page, 1 if write_kv else 0, _dtype_code(qkv), _stream()), "rope_kv4_write")
 
 
 def kv4_read(pages: Kv4Pages, positions: torch.Tensor, token_req: torch.Tensor, block_table: torch.Tensor, dtype: torch.dtype = torch.bfloat16):
     """-> (keys, values) [N, kv_heads, head_dim] of the tokens at ``positions`` of requests ``token_req`` as the pages hold them (keys rotated), rounded once to ``dtype``."""
+    if not isinstance(pages, Kv4Pages):
+        raise KernelRefused("kv4_read takes 4-bit pages (Kv4Pages)")
     n = _check_kv4(pages, positions, token_req, block_table, pages.kv_heads, pages.head_dim, "kv4_read")
     k, v = (torch.empty((n, pages.kv_heads, pages.head_dim), dtype=dtype, device=pages.pool.device) for _ in range(2))
-    _check(build.core().ns_kv4_read(_ptr(k), _ptr(v), _ptr(pages.pool), _ptr(positions), _ptr(token_req), _ptr(block_table), c_int(block_table.stride(0)), c_int(n),
-                                    c_int(pages.kv_heads), c_int(pages.head_dim), c_int(pages.page), c_int(_dtype_code(k)), _stream()), "kv4_read")
+    _check(_entry("ns_kv4_read", "ppppppiiiiiip")(k.data_ptr(), v.data_ptr(), pages.pool.data_ptr(), positions.data_ptr(), token_req.data_ptr(), block_table.data_ptr(), block_table.stride(0),
+                                                 n, pages.kv_heads, pages.head_dim, pages.page, _dtype_code(k), _stream()), "kv4_read")
     return k, v
 
 
 def _check_kv4_attn(q, out, pages: Kv4Pages, heads: int, kv_heads: int, head_dim: int, window: int, splits: int, workspace, cols: int, what: str):
     _gpu(q, out)
-    n = q.shape[0]
     if heads < 1 or kv_heads < 1 or heads % kv_heads:
         raise KernelRefused(f"{what}: {heads} heads are not a multiple of {kv_heads} key/value heads")
     if pages.kv_heads != kv_heads or pages.head_dim != head_dim:
         raise KernelRefused(f"{what}: pages of {pages.kv_heads} heads of {pages.head_dim}, asked for {kv_heads} of {head_dim}")
-    if q.dim() != 2 or q.shape[1] < heads * head_dim or (n and q.stride(1) != 1):
+    n, width = q.shape if q.dim() == 2 else (0, 0)
+    if width < heads * head_dim or (n and q.stride(1) != 1):
         raise KernelRefused(f"{what}: q must be [tokens, at least {heads * head_dim}]")
     if out.shape != (n, heads * head_dim) or out.dtype != q.dtype or not out.is_contiguous():
         raise KernelRefused(f"{what}: out must be contiguous [{n}, {heads * head_dim}] of q's dtype")
@@ -1468,11 +1497,11 @@ def kv4_tiles_take(head_dim: int) -> bool:
 
 
 def attention_kv4(q, out, pages: Kv4Pages, tiles, block_table, heads: int, kv_heads: int, head_dim: int, scale: float, rows: bool, window: int = 0, splits: int = 1,
-                  workspace: tuple[torch.Tensor, torch.Tensor] | None = None, groups: int = 1, wave_tokens: int = 16) -> torch.Tensor:
+                  workspace: tuple[torch.Tensor, torch.Tensor] | None = None, groups: int = 1, form: int = 0) -> torch.Tensor:
     """Attention over 4-bit pages on the matrix cores, head sizes 64 and 128, bfloat16 and float32, of the tokens that ``tiles`` (int32 [n_tiles, 8], as for ``attention_mfma``) describe:
     with ``rows`` single tokens, a tile each, otherwise portions in tiles of up to 32 tokens.  Tokens that no tile describes are left as they are.  ``splits`` > 1 cuts the keys of every tile into
     that many ranges and needs ``workspace`` = float32 tensors of columns * splits * head_dim and columns * splits values, columns = tiles * (1 or 32) * heads.  Single tokens
-    use as many of their ranges as make about ``groups`` workgroups of all tokens' keys.  A wave takes ``wave_tokens`` of a portion's tile, 16 or, of bfloat16, 32."""
+    use as many of their ranges as make about ``groups`` workgroups of all tokens' keys.  ``form``: the waves of a workgroup for single tokens (4 or 8), the tokens of a portion's tile that a wave takes (16 or, of bfloat16, 32)."""
     if not isinstance(pages, Kv4Pages):
         raise KernelRefused("attention_kv4 takes 4-bit pages (Kv4Pages)")
     if not kv4_tiles_take(head_dim):
@@ -1482,15 +1511,16 @@ def attention_kv4(q, out, pages: Kv4Pages, tiles, block_table, heads: int, kv_he
     _kv4_table(block_table, "attention_kv4")
     if tiles.dim() != 2 or tiles.shape[1] != TILE_INTS:
         raise KernelRefused(f"attention_kv4: tiles must be int32 [n_tiles, {TILE_INTS}]")
-    if groups < 1 or pages.pool.numel() // pages.pool.shape[3] >= 1 << 31:
+    if groups < 1 or pages.records >= 1 << 31:
         raise KernelRefused("attention_kv4: at least one workgroup, and fewer than 2^31 records in the pool")
-    if wave_tokens not in (16, 32) or (wave_tokens == 32 and q.dtype == torch.float32):
-        raise KernelRefused("attention_kv4: a wave takes 16 tokens, of bfloat16 also 32")
+    form = form or (4 if rows else 16)
+    if form not in ((4, 8) if rows else (16,) if q.dtype == torch.float32 else (16, 32)):
+        raise KernelRefused("attention_kv4: a workgroup has 4 or 8 waves for single tokens; a wave takes 16 tokens of a portion, of bfloat16 also 32")
     n_tiles = tiles.shape[0]
     po, pl = _check_kv4_attn(q, out, pages, heads, kv_heads, head_dim, window, splits, workspace, n_tiles * (1 if rows else 32) * heads, "attention_kv4")
-    _check(build.core().ns_attn_kv4(_ptr(out), _ptr(po), _ptr(pl), _ptr(q), c_int(q.stride(0)), _ptr(pages.pool), _ptr(tiles), _ptr(block_table), c_int(block_table.stride(0)),
-                                    c_int(n_tiles), c_int(heads), c_int(kv_heads), c_int(head_dim), c_int(pages.page), c_int(1 if rows else 0), c_int(wave_tokens), c_int(splits),
-                                    c_int(groups), c_int(window), c_float(scale), c_int(_dtype_code(q)), _stream()), "attention_kv4")
+    _check(_entry("ns_attn_kv4", "ppppipppiiiiiiiiiiifip")(out.data_ptr(), _address(po), _address(pl), q.data_ptr(), q.stride(0), pages.pool.data_ptr(), tiles.data_ptr(),
+                                                           block_table.data_ptr(), block_table.stride(0), n_tiles, heads, kv_heads, head_dim, pages.page, 1 if rows else 0, form,
+                                                           splits, groups, window, scale, _dtype_code(q), _stream()), "attention_kv4")
     return out
 
 

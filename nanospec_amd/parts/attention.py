@@ -39,6 +39,10 @@ KV4_NARROW_KEYS = 4096
 # Workgroups of four waves that single tokens' keys are cut for, for each compute unit.  Of 1, 2, 3 and 4: 8 rows of 4,000 keys 18.2, 17.6, 20.6, 21.4; 61 of 200 to 12,000 89, 93, 95, 90;
 # 2 of 100,000 (64 heads) 64, 62, 67, 70; one of 32,000 20, 24, 24, 24; 64 of 6,000 (64 channels) 67, 62, 62, 65.
 KV4_GROUPS_PER_UNIT = 2
+# Rows are not cut, and nothing is joined, up to the first of these keys, or, of many (row, key/value head)s, up to so many keys for each of them, but to no more than the last.  Cut, and whole with 8
+# waves a workgroup (with 4): 1 row of 1,000 keys 10.4, 9.3 (10.5), of 1,500 9.9, 11.2 (13.5); 8 of 1,000 10.9, 10.8 (12.8); 16 of 2,000 16.8, 17.0 (22.5); 32 of 4,000 36.1, 30.9 (42.4);
+# 64 of 500 19.3, 16.0 (12.7), of 2,000 38.1, 32.8 (30.5).  Whole rows have 8 waves where there are no more of them than compute units.
+KV4_WHOLE_KEYS = 1152, 16, 4096
 QKV_JOIN_MAX_RANGES = 4  # 17 to 128 rows: the kernel that joins the ranges of the q/k/v product, rotates and writes the cache reads
 #                          every range, so more of them cost it what they gain the product
 
@@ -94,9 +98,12 @@ class TilePlan:
     @staticmethod
     def views(ctx):
         """-> (portion tiles, one-token tiles) as int32 [tiles, TILE_INTS] device views."""
-        region, (tc, td) = ctx.plans[TilePlan.key]
-        cut = ops.TILE_INTS * tc
-        return region[:cut].view(tc, ops.TILE_INTS), region[cut : cut + ops.TILE_INTS * td].view(td, ops.TILE_INTS)
+        views = getattr(ctx, "tile_views", None)  # (every layer of the step asks)
+        if views is None:
+            region, (tc, td) = ctx.plans[TilePlan.key]
+            cut = ops.TILE_INTS * tc
+            views = ctx.tile_views = region[:cut].view(tc, ops.TILE_INTS), region[cut : cut + ops.TILE_INTS * td].view(td, ops.TILE_INTS)
+        return views
 
 
 TILES = TilePlan()
@@ -239,7 +246,7 @@ def f32_attention(ctx, q, out, cache, table, heads: int, kv_heads: int, head_dim
 def kv4_attention(ctx, q, out, pages, table, heads: int, kv_heads: int, head_dim: int, scale: float, window: int = 0) -> torch.Tensor:
     """Attention of the batch's tokens over pages of 4 bits (``ops.Kv4Pages``): head sizes 64 and 128 on the matrix cores, portions and single tokens by their tiles, others in plain
     32-bit arithmetic.  A batch without tiles has its tokens all in the latter."""
-    take, units, group = ctx.arena.take, ops.compute_units(q.device), heads // kv_heads
+    take, units, group = ctx.arena.take, ops._units_of(q), heads // kv_heads
     span = window or 1 << 30
 
     def workspace(columns: int, splits: int):
@@ -258,15 +265,17 @@ def kv4_attention(ctx, q, out, pages, table, heads: int, kv_heads: int, head_dim
         # ranges until there are eight waves for each compute unit, if there are not without
         waves, least, most = tiles * heads * (TilePlan.TOKENS // wave_tokens), *KV4_PORTION_KEYS
         splits = 1 if waves >= 8 * units else max(1, min(KV4_MAX_RANGES, max(-(-8 * units // waves), -(-longest // most)), longest // least))
-        ops.attention_kv4(q, out, pages, portions, table, heads, kv_heads, head_dim, scale, rows=False, window=window, splits=splits, wave_tokens=wave_tokens,
+        ops.attention_kv4(q, out, pages, portions, table, heads, kv_heads, head_dim, scale, rows=False, window=window, splits=splits, form=wave_tokens,
                           workspace=workspace(tiles * TilePlan.TOKENS * heads, splits))
     if singles.shape[0]:
         tiles, longest = singles.shape[0], min(ctx.max_kv_len, span)
-        # the kernel cuts each row by the keys that all of them have, so that it comes to about ``groups`` workgroups; here is said how often it may at most
         items = tiles * kv_heads * -(-group // 16)
+        base, each, most = KV4_WHOLE_KEYS
+        whole = longest <= min(most, max(base, each * items))
+        # cut: the kernel cuts each row by the keys that all of them have, so that it comes to about ``groups`` workgroups; here is said how often it may at most
         groups = KV4_GROUPS_PER_UNIT * units
-        splits = max(1, min(KV4_MAX_RANGES, 2 + 4 * groups // items, -(-longest // KV4_RANGE_KEYS)))
-        ops.attention_kv4(q, out, pages, singles, table, heads, kv_heads, head_dim, scale, rows=True, window=window, splits=splits, groups=groups,
+        splits = 1 if whole else max(1, min(KV4_MAX_RANGES, 2 + 4 * groups // items, -(-longest // KV4_RANGE_KEYS)))
+        ops.attention_kv4(q, out, pages, singles, table, heads, kv_heads, head_dim, scale, rows=True, window=window, splits=splits, groups=groups, form=8 if whole and items <= units else 4,
                           workspace=workspace(tiles * heads, splits))
     return out
 
