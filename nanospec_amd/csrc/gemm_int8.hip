@@ -152,8 +152,8 @@ extern "C" int ns_int8_rows(void* codes, float* scales, const void* x, int x_str
 }
 
 // ------------------------------------------------------------------------------------------------------------------------------------
-// Few rows: the weight streams, a workgroup a tile of 16 of its rows and 16 of x, its waves the pieces of K in turn; their sums meet in LDS.  Bound by memory: 16 rows of 28,672 x 4,096
-// 21 us, 5.6 TB/s of weights.
+// Few rows: the weight streams, a workgroup a tile of 16 of its rows and 16 RB of x, its waves the pieces of K in turn; their sums meet in LDS.  Bound by memory with up to 16 rows: of
+// 28,672 x 4,096 21 us, 5.6 TB/s of weights; with more by what a compute unit reads of both operands, some 60 bytes a ns (64 rows of 4,096 x 4,096 in RB 1, 2, 4: 12.8, 9.8, 8.1 us).
 struct Int8Params {
   void* out;
   const int8_t *x, *w;
@@ -184,59 +184,80 @@ __device__ __forceinline__ void int8_store(const Int8Params& p, int row, int col
 }
 
 // AHEAD: pieces of a wave whose loads are on their way at a time.  Eight from K 4,096 on (16 rows of 4,096 x 4,096 5.1 us, four 5.3; of 57,344 x 8,192 78.0 and 78.9), four below
-// (16,384 x 2,048 7.9, eight 10.5: half of them beyond the end).
-template <typename T, int WAVES, int AHEAD>
+// (16,384 x 2,048 7.9, eight 10.5: half of them beyond the end), and four with more rows (64 rows of 4,096 x 14,336 21.6, eight 23.3).
+template <typename T, int WAVES, int AHEAD, int RB>
 __global__ __launch_bounds__(WAVES * 64) void gemm_int8_few_kernel(const Int8Params p) {
-  __shared__ i32x4 sums[WAVES][64];
+  __shared__ i32x4 sums[WAVES][RB][64];
   const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), r = lane % 16, g = lane / 16;
-  const int m0 = blockIdx.y * 16, pieces = p.KP / 64;
+  const int m0 = blockIdx.y * 16 * RB, pieces = p.KP / 64, blocks = (p.M - 1 - m0) / 16 + 1;
   const i32x4* w = reinterpret_cast<const i32x4*>(p.w + (size_t)blockIdx.x * 16 * p.KP) + lane;
-  const i32x4* x = reinterpret_cast<const i32x4*>(p.x + (size_t)m0 * p.KP) + lane;
-  i32x4 acc = {0, 0, 0, 0};
+  const i32x4* x[RB];  // (row blocks beyond the last are the last; their sums are not written)
+#pragma unroll
+  for (int i = 0; i < RB; ++i) x[i] = reinterpret_cast<const i32x4*>(p.x + (size_t)(m0 + 16 * min(i, blocks - 1)) * p.KP) + lane;
+  i32x4 acc[RB];
+#pragma unroll
+  for (int i = 0; i < RB; ++i) acc[i] = i32x4{0, 0, 0, 0};
   int kc = wave;
-  i32x4 a[AHEAD], b[AHEAD];
+  i32x4 a[AHEAD], b[AHEAD][RB];
   for (; kc + (AHEAD - 1) * WAVES < pieces; kc += AHEAD * WAVES) {
 #pragma unroll
-    for (int u = 0; u < AHEAD; ++u) a[u] = __builtin_nontemporal_load(w + (size_t)(kc + u * WAVES) * 64), b[u] = x[(size_t)(kc + u * WAVES) * 64];
+    for (int u = 0; u < AHEAD; ++u) {
+      a[u] = __builtin_nontemporal_load(w + (size_t)(kc + u * WAVES) * 64);
 #pragma unroll
-    for (int u = 0; u < AHEAD; ++u) acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(a[u], b[u], acc, 0, 0, 0);
+      for (int i = 0; i < RB; ++i) b[u][i] = x[i][(size_t)(kc + u * WAVES) * 64];
+    }
+#pragma unroll
+    for (int u = 0; u < AHEAD; ++u)
+#pragma unroll
+      for (int i = 0; i < RB; ++i) acc[i] = __builtin_amdgcn_mfma_i32_16x16x64_i8(a[u], b[u][i], acc[i], 0, 0, 0);
   }
   if (kc < pieces) {  // the rest (beyond it the last piece is read once more and not multiplied)
 #pragma unroll
     for (int u = 0; u < AHEAD; ++u) {
       const int at = min(kc + u * WAVES, pieces - 1);
-      a[u] = __builtin_nontemporal_load(w + (size_t)at * 64), b[u] = x[(size_t)at * 64];
+      a[u] = __builtin_nontemporal_load(w + (size_t)at * 64);
+#pragma unroll
+      for (int i = 0; i < RB; ++i) b[u][i] = x[i][(size_t)at * 64];
     }
 #pragma unroll
     for (int u = 0; u < AHEAD; ++u)
-      if (kc + u * WAVES < pieces) acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(a[u], b[u], acc, 0, 0, 0);
-  }
-  sums[wave][lane] = acc;
-  __syncthreads();
-  if (wave) return;
+      if (kc + u * WAVES < pieces)
 #pragma unroll
-  for (int v = 1; v < WAVES; ++v) acc += sums[v][lane];
-  const int row = m0 + r, col = blockIdx.x * 16 + 4 * g;
-  if (row < p.M && col < p.N) int8_store<T>(p, row, col, acc, p.xs[row]);
+        for (int i = 0; i < RB; ++i) acc[i] = __builtin_amdgcn_mfma_i32_16x16x64_i8(a[u], b[u][i], acc[i], 0, 0, 0);
+  }
+#pragma unroll
+  for (int i = 0; i < RB; ++i) sums[wave][i][lane] = acc[i];
+  __syncthreads();
+  if (wave >= RB) return;
+  i32x4 sum = sums[0][wave][lane];
+#pragma unroll
+  for (int v = 1; v < WAVES; ++v) sum += sums[v][wave][lane];
+  const int row = m0 + 16 * wave + r, col = blockIdx.x * 16 + 4 * g;
+  if (row < p.M && col < p.N) int8_store<T>(p, row, col, sum, p.xs[row]);
 }
 
 template <typename T>
-static int launch_int8_few(const Int8Params& p, hipStream_t stream) {
-  const dim3 grid((p.N + 15) / 16, (p.M + 15) / 16);
-  if (p.KP >= 4096)
-    gemm_int8_few_kernel<T, 8, 8><<<grid, 512, 0, stream>>>(p);
+static int launch_int8_few(const Int8Params& p, int blocks, hipStream_t stream) {
+  const dim3 grid((p.N + 15) / 16, (p.M + 16 * blocks - 1) / (16 * blocks));
+  if (blocks == 4)
+    gemm_int8_few_kernel<T, 8, 4, 4><<<grid, 512, 0, stream>>>(p);
+  else if (blocks == 2)
+    gemm_int8_few_kernel<T, 8, 4, 2><<<grid, 512, 0, stream>>>(p);
+  else if (p.KP >= 4096)
+    gemm_int8_few_kernel<T, 8, 8, 1><<<grid, 512, 0, stream>>>(p);
   else
-    gemm_int8_few_kernel<T, 8, 4><<<grid, 512, 0, stream>>>(p);
+    gemm_int8_few_kernel<T, 8, 4, 1><<<grid, 512, 0, stream>>>(p);
   return ns_launch_status();
 }
 
-extern "C" int ns_gemm_int8(void* out, const void* x, const float* xs, const void* w, const float* ws, int M, int N, int KP, int out_stride, int dtype, hipStream_t stream) {
-  if (M < 0 || N <= 0 || KP < 512 || KP % 256 || KP > INT8_MAX_K || out_stride < N) return NS_ERR_BAD_ARG;
+// ``blocks``: row blocks of 16 of a workgroup's tile, 1, 2 or 4.
+extern "C" int ns_gemm_int8(void* out, const void* x, const float* xs, const void* w, const float* ws, int M, int N, int KP, int out_stride, int blocks, int dtype, hipStream_t stream) {
+  if (M < 0 || N <= 0 || KP < 512 || KP % 256 || KP > INT8_MAX_K || out_stride < N || (blocks != 1 && blocks != 2 && blocks != 4)) return NS_ERR_BAD_ARG;
   if ((((uintptr_t)x | (uintptr_t)w | (uintptr_t)ws) & 15) || (M + 15) / 16 > 65535) return NS_ERR_UNSUPPORTED;
   if (M == 0) return NS_OK;
   const Int8Params p{out, (const int8_t*)x, (const int8_t*)w, xs, ws, M, N, KP, out_stride, 1, int8_quads(out, N, out_stride, dtype)};
-  if (dtype == NS_DTYPE_F32) return launch_int8_few<float>(p, stream);
-  if (dtype == NS_DTYPE_BF16) return launch_int8_few<bf16_t>(p, stream);
+  if (dtype == NS_DTYPE_F32) return launch_int8_few<float>(p, blocks, stream);
+  if (dtype == NS_DTYPE_BF16) return launch_int8_few<bf16_t>(p, blocks, stream);
   return NS_ERR_UNSUPPORTED;
 }
 

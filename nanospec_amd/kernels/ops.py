@@ -1282,28 +1282,38 @@ def silu_mul_int8(gu: torch.Tensor, take=None) -> Int8Rows:
 
 INT8_TILES = ((64, 64), (64, 128), (128, 64), (128, 128), (256, 128), (256, 256))  # rows of x by rows of the weight, as ``ns_gemm_int8_many`` numbers them
 INT8_JOIN_ROWS = 65535  # that ranges of K are joined for
-INT8_FEW_WORK = 5e7  # blocks of 16 rows of x times columns times K
 INT8_TILE_US = (2.02, 3.43, 3.01, 5.42, 7.30, 10.13)  # of a tile for 1,024 of K, and once a tile
 INT8_TILE_ONCE_US = (0.06, 0.16, 0.47, 0.15, 1.53, 4.09)
+INT8_FEW_RATES = {1: 47e3, 2: 53e3, 4: 60e3}  # bytes of both operands that a compute unit gets a us in the kernel for few rows, by its row blocks
+INT8_WEIGHT_RATE = 5.2e6  # bytes a us of a weight that streams
 
 
 @functools.lru_cache(maxsize=1 << 14)
-def int8_plan(m: int, n: int, k: int, units: int) -> tuple[int, int] | None:
-    """(tile, ranges of K) of a product of m rows and n columns in tiles, or None where the kernel for few rows is the faster one.
+def int8_plan(m: int, n: int, k: int, units: int) -> tuple[int, int]:
+    """(tile, ranges of K) of a product of m rows and n columns, or (-row blocks, 1) where the kernel for few rows is the faster one.
 
-    That one reads the weight once for every 16 rows, so it is taken up to 16 rows and as long as what it reads fits the caches.  us, it and the best tiles: 32 rows of 4,096 x 4,096 6.8 and 9.7, 48 8.5 and
-    10.1, 64 13.0 and 10.9; of 6,144 x 4,096 32 10.1 and 11.0, 48 15.0 and 12.2; of 2,048 x 2,048 128 6.4 and 7.6; of 16,384 x 2,048 16 8.3 and 9.0, 24 13.1 and 9.4.
-    The tiles are chosen by what they take, in us: 3.8, and for every round of as many tiles as there are units a tile's time, but no less than the weight at 5.2 TB/s; ranges of K 2.0 more, and their sums
-    at 2.5 TB/s.  Over 198 products (16 to 2,048 rows, 1,000 x 1,111 to 8,192 x 28,672) the choice takes 1.02 times as long as the best of all tiles and ranges, 1.27 at worst (1,500 rows of 12,288 x 3,000)."""
-    if m <= 16 or -(-m // 16) * n * k <= INT8_FEW_WORK:
-        return None
+    Chosen by what they take, in us.  The kernel for few rows, with 1, 2 or 4 blocks of 16 rows a workgroup: 2.6, and for every round of as many workgroups as there are units what they read of both operands at
+    ``INT8_FEW_RATES``.  Tiles: 3.8, and for every round a tile's time; ranges of K 2.0 more, and their sums at 2.5 TB/s.  Neither is faster than the weight streams (a quarter slower from few tiles).
+    Measured, it and the best tiles: 16 rows of 16,384 x 2,048 8.3 and 9.0; 32 of 4,096 x 4,096 6.5 and 10.0, 64 8.1 and 11.3, 96 12.4 and 11.3; 32 of 6,144 x 4,096 9.7 and 11.4, 64 13.4 and 12.8; 128 of
+    2,048 x 2,048 5.2 and 7.5; 64 of 4,096 x 14,336 21.6 and 17.5.  Over 198 products in tiles (16 to 2,048 rows, 1,000 x 1,111 to 8,192 x 28,672) the choice among those takes 1.02 times as long as the best of all tiles
+    and ranges, 1.27 at worst (1,500 rows of 12,288 x 3,000)."""
     kp, best = int8_padded_k(k), None
+    stream = n * kp / INT8_WEIGHT_RATE
+    for blocks, rate in INT8_FEW_RATES.items():
+        rows = -(-m // (16 * blocks))
+        if rows > INT8_JOIN_ROWS:  # (a grid's)
+            continue
+        us = 2.6 + max(-(-(-(-n // 16) * rows) // units) * kp * 16 * (1 + blocks) / rate, stream)
+        if best is None or us < best[0]:
+            best = us, -blocks, 1
+        if m <= 16 * blocks:
+            break
     for form, (bm, bn) in enumerate(INT8_TILES):
         tiles = -(-m // bm) * -(-n // bn)
         for ranges in (1, 2, 3, 4, 6, 8):
             if ranges > 1 and (kp < ranges * INT8_K_MIN or m > INT8_JOIN_ROWS):
                 break
-            us = max(3.8 + -(-tiles * ranges // units) * (INT8_TILE_US[form] * kp / (1024 * ranges) + INT8_TILE_ONCE_US[form]), 3.8 + n * kp / 5.2e6)
+            us = 3.8 + max(-(-tiles * ranges // units) * (INT8_TILE_US[form] * kp / (1024 * ranges) + INT8_TILE_ONCE_US[form]), stream / min(1, 0.7 + 0.3 * tiles * ranges / units))
             us += 2.0 + ranges * m * n * 4 / 2.5e6 if ranges > 1 else 0.0
             if best is None or us < best[0]:
                 best = us, form, ranges
@@ -1327,11 +1337,10 @@ def linear_int8(x: Int8Rows, w: Int8Weight, out: torch.Tensor | None = None, dty
         raise KernelRefused(f"linear_int8: out must be [{m}, {n}] with unit stride along a row")
     code = _dtype_code(out)
     operands = (data.data_ptr(), scales.data_ptr(), w.data.data_ptr(), w.scales.data_ptr(), m, n, w.kp, max(stride, n))
-    plan = int8_plan(m, n, w.k, _units_of(out))
-    if plan is None:
-        _check(_entry("ns_gemm_int8", "pppppiiiiip")(out.data_ptr(), *operands, code, _stream()), "linear_int8")
+    form, ranges = int8_plan(m, n, w.k, _units_of(out)) if m else (-1, 1)
+    if form < 0:
+        _check(_entry("ns_gemm_int8", "pppppiiiiiip")(out.data_ptr(), *operands, -form, code, _stream()), "linear_int8")
         return out
-    form, ranges = plan
     parts = None
     if ranges > 1:
         shape = (ranges * m * (-(-n // 4) * 4),)

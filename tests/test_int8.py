@@ -65,14 +65,15 @@ def test_products_that_are_refused(monkeypatch):
 
 def test_plan():
     """Few rows, or little to read, go by 16 rows; ranges of K are as long as a tile takes at least; a plan stands for every size."""
-    assert ops.int8_plan(1, 28672, 4096, 256) is None and ops.int8_plan(16, 28672, 4096, 256) is None and ops.int8_plan(32, 4096, 4096, 256) is None
-    assert ops.int8_plan(17, 28672, 4096, 256) is not None and ops.int8_plan(64, 4096, 4096, 256) is not None
+    few = lambda *sizes: ops.int8_plan(*sizes, 256)[0] < 0
+    assert few(1, 28672, 4096) and few(16, 28672, 4096) and few(32, 4096, 4096) and not few(48, 28672, 4096) and not few(2048, 4096, 4096)
     for m in (17, 100, 999, 4096, 70000):
         for n in (1, 1000, 4096, 128256):
             for k in (1, 513, 4096, 32768):
-                plan = ops.int8_plan(m, n, k, 256)
-                if plan is not None:
-                    form, ranges = plan
+                form, ranges = ops.int8_plan(m, n, k, 256)
+                if form < 0:
+                    assert -form in (1, 2, 4) and ranges == 1 and -(-m // (-16 * form)) <= 65535
+                else:
                     assert 0 <= form < len(ops.INT8_TILES) and ops.int8_padded_k(k) >= ranges * ops.INT8_K_MIN
                     tiles = -(-m // ops.INT8_TILES[form][0]) * -(-n // ops.INT8_TILES[form][1])
                     assert tiles * ranges <= 1 << 22
@@ -98,4 +99,4 @@ def test_plans_of_more_rows_than_are_joined():
     for m in (65535, 65536, 200_000):
         for n, k in ((17, 32768), (64, 8192), (4096, 4096)):
             plan = ops.int8_plan(m, n, k, 256)
-            assert plan is not None and (plan[1] == 1 or m <= ops.INT8_JOIN_ROWS)
+            assert plan[0] >= 0 and (plan[1] == 1 or m <= ops.INT8_JOIN_ROWS)

@@ -171,6 +171,27 @@ def test_product_in_every_tile(m, n, k, ranges, form):
     assert bool((out[m] == 7).all()) and bool((out[:, n:] == 7).all())
 
 
+@pytest.mark.parametrize("blocks", [1, 2, 4])
+@pytest.mark.parametrize("m,n,k", [(1, 4, 512), (17, 65, 768), (33, 30, 4096), (64, 16, 1300), (65, 100, 8192), (130, 260, 1280), (16, 17, 14336)])
+def test_product_in_every_row_block(m, n, k, blocks):
+    """The kernel for few rows with row blocks that the plan would not choose."""
+    import ctypes
+
+    from nanospec_amd.kernels import build
+
+    ops = _ops()
+    cx, xs, cw, ws = _operands(m, n, k, m + k)
+    w, x = ops.Int8Weight(cw.to(DEV), ws.to(DEV)), _rows(cx, xs)
+    out = torch.full((m + 1, n + 3), 7.0, device=DEV)
+    i = ctypes.c_int
+    status = build.core().ns_gemm_int8(ops._ptr(out), ops._ptr(x.data), ops._ptr(x.scales), ops._ptr(w.data), ops._ptr(w.scales), i(m), i(n), i(w.kp), i(n + 3), i(blocks), i(ops.F32),
+                                       ops._stream())
+    assert status == 0
+    want = (cx.double() @ cw.double().T) * xs.double()[:, None] * ws.double()
+    assert bool(((out[:m, :n].cpu().double() - want).abs() <= 4 * 2.0**-24 * 1.001 * want.abs()).all())
+    assert bool((out[m] == 7).all()) and bool((out[:, n:] == 7).all())
+
+
 def test_product_of_the_largest_sums():
     """32,768 products of 127 * 127: 528,515,072, of either sign."""
     ops = _ops()
