@@ -160,17 +160,23 @@ struct Int8Params {
   const float *xs, *ws;
   int M, N, KP, out_stride, ranges;
   int quads;  // rows of the result are whole pieces of four values, side by side in memory
+  int whole;  // ... of 16 bytes
 };
+static int int8_whole(const void* out, int N, int out_stride, int dtype) {
+  const int v = dtype == NS_DTYPE_F32 ? 4 : 8;
+  return N % v == 0 && out_stride % v == 0 && ((uintptr_t)out & 15) == 0;
+}
 static int int8_quads(const void* out, int N, int out_stride, int dtype) {
   return N % 4 == 0 && out_stride % 4 == 0 && ((uintptr_t)out & (dtype == NS_DTYPE_F32 ? 15 : 7)) == 0;
 }
 
+// the scales of four neighbours (there are as many as the weight has rows with its padding)
+__device__ __forceinline__ f32x4 int8_scales(const Int8Params& p, int col) { return *reinterpret_cast<const f32x4*>(p.ws + col); }
 // four neighbours of a row of the result; at once where rows lie so that they may be
 template <typename T>
-__device__ __forceinline__ void int8_store(const Int8Params& p, int row, int col, const i32x4 sum, float xs) {
+__device__ __forceinline__ void int8_store(const Int8Params& p, int row, int col, const i32x4 sum, float xs, const f32x4 ws) {
   typedef T vec_t __attribute__((ext_vector_type(4)));
   T* to = (T*)p.out + (size_t)row * p.out_stride + col;
-  const f32x4 ws = *reinterpret_cast<const f32x4*>(p.ws + col);  // (as many scales as the weight has rows with its padding)
   vec_t r;
 #pragma unroll
   for (int e = 0; e < 4; ++e) r[e] = from_f<T>((float)sum[e] * xs * ws[e]);
@@ -233,7 +239,7 @@ __global__ __launch_bounds__(WAVES * 64) void gemm_int8_few_kernel(const Int8Par
 #pragma unroll
   for (int v = 1; v < WAVES; ++v) sum += sums[v][wave][lane];
   const int row = m0 + 16 * wave + r, col = blockIdx.x * 16 + 4 * g;
-  if (row < p.M && col < p.N) int8_store<T>(p, row, col, sum, p.xs[row]);
+  if (row < p.M && col < p.N) int8_store<T>(p, row, col, sum, p.xs[row], int8_scales(p, col));
 }
 
 template <typename T>
@@ -255,7 +261,7 @@ extern "C" int ns_gemm_int8(void* out, const void* x, const float* xs, const voi
   if (M < 0 || N <= 0 || KP < 512 || KP % 256 || KP > INT8_MAX_K || out_stride < N || (blocks != 1 && blocks != 2 && blocks != 4)) return NS_ERR_BAD_ARG;
   if ((((uintptr_t)x | (uintptr_t)w | (uintptr_t)ws) & 15) || (M + 15) / 16 > 65535) return NS_ERR_UNSUPPORTED;
   if (M == 0) return NS_OK;
-  const Int8Params p{out, (const int8_t*)x, (const int8_t*)w, xs, ws, M, N, KP, out_stride, 1, int8_quads(out, N, out_stride, dtype)};
+  const Int8Params p{out, (const int8_t*)x, (const int8_t*)w, xs, ws, M, N, KP, out_stride, 1, int8_quads(out, N, out_stride, dtype), 0};
   if (dtype == NS_DTYPE_F32) return launch_int8_few<float>(p, blocks, stream);
   if (dtype == NS_DTYPE_BF16) return launch_int8_few<bf16_t>(p, blocks, stream);
   return NS_ERR_UNSUPPORTED;
@@ -388,20 +394,63 @@ __global__ __launch_bounds__(Q::WAVES * NS_WAVE) __attribute__((amdgpu_waves_per
   t.run(k1 - k0);
 
   const int r = t.lane % 16, g = t.lane / 16, np = (p.N + 3) & ~3;
+  if constexpr (RANGES) {
+#pragma unroll
+    for (int i = 0; i < Q::MI; ++i) {
+      const int row = m0 + 16 * (t.wm * Q::MI + i) + r;
+      if (row >= p.M) continue;
+#pragma unroll
+      for (int j = 0; j < Q::NJ; ++j) {
+        const int col = n0 + 16 * (t.wn * Q::NJ + j) + 4 * g;
+        if (col < p.N) *reinterpret_cast<i32x4*>(a.parts + ((size_t)range * p.M + row) * np + col) = t.acc[i][j];
+      }
+    }
+    return;
+  }
+  // all scales before the first result goes out: a load behind a store waits until that has been written (4 us a tile of 256 x 256)
+  float xs[Q::MI];
+  f32x4 ws[Q::NJ];
+#pragma unroll
+  for (int i = 0; i < Q::MI; ++i) xs[i] = p.xs[min(m0 + 16 * (t.wm * Q::MI + i) + r, p.M - 1)];
+#pragma unroll
+  for (int j = 0; j < Q::NJ; ++j) ws[j] = int8_scales(p, min(n0 + 16 * (t.wn * Q::NJ + j) + 4 * g, (p.N - 1) & ~3));
+  const int row0 = m0 + 16 * t.wm * Q::MI, col0 = n0 + 16 * t.wn * Q::NJ;  // of this wave's part
+  if (p.whole) {
+    // by way of LDS, which nobody reads any more, a fragment's 16 rows at a time: pieces of 16 bytes, a row's side by side (2,048 x 24,576 with K 1,024 59 us; of 8 bytes from the
+    // registers, four of a row side by side, 67)
+    constexpr int V = 16 / sizeof(T), COLS = Q::NJ * 16, LINE = COLS * (int)sizeof(T) + 16, LANES = COLS / V, ROWS = NS_WAVE / LANES, DEEP = 2;
+    static_assert(Q::WAVES * DEEP * 16 * LINE <= Q::BYTES && 16 % ROWS == 0, "a wave's lines");
+    typedef T four_t __attribute__((ext_vector_type(4)));
+    uint8_t* lines = int8_tiles + t.wave * (DEEP * 16 * LINE);
+#pragma unroll
+    for (int i = 0; i < Q::MI; ++i) {
+      uint8_t* at = lines + i % DEEP * (16 * LINE);
+#pragma unroll
+      for (int j = 0; j < Q::NJ; ++j) {
+        four_t v;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = from_f<T>((float)t.acc[i][j][e] * xs[i] * ws[j][e]);
+        *reinterpret_cast<four_t*>(at + r * LINE + (16 * j + 4 * g) * (int)sizeof(T)) = v;
+      }
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+#pragma unroll
+      for (int q = 0; q < 16 / ROWS; ++q) {
+        const int line = q * ROWS + t.lane / LANES, row = row0 + 16 * i + line, col = col0 + t.lane % LANES * V;
+        const i32x4 v = *reinterpret_cast<const i32x4*>(at + line * LINE + t.lane % LANES * 16);
+        if (row < p.M && col < p.N) *reinterpret_cast<i32x4*>((T*)p.out + (size_t)row * p.out_stride + col) = v;
+      }
+    }
+    return;
+  }
 #pragma unroll
   for (int i = 0; i < Q::MI; ++i) {
-    const int row = m0 + 16 * (t.wm * Q::MI + i) + r;
+    const int row = row0 + 16 * i + r;
     if (row >= p.M) continue;
-    const float xs = RANGES ? 0.f : p.xs[row];
 #pragma unroll
     for (int j = 0; j < Q::NJ; ++j) {
-      const int col = n0 + 16 * (t.wn * Q::NJ + j) + 4 * g;
-      if (col >= p.N) continue;
-      if constexpr (RANGES) {
-        *reinterpret_cast<i32x4*>(a.parts + ((size_t)range * p.M + row) * np + col) = t.acc[i][j];
-      } else {
-        int8_store<T>(p, row, col, t.acc[i][j], xs);
-      }
+      const int col = col0 + 16 * j + 4 * g;
+      if (col < p.N) int8_store<T>(p, row, col, t.acc[i][j], xs[i], ws[j]);
     }
   }
 }
@@ -415,7 +464,7 @@ __global__ __launch_bounds__(256) void gemm_int8_join_kernel(const Int8ManyParam
   if (col >= p.N) return;
   i32x4 sum = {0, 0, 0, 0};
   for (int s = 0; s < p.ranges; ++s) sum += *reinterpret_cast<const i32x4*>(a.parts + ((size_t)s * p.M + row) * np + col);
-  int8_store<T>(p, row, col, sum, p.xs[row]);
+  int8_store<T>(p, row, col, sum, p.xs[row], int8_scales(p, col));
 }
 
 template <class Q, typename T>
@@ -454,7 +503,7 @@ extern "C" int ns_gemm_int8_many(void* out, void* parts, const void* x, const fl
   if (M < 0 || N <= 0 || KP < 512 || KP % 256 || KP > INT8_MAX_K || out_stride < N || ranges < 1 || (ranges > 1 && !parts)) return NS_ERR_BAD_ARG;
   if (((uintptr_t)x | (uintptr_t)w | (uintptr_t)ws | (uintptr_t)parts) & 15) return NS_ERR_UNSUPPORTED;
   if (M == 0) return NS_OK;
-  const Int8ManyParams a{{out, (const int8_t*)x, (const int8_t*)w, xs, ws, M, N, KP, out_stride, ranges, int8_quads(out, N, out_stride, dtype)}, (int*)parts, 0, 0};
+  const Int8ManyParams a{{out, (const int8_t*)x, (const int8_t*)w, xs, ws, M, N, KP, out_stride, ranges, int8_quads(out, N, out_stride, dtype), int8_whole(out, N, out_stride, dtype)}, (int*)parts, 0, 0};
   if (dtype == NS_DTYPE_F32) return launch_int8_many<float>(a, form, stream);
   if (dtype == NS_DTYPE_BF16) return launch_int8_many<bf16_t>(a, form, stream);
   return NS_ERR_UNSUPPORTED;

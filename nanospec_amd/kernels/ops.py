@@ -1289,10 +1289,31 @@ INT8_WEIGHT_RATE = 5.2e6  # bytes a us of a weight that streams
 
 
 @functools.lru_cache(maxsize=1 << 14)
-def int8_plan(m: int, n: int, k: int, units: int) -> tuple[int, int]:
-    """(tile, ranges of K) of a product of m rows and n columns, or (-row blocks, 1) where the kernel for few rows is the faster one.
+def int8_plan(m: int, n: int, k: int, units: int) -> tuple[tuple[int, int, int], ...]:
+    """The pieces of a product of m rows and n columns: (columns, tile, ranges of K), or (columns, -row blocks, 1) where the kernel for few rows is the faster one.  It is one piece, or two where tiles for as many
+    columns as fill all units some times over leave a last round half empty, and smaller ones for the rest do not (2,048 rows of 28,672 x 4,096, 3 1/2 rounds of the largest tile: 263 us, in two pieces 227)."""
+    us, form, ranges = _int8_piece(m, n, k, units)
+    pieces = ((n, form, ranges),)
+    for form, (bm, bn) in enumerate(INT8_TILES):
+        down, across = -(-m // bm), -(-n // bn)
+        columns = down * across // units * units // down * bn  # of the rounds that are full
+        if 0 < columns < n:
+            rest, other, ranges = _int8_piece(m, n - columns, k, units)
+            if _int8_tiles_us(form, 1, m, columns, k, units) + rest < us:
+                us, pieces = _int8_tiles_us(form, 1, m, columns, k, units) + rest, ((columns, form, 1), (n - columns, other, ranges))
+    return pieces
 
-    Chosen by what they take, in us.  The kernel for few rows, with 1, 2 or 4 blocks of 16 rows a workgroup: 2.6, and for every round of as many workgroups as there are units what they read of both operands at
+
+def _int8_tiles_us(form: int, ranges: int, m: int, n: int, k: int, units: int) -> float:
+    (bm, bn), kp = INT8_TILES[form], int8_padded_k(k)
+    items = -(-m // bm) * -(-n // bn) * ranges
+    us = -(-items // units) * (INT8_TILE_US[form] * kp / (1024 * ranges) + INT8_TILE_ONCE_US[form])
+    us = 3.8 + max(us, n * kp / INT8_WEIGHT_RATE / min(1, 0.7 + 0.3 * items / units))
+    return us + 2.0 + ranges * m * n * 4 / 2.5e6 if ranges > 1 else us
+
+
+def _int8_piece(m: int, n: int, k: int, units: int) -> tuple[float, int, int]:
+    """-> (us, tile or -row blocks, ranges of K) of a product in one piece.  Chosen by what they take, in us.  The kernel for few rows, with 1, 2 or 4 blocks of 16 rows a workgroup: 2.6, and for every round of as many workgroups as there are units what they read of both operands at
     ``INT8_FEW_RATES``.  Tiles: 3.8, and for every round a tile's time; ranges of K 2.0 more, and their sums at 2.5 TB/s.  Neither is faster than the weight streams (a quarter slower from few tiles).
     Measured, it and the best tiles: 16 rows of 16,384 x 2,048 8.3 and 9.0; 32 of 4,096 x 4,096 6.5 and 10.0, 64 8.1 and 11.3, 96 12.4 and 11.3; 32 of 6,144 x 4,096 9.7 and 11.4, 64 13.4 and 12.8; 128 of
     2,048 x 2,048 5.2 and 7.5; 64 of 4,096 x 14,336 21.6 and 17.5.  Over 198 products in tiles (16 to 2,048 rows, 1,000 x 1,111 to 8,192 x 28,672) the choice among those takes 1.02 times as long as the best of all tiles
@@ -1308,16 +1329,14 @@ def int8_plan(m: int, n: int, k: int, units: int) -> tuple[int, int]:
             best = us, -blocks, 1
         if m <= 16 * blocks:
             break
-    for form, (bm, bn) in enumerate(INT8_TILES):
-        tiles = -(-m // bm) * -(-n // bn)
+    for form in range(len(INT8_TILES)):
         for ranges in (1, 2, 3, 4, 6, 8):
             if ranges > 1 and (kp < ranges * INT8_K_MIN or m > INT8_JOIN_ROWS):
                 break
-            us = 3.8 + max(-(-tiles * ranges // units) * (INT8_TILE_US[form] * kp / (1024 * ranges) + INT8_TILE_ONCE_US[form]), stream / min(1, 0.7 + 0.3 * tiles * ranges / units))
-            us += 2.0 + ranges * m * n * 4 / 2.5e6 if ranges > 1 else 0.0
+            us = _int8_tiles_us(form, ranges, m, n, k, units)
             if best is None or us < best[0]:
                 best = us, form, ranges
-    return best[1], best[2]
+    return best
 
 
 def linear_int8(x: Int8Rows, w: Int8Weight, out: torch.Tensor | None = None, dtype: torch.dtype = torch.bfloat16, take=None) -> torch.Tensor:
@@ -1336,16 +1355,18 @@ def linear_int8(x: Int8Rows, w: Int8Weight, out: torch.Tensor | None = None, dty
     if out.shape != (m, n) or (m and step != 1) or (m > 1 and stride < n):
         raise KernelRefused(f"linear_int8: out must be [{m}, {n}] with unit stride along a row")
     code = _dtype_code(out)
-    operands = (data.data_ptr(), scales.data_ptr(), w.data.data_ptr(), w.scales.data_ptr(), m, n, w.kp, max(stride, n))
-    form, ranges = int8_plan(m, n, w.k, _units_of(out)) if m else (-1, 1)
-    if form < 0:
-        _check(_entry("ns_gemm_int8", "pppppiiiiiip")(out.data_ptr(), *operands, -form, code, _stream()), "linear_int8")
-        return out
-    parts = None
-    if ranges > 1:
-        shape = (ranges * m * (-(-n // 4) * 4),)
-        parts = take(shape, torch.int32) if take is not None else torch.empty(shape, dtype=torch.int32, device=out.device)
-    _check(_entry("ns_gemm_int8_many", "ppppppiiiiiiip")(out.data_ptr(), _address(parts), *operands, form, ranges, code, _stream()), "linear_int8")
+    to, size, at = out.data_ptr(), out.element_size(), 0
+    for columns, form, ranges in int8_plan(m, n, w.k, _units_of(out)) if m else ():
+        operands = (data.data_ptr(), scales.data_ptr(), w.data.data_ptr() + at * w.kp, w.scales.data_ptr() + 4 * at, m, columns, w.kp, max(stride, n))
+        if form < 0:
+            _check(_entry("ns_gemm_int8", "pppppiiiiiip")(to + at * size, *operands, -form, code, _stream()), "linear_int8")
+        else:
+            parts = None
+            if ranges > 1:
+                shape = (ranges * m * (-(-columns // 4) * 4),)
+                parts = take(shape, torch.int32) if take is not None else torch.empty(shape, dtype=torch.int32, device=out.device)
+            _check(_entry("ns_gemm_int8_many", "ppppppiiiiiiip")(to + at * size, _address(parts), *operands, form, ranges, code, _stream()), "linear_int8")
+        at += columns
     return out
 
 

@@ -64,18 +64,22 @@ def test_products_that_are_refused(monkeypatch):
 
 
 def test_plan():
-    """Few rows, or little to read, go by 16 rows; ranges of K are as long as a tile takes at least; a plan stands for every size."""
-    few = lambda *sizes: ops.int8_plan(*sizes, 256)[0] < 0
+    """Few rows, or little to read, go by row blocks; ranges of K are as long as a tile takes at least; pieces are whole tiles' columns and make up the product; a plan stands for every size."""
+    few = lambda *sizes: ops.int8_plan(*sizes, 256)[0][1] < 0
     assert few(1, 28672, 4096) and few(16, 28672, 4096) and few(32, 4096, 4096) and not few(48, 28672, 4096) and not few(2048, 4096, 4096)
+    assert len(ops.int8_plan(2048, 28672, 4096, 256)) == 2
     for m in (17, 100, 999, 4096, 70000):
-        for n in (1, 1000, 4096, 128256):
+        for n in (1, 1000, 4096, 10007, 28672, 128256):
             for k in (1, 513, 4096, 32768):
-                form, ranges = ops.int8_plan(m, n, k, 256)
-                if form < 0:
-                    assert -form in (1, 2, 4) and ranges == 1 and -(-m // (-16 * form)) <= 65535
-                else:
-                    assert 0 <= form < len(ops.INT8_TILES) and ops.int8_padded_k(k) >= ranges * ops.INT8_K_MIN
-                    tiles = -(-m // ops.INT8_TILES[form][0]) * -(-n // ops.INT8_TILES[form][1])
+                pieces = ops.int8_plan(m, n, k, 256)
+                assert sum(c for c, _, _ in pieces) == n and len(pieces) <= 2
+                for i, (columns, form, ranges) in enumerate(pieces):
+                    if form < 0:
+                        assert -form in (1, 2, 4) and ranges == 1 and -(-m // (-16 * form)) <= 65535
+                        continue
+                    assert form < len(ops.INT8_TILES) and ops.int8_padded_k(k) >= ranges * ops.INT8_K_MIN
+                    assert i == len(pieces) - 1 or columns % ops.INT8_TILES[form][1] == 0
+                    tiles = -(-m // ops.INT8_TILES[form][0]) * -(-columns // ops.INT8_TILES[form][1])
                     assert tiles * ranges <= 1 << 22
 
 
@@ -99,4 +103,4 @@ def test_plans_of_more_rows_than_are_joined():
     for m in (65535, 65536, 200_000):
         for n, k in ((17, 32768), (64, 8192), (4096, 4096)):
             plan = ops.int8_plan(m, n, k, 256)
-            assert plan[0] >= 0 and (plan[1] == 1 or m <= ops.INT8_JOIN_ROWS)
+            assert all(ranges == 1 or m <= ops.INT8_JOIN_ROWS for _, _, ranges in plan)

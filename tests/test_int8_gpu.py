@@ -129,7 +129,7 @@ def _rows(cx, xs):
 
 
 PRODUCTS = [(1, 1, 1), (1, 2048, 2048), (16, 33, 512), (17, 20, 513), (3, 500, 14336), (33, 130, 4096), (64, 1000, 1100), (65, 4096, 768), (128, 257, 2304), (129, 100, 1024),
-            (255, 512, 512), (300, 1023, 3333), (520, 64, 8192), (1100, 2050, 640), (8, 7168, 4096), (61, 4096, 4096)]
+            (255, 512, 512), (300, 1023, 3333), (520, 64, 8192), (1100, 2050, 640), (8, 7168, 4096), (61, 4096, 4096), (1300, 13003, 600)]
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
