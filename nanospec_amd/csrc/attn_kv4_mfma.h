@@ -177,6 +177,60 @@ struct Kv4Wave {
     for (int i = 0; i < 2; ++i) m[i] = *reinterpret_cast<const u32x4*>(p.v + 8 * HD + 32 * of_values + 16 * i);
   }
 
+  // From the products of 8 keys with a column of tile c to its weights, in p.  ``v_mark``: steps for values as bits (what is below counts for nothing), ``most_of`` the largest.
+  __device__ __forceinline__ void soften(int c, const f32x4v* d, const float* k_step, const float* k_low, const float* v_step, const float* v_low, const uint32_t* v_mark, uint32_t most_of, int k0,
+                                         bool mask, f16x8* p) {
+    float s[8], top = -INFINITY;
+    uint32_t most = most_of;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) s[e] = fmaf(k_step[e], d[e / 4][e % 4], k_low[e] * qsum[c]);
+    if (mask) {
+      most = 0;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const int key = k0 + 8 * t + e;
+        const bool seen = key <= kpos[c] && key >= kfirst[c];
+        s[e] = seen ? s[e] : -INFINITY;
+        most = max(most, seen ? v_mark[e] : 0u);
+      }
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) top = fmaxf(top, s[e]);
+    // the exponent above the largest step, at least -64 (smaller ones lose what float16 does not hold of them)
+    const float reach = top * unscale[c] + fmaxf((float)(int)(most >> 23) - 126.f, -64.f);
+    if (__any(reach > R[c] + KV4_SLACK)) {
+      const float want = quarters_max(reach), next = want > R[c] + KV4_SLACK ? want : R[c], base = next == -INFINITY ? 0.f : next;
+      const float shrink = __builtin_amdgcn_exp2f(R[c] - base);
+      R[c] = next;
+      l[c] *= shrink;
+      z[c] *= shrink;
+#pragma unroll
+      for (int n = 0; n < NB; ++n)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) o[c][n][i] *= shrink;
+    }
+    const float base = R[c] == -INFINITY ? 0.f : R[c];
+    float w[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      w[e] = __builtin_amdgcn_exp2f(fmaf(s[e], unscale[c], -base));
+      l[c] += w[e];
+    }
+    if (mask) {  // (what a column does not see may be no number)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) z[c] += s[e] != -INFINITY ? w[e] * v_low[e] : 0.f;
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) z[c] = fmaf(w[e], v_low[e], z[c]);
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const float ps = w[e] * v_step[e];
+      p[0][e] = (_Float16)ps;
+      if constexpr (PARTS == 2) p[1][e] = (_Float16)(ps - (float)p[0][e]);
+    }
+  }
+
   // The 32 keys from k0 on.  ``mask``: some column may not see all of them.  What has been used of the block is loaded anew, from ``then``, at once: a load has most
   // of a block's time to arrive, and there is one set of registers for them.
   __device__ __forceinline__ void block(Kv4Block<HD>& b, int k0, bool mask, const At& then) {
@@ -199,9 +253,9 @@ struct Kv4Wave {
       const uint32_t km = b.km[e / 4][e % 4], vm = b.vm[e / 4][e % 4];
       k_step[e] = kv4_step(km);
       k_low[e] = kv4_low(km);
-      v_mark[e] = vm;
       v_step[e] = kv4_step(vm);
       v_low[e] = kv4_low(vm);
+      v_mark[e] = vm;
       most_of = max(most_of, vm);
     }
     load_marks(b.km, then, 0);
@@ -217,55 +271,7 @@ struct Kv4Wave {
 #pragma unroll
           for (int h = 0; h < PARTS; ++h) d[a] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ka[a][g], q[c][h][g], d[a], 0, 0, 0);
       }
-      float s[8], top = -INFINITY;
-      uint32_t most = most_of;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) s[e] = fmaf(k_step[e], d[e / 4][e % 4], k_low[e] * qsum[c]);
-      if (mask) {
-        most = 0;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const int key = k0 + 8 * t + e;
-          const bool seen = key <= kpos[c] && key >= kfirst[c];
-          s[e] = seen ? s[e] : -INFINITY;
-          most = max(most, seen ? v_mark[e] : 0u);
-        }
-      }
-#pragma unroll
-      for (int e = 0; e < 8; ++e) top = fmaxf(top, s[e]);
-      // the exponent above the largest step, at least -64 (smaller ones lose what float16 does not hold of them)
-      const float reach = top * unscale[c] + fmaxf((float)(int)(most >> 23) - 126.f, -64.f);
-      if (__any(reach > R[c] + KV4_SLACK)) {
-        const float want = quarters_max(reach), next = want > R[c] + KV4_SLACK ? want : R[c], base = next == -INFINITY ? 0.f : next;
-        const float shrink = __builtin_amdgcn_exp2f(R[c] - base);
-        R[c] = next;
-        l[c] *= shrink;
-        z[c] *= shrink;
-#pragma unroll
-        for (int n = 0; n < NB; ++n)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) o[c][n][i] *= shrink;
-      }
-      const float base = R[c] == -INFINITY ? 0.f : R[c];
-      float w[8];
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        w[e] = __builtin_amdgcn_exp2f(fmaf(s[e], unscale[c], -base));
-        l[c] += w[e];
-      }
-      if (mask) {  // (what a column does not see may be no number)
-#pragma unroll
-        for (int e = 0; e < 8; ++e) z[c] += s[e] != -INFINITY ? w[e] * v_low[e] : 0.f;
-      } else {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) z[c] = fmaf(w[e], v_low[e], z[c]);
-      }
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const float ps = w[e] * v_step[e];
-        p[c][0][e] = (_Float16)ps;
-        if constexpr (PARTS == 2) p[c][1][e] = (_Float16)(ps - (float)p[c][0][e]);
-      }
+      soften(c, d, k_step, k_low, v_step, v_low, v_mark, most_of, k0, mask, p[c]);
       __builtin_amdgcn_sched_barrier(0);
     }
     // values as operands, four channels of each 64 a lane
@@ -320,7 +326,7 @@ struct Kv4Wave {
 // Bound by memory where the rows are long and many (61 rows of 200 to 12,000 keys, 8 key/value heads of 128 channels: 94 us, 4.2 TB/s; 64 rows of 6,000: 5.3), by one workgroup's
 // chain of loads where they are few (a row of 1,000, in eight waves: 9.3 us).  Two blocks on their way at a time were slower everywhere (their registers cost a wave a SIMD).
 template <typename T, int HD, int PARTS, int WAVES>
-__global__ __launch_bounds__(WAVES * 64) __attribute__((amdgpu_waves_per_eu(2))) void attn_kv4_rows_kernel(const Kv4AttnParams a) {
+__global__ __launch_bounds__(WAVES * 64) __attribute__((amdgpu_waves_per_eu(3))) void attn_kv4_rows_kernel(const Kv4AttnParams a) {
   typedef Kv4Wave<T, HD, 1, PARTS> Wave;
   __shared__ float outs[WAVES][16][HD + 4];
   __shared__ float weights[WAVES][16];
@@ -394,10 +400,49 @@ __global__ __launch_bounds__(WAVES * 64) __attribute__((amdgpu_waves_per_eu(2)))
   }
 }
 
+// The results of a wave's columns, ``tokens`` tokens of a head from row ``row`` on, whole or as a range of theirs (``column``: its first token among all tiles').
+template <typename T, int HD, int CT, class Wave>
+__device__ __forceinline__ void kv4_columns_out(const Wave& w, const Kv4AttnParams& a, int row, int tokens, int column, int head, int split) {
+#pragma unroll
+  for (int c = 0; c < CT; ++c) {
+    float total, low;
+    const float weight = w.weight(c, total, low), inv = total == 0.f ? 0.f : 1.f / total;
+    const int token = 16 * c + w.col;
+    if (token >= tokens) continue;
+    if (a.splits == 1) {
+      T* to_ = (T*)a.out + ((size_t)(row + token) * a.heads + head) * HD;
+#pragma unroll
+      for (int nb = 0; nb < Wave::NB; ++nb) {
+        typedef T vec_t __attribute__((ext_vector_type(16 / sizeof(T))));
+        constexpr int V = 16 / sizeof(T);
+#pragma unroll
+        for (int e0 = 0; e0 < 16; e0 += V) {
+          vec_t r;
+#pragma unroll
+          for (int e = 0; e < V; ++e) r[e] = from_f<T>((w.sum_of(c, nb, e0 + e) + low) * inv);
+          *reinterpret_cast<vec_t*>(to_ + 64 * nb + 16 * w.t + e0) = r;
+        }
+      }
+    } else {
+      const size_t pc = (((size_t)column + token) * a.heads + head) * a.splits + split;
+#pragma unroll
+      for (int nb = 0; nb < Wave::NB; ++nb)
+#pragma unroll
+        for (int e0 = 0; e0 < 16; e0 += 4) {
+          f32x4v r;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) r[e] = (w.sum_of(c, nb, e0 + e) + low) * inv;
+          *reinterpret_cast<f32x4v*>(a.part_o + pc * HD + 64 * nb + 16 * w.t + e0) = r;
+        }
+      if (w.t == 0) a.part_l[pc] = weight;
+    }
+  }
+}
+
 // Portions: a wave 16 CT tokens of a head, four waves a workgroup that share nothing but their place.
-// Bound by vector instructions: a block of 32 keys and 32 columns of 128 channels has 32 matrix instructions (512 cycles) and about 290 others (1,350), of which 112 make operands of the
-// codes and 16 are exponentials.  2,048 tokens at 16,000 keys: 776 us, 736 TFLOP/s; 2,048 at none 69 us.  Four tiles of columns a wave (each operand made for twice as many) leave one wave a
-// SIMD and nothing to fill its waits: 1,203 and 149 us.
+// Bound by vector instructions: a block of 32 keys and 32 columns of 128 channels has 32 matrix instructions (512 cycles) and about 300 others (1,350), of which 112 make operands of the
+// codes and 16 are exponentials; they are under way 73% of the time.  2,048 tokens at 16,000 keys: 776 us, 736 TFLOP/s; 2,048 at none 69 us.  Four tiles of columns a wave (each operand made
+// for twice as many) leave one wave a SIMD and nothing to fill its waits: 1,203 and 149 us.  Operands made by four waves for each other, by way of LDS, with a barrier a block: 828 and 90.
 template <typename T, int HD, int CT, int PARTS>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void attn_kv4_tiles_kernel(const Kv4AttnParams a) {
   typedef Kv4Wave<T, HD, CT, PARTS> Wave;
@@ -425,38 +470,5 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void a
     w.query(c, (const T*)a.q + (size_t)(row0 + t0 + token) * a.q_stride + head * HD, a.scale_log2, a.wide);
   }
   w.walk(from, to, 1, (first_of_last + 31) / 32, (pos0 + 1) / 32, first / 8, last / 8, a.block_table + (size_t)req * a.table_stride, a.pool, a.kv_heads, kvh, shift);
-#pragma unroll
-  for (int c = 0; c < CT; ++c) {
-    float total, low;
-    const float weight = w.weight(c, total, low), inv = total == 0.f ? 0.f : 1.f / total;
-    const int token = 16 * c + w.col;
-    if (token >= tokens) continue;
-    if (a.splits == 1) {
-      T* to_ = (T*)a.out + ((size_t)(row0 + t0 + token) * a.heads + head) * HD;
-#pragma unroll
-      for (int nb = 0; nb < Wave::NB; ++nb) {
-        typedef T vec_t __attribute__((ext_vector_type(16 / sizeof(T))));
-        constexpr int V = 16 / sizeof(T);
-#pragma unroll
-        for (int e0 = 0; e0 < 16; e0 += V) {
-          vec_t r;
-#pragma unroll
-          for (int e = 0; e < V; ++e) r[e] = from_f<T>((w.sum_of(c, nb, e0 + e) + low) * inv);
-          *reinterpret_cast<vec_t*>(to_ + 64 * nb + 16 * w.t + e0) = r;
-        }
-      }
-    } else {
-      const size_t pc = (((size_t)tile * KV4_TILE_TOKENS + piece * TOKENS + token) * a.heads + head) * a.splits + split;
-#pragma unroll
-      for (int nb = 0; nb < Wave::NB; ++nb)
-#pragma unroll
-        for (int e0 = 0; e0 < 16; e0 += 4) {
-          f32x4v r;
-#pragma unroll
-          for (int e = 0; e < 4; ++e) r[e] = (w.sum_of(c, nb, e0 + e) + low) * inv;
-          *reinterpret_cast<f32x4v*>(a.part_o + pc * HD + 64 * nb + 16 * w.t + e0) = r;
-        }
-      if (w.t == 0) a.part_l[pc] = weight;
-    }
-  }
+  kv4_columns_out<T, HD, CT>(w, a, row0 + t0, tokens, (tile * KV4_TILE_TOKENS + piece * TOKENS), head, split);
 }
