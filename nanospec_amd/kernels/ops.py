@@ -1347,7 +1347,7 @@ def linear_int8(x: Int8Rows, w: Int8Weight, out: torch.Tensor | None = None, dty
     data, scales = x.data, x.scales
     _gpu(data, scales, w.data, out)
     m, n = scales.shape[0], w.n
-    if x.k != w.k or data.shape != (-(-m // 16), w.kp // 64, 4, 16, 16) or data.dtype != torch.int8 or not data.is_contiguous() or scales.dim() != 1 or scales.dtype != torch.float32:
+    if x.k != w.k or data.shape != (-(-m // 16), w.kp // 64, 4, 16, 16) or data.dtype != torch.int8 or not data.is_contiguous() or scales.dim() != 1 or scales.dtype != torch.float32 or not scales.is_contiguous():
         raise KernelRefused(f"linear_int8: rows of {x.k}, a weight of {w.k}")
     if out is None:
         out = torch.empty((m, n), dtype=dtype, device=data.device)

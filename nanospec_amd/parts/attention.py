@@ -30,9 +30,9 @@ F32_RANGE_KEYS = 128  # keys of a range of a single token's row in 32-bit: two t
 # Attention over keys and values in 4 bits (us, 32 heads on 8 of 128 channels unless said otherwise)
 KV4_MAX_RANGES = 64  # of a row's keys
 KV4_RANGE_KEYS = 256  # the fewest keys of a single token's: with fewer a workgroup's beginning and end are longer than its blocks
-# The fewest keys of a range of a portion's, and the most where there are ranges at all (their lengths differ with the tiles': 666 tokens at 20,000 keys 480 in 2 ranges, 396 in 4, 372 in 5,
-# 371 in 8).  Ranges cost what joining their results takes: 2,048 tokens 69 in one range, 103 in two; 100 tokens at 1,000 keys 28 and, in 8, 19.
-KV4_PORTION_KEYS = 128, 4096
+# The fewest keys of a range of a portion's, and the most where there are ranges at all (their lengths differ with the tiles': 666 tokens at 20,000 keys 440 in 2 ranges, 364 in 4, 347 in 6,
+# 339 in 8, 352 in 12; 512 at 8,000 158 in 2, 117 in 4, 128 in 6).  Ranges cost what joining their results takes: 2,048 tokens 69 in one range, 103 in two; 100 tokens at 1,000 keys 28 and, in 8, 19.
+KV4_PORTION_KEYS = 128, 2560
 # The keys up to which a wave takes 16 tokens of a portion (three or four waves a SIMD, which hide each other's waits and end evenly) instead of 32 (two, each key made an operand once for
 # both halves).  2,048 tokens 69 and 81, 100 at 1,000 keys 19 and 23; 512 at 8,000 133 and 118, 2,048 at 16,000 888 and 778.
 KV4_NARROW_KEYS = 4096
@@ -366,6 +366,8 @@ class Attention:
         s = self.spec
         plain = layouts == "both"
         int8 = products == "int8"
+        if int8 and s.general:
+            raise ValueError("an attention layer with options beyond a window has no products in 8-bit integers")
         q, k, v, o = self._names
         rows = s.heads * s.head_dim + (s.kv_heads * (s.head_dim + (0 if s.value_is_key else s.v_dim)) if s.own_kv else 0)
         self.gate_at = rows  # the output gate's logits, if the layer has a gate, are the last columns of the first product
@@ -402,8 +404,8 @@ class Attention:
         if s.general:
             # the general path: one product for what the layer projects, then norm / cache write and attention as kernels
             self.wqkv_rope = None
-            self.wqkv = Int8Linear(wqkv) if int8 else LinearWeight(wqkv, keep_plain=plain)
-            self.wo = Int8Linear(get(o).to(device=device, dtype=dtype)) if int8 else LinearWeight(get(o).to(device=device, dtype=dtype).contiguous(), keep_plain=plain)
+            self.wqkv = LinearWeight(wqkv, keep_plain=plain)
+            self.wo = LinearWeight(get(o).to(device=device, dtype=dtype).contiguous(), keep_plain=plain)
             return
         self.reads_int8 = int8
         if int8:

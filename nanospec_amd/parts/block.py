@@ -192,10 +192,10 @@ class StreamBlock:
         """How many buffers the block can leave unwritten outputs in (``forward``'s ``delta_out``)."""
         return 2 if self.parallel and self.ffn is not None and self.extra is None else 1
 
-    takes_layouts = takes_products = True
+    takes_layouts = True
 
-    def load(self, get, dtype, device, layouts: str = "both", products: str = "model") -> None:
-        load_parts(self.parts, get, dtype, device, layouts, products)
+    def load(self, get, dtype, device, layouts: str = "both") -> None:
+        load_parts(self.parts, get, dtype, device, layouts, "model")
         S, m = self.copies, float(self.spec.mult)
         self.dtype = dtype
         self._hc = []

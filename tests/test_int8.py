@@ -56,7 +56,7 @@ def test_products_that_are_refused(monkeypatch):
     rows = ops.Int8Rows.from_codes(torch.zeros((3, 600), dtype=torch.int8), torch.zeros(3))
     for call in (lambda: ops.linear_int8(torch.zeros(3, 600), w), lambda: ops.linear_int8(rows, torch.zeros(48, 600)), lambda: ops.linear_int8(rows, w, out=torch.zeros(3, 47)),
                  lambda: ops.linear_int8(rows, w, out=torch.zeros(48, 3).t()), lambda: ops.linear_int8(rows, w, dtype=torch.float16),
-                 lambda: ops.linear_int8(ops.Int8Rows(rows.data, rows.scales, 601), w), lambda: ops.linear_int8(ops.Int8Rows(rows.data, torch.zeros(17), 600), w),
+                 lambda: ops.linear_int8(ops.Int8Rows(rows.data, rows.scales, 601), w), lambda: ops.linear_int8(ops.Int8Rows(rows.data, torch.zeros(17), 600), w), lambda: ops.linear_int8(ops.Int8Rows(rows.data, torch.zeros(6)[::2], 600), w),
                  lambda: ops.linear_int8(ops.Int8Rows(rows.data[:, :8], rows.scales, 600), w), lambda: ops.linear_int8(ops.Int8Rows(rows.data.float(), rows.scales, 600), w),
                  lambda: ops.Int8Rows.from_codes(torch.zeros(3, 600), torch.zeros(3)), lambda: ops.Int8Rows.from_codes(torch.zeros((3, 600), dtype=torch.int8), torch.zeros(2))):
         with pytest.raises(ops.KernelRefused):
@@ -94,6 +94,11 @@ def test_models_refuse_products_that_are_not_built():
     net = DecoderModel(LlamaConfig.from_hf(TINY["A"]["cfg"]).model_spec())
     with pytest.raises(ValueError, match="products="):
         net.load(None, torch.float32, "cpu", products="int4")
+    from nanospec_amd.config import VuzelixConfig
+    from test_vuzelix_config import CFG
+
+    with pytest.raises(ValueError, match="not built for StreamBlock"):
+        DecoderModel(VuzelixConfig.from_hf(CFG).model_spec()).load(None, torch.float32, "cpu", products="int8")
     net.layers[1].ffn = SimpleNamespace()
     with pytest.raises(ValueError, match="not built for SimpleNamespace"):
         net.load(None, torch.float32, "cpu", products="int8")

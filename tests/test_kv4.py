@@ -99,6 +99,22 @@ def test_attention_refuses(monkeypatch, change):
         ops.attention_kv4_plain(**args)
 
 
+@pytest.mark.parametrize("change", [
+    dict(heads=3), dict(kv_heads=4), dict(head_dim=128), dict(pages=ops.Kv4Pages.empty(2, 2, 8, 96, "cpu"), head_dim=96, q=torch.zeros(3, 384), out=torch.zeros(3, 384)),
+    dict(pages=torch.zeros(2, 2, 1, 576, dtype=torch.uint8)), dict(q=torch.zeros(3, 200)), dict(out=torch.zeros(3, 200)), dict(out=torch.zeros(3, 256).bfloat16()), dict(q=torch.zeros(256)),
+    dict(tiles=torch.zeros((2, 8), dtype=torch.int64)), dict(tiles=torch.zeros((2, 6), dtype=torch.int32)), dict(tiles=torch.zeros(8, dtype=torch.int32)),
+    dict(block_table=torch.zeros((1, 2))), dict(window=-1), dict(splits=0), dict(splits=65), dict(splits=2), dict(groups=0), dict(form=5), dict(form=16), dict(rows=False, form=8),
+    dict(rows=False, form=32), dict(splits=2, workspace=(torch.zeros(2 * 4 * 2 * 64 - 1), torch.zeros(16))), dict(splits=2, rows=False, workspace=(torch.zeros(2 * 4 * 2 * 64), torch.zeros(16))),
+    dict(splits=2, workspace=(torch.zeros(1024).bfloat16(), torch.zeros(16)))])
+def test_attention_by_tiles_refuses(monkeypatch, change):
+    monkeypatch.setattr(ops, "_gpu", lambda *tensors: None)
+    args = dict(q=torch.zeros(3, 256), out=torch.zeros(3, 256), pages=ops.Kv4Pages.empty(2, 2, 8, 64, "cpu"), tiles=torch.zeros((2, 8), dtype=torch.int32),
+                block_table=torch.zeros((1, 2), dtype=torch.int32), heads=4, kv_heads=2, head_dim=64, scale=1.0, rows=True)
+    args.update(change)
+    with pytest.raises(ops.KernelRefused):
+        ops.attention_kv4(**args)
+
+
 def test_tensors_on_the_cpu_are_refused():
     with pytest.raises(ops.KernelRefused, match="GPU"):
         ops.kv4_read(ops.Kv4Pages.empty(1, 1, 8, 32, "cpu"), torch.zeros(1, dtype=torch.int32), torch.zeros(1, dtype=torch.int32), torch.zeros((1, 1), dtype=torch.int32))

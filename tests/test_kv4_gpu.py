@@ -165,8 +165,8 @@ def _pool(pages, kv_heads, page, hd, seed, spread=1.0, held=None):
 
 def tolerance(dtype, out, size, hd, keys, v_step, v_most):
     """How far attention may be off, for |out| and the sizes at hand (``size``: the largest sum of |q| |k| scale of a visible pair).
-    A score is at most 2 hd + 4 roundings of 2^-24 of ``size`` off (plain products and sums in 32 bits); where codes are multiplied with 1,024 on top of them, which is taken off in the
-    first sum, so are 1,024 |q| of the step in the place of at most 15: at most 70 times as much, in hd / 8 + 2 roundings.  float32 takes the codes as they are.
+    A score is at most 2 hd + 4 roundings of 2^-24 of ``size`` off (products and sums in 32 bits).  On the matrix cores queries are float16, one value for bfloat16, two for float32, scaled so that the
+    largest channel lies at 256 (or 16, where codes count sixteen times): a bfloat16 channel is exact but for what is below 2^-29 of the largest.  For bfloat16 70 roundings for every 8 channels are allowed.
     The soft-max's weights are off by exp(2 delta) - 1 and the roundings of 2^x (2 units); bfloat16 rounds them to float16 on their way into the second product: 2^-11, and 2^-25 of the
     largest for those below the normal range, times keys; sums over the keys add 2^-24 each, of all that is summed (values and codes times steps: at most v_most + 8 steps)."""
     exact = dtype == torch.float32
@@ -231,3 +231,119 @@ def test_attention(case, heads, kv_heads, hd, page, dtype):
 def test_attention_window(heads, kv_heads, hd, page, window, dtype):
     got, want, tol, _ = _attend("mixed", heads, kv_heads, hd, page, dtype, window=window, seed=window)
     assert bool(((got - want).abs() <= tol).all())
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("heads,kv_heads,hd,page", [(8, 2, 64, 16), (6, 1, 128, 16), (32, 8, 64, 8)])
+def test_attention_where_the_kernel_takes_another_form(heads, kv_heads, hd, page, dtype):
+    """Portions over more keys than go by 16 tokens a wave, in ranges; rows that are whole, more than there are compute units; rows of very different lengths, cut by them; values of very
+    different steps."""
+    rows = [(37 * i) % 700 for i in range(70)]
+    for case, spread in ((([40, 33], [5000, 4097]), 1.0), (([1] * 70, rows), 1.0), (([1] * 5, [6000, 3, 900, 0, 2500]), 1.0), (([1, 50, 1], [2000, 100, 31]), 2.0)):
+        if len(case[0]) == 2 and heads == 32:
+            continue  # (the oracle's time)
+        got, want, tol, _ = _attend(case, heads, kv_heads, hd, page, dtype, seed=len(rows) + hd, spread=spread)
+        assert bool(((got - want).abs() <= tol).all()), (case, float(((got - want).abs() / tol).max()))
+
+
+def _layer(hd, heads=4, kv_heads=2):
+    return dict(heads=heads, kv_heads=kv_heads, hd=hd, inv=(1.0 / 10000.0 ** (torch.arange(0, hd, 2, dtype=torch.float32) / hd)).to(DEV))
+
+
+def _step(layer, qkv, lens, starts, tables, pool, dtype):
+    """Write and attention of a step, as a layer calls them.  -> [tokens, heads * hd]"""
+    from nanospec_amd.parts.attention import kv4_attention
+
+    ops, heads, kv_heads, hd = _ops(), layer["heads"], layer["kv_heads"], layer["hd"]
+    ctx = oracle.batch_context(lens, starts, tables, DEV)
+    dev = qkv.to(device=DEV, dtype=dtype, copy=True)
+    ops.rope_kv4_write(dev, ctx.positions, ctx.token_req, ctx.block_tables[0], layer["inv"], pool, heads, kv_heads, hd, hd)
+    out = torch.empty((dev.shape[0], heads * hd), dtype=dtype, device=DEV)
+    return kv4_attention(ctx, dev, out, pool, ctx.block_tables[0], heads, kv_heads, hd, hd**-0.5)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("hd", [64, 96, 128])
+@pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
+def test_a_bad_key_or_value_is_seen_by_those_who_see_it(hd, bad, dtype):
+    """A token whose key or value holds no number, or an infinity: whoever comes later in its request has no number in that head's group, everybody else the same bits as without it."""
+    ops, layer = _ops(), _layer(hd)
+    heads, kv_heads = layer["heads"], layer["kv_heads"]
+    lens, starts = [70, 70], [0, 0]
+    tables, pages = oracle.scattered_tables([6, 6], 1, 3)
+    qkv = _rand((140, (heads + 2 * kv_heads) * hd), hd)
+    run = lambda x: _step(layer, x, lens, starts, tables, ops.Kv4Pages.empty(pages, kv_heads, 16, hd, DEV), dtype).view(140, heads, hd).clone()
+    clean = run(qkv)
+    for column, group in ((heads * hd + 5, 0), ((heads + kv_heads) * hd + hd + 7, 1)):  # a key of head 0, a value of head 1
+        worse = qkv.clone()
+        worse[40, column] = bad
+        got = run(worse)
+        hit = torch.zeros(140, heads, dtype=torch.bool, device=DEV)
+        hit[40:70, group * 2 : group * 2 + 2] = True
+        assert bool(torch.isnan(got[hit]).all()) and torch.equal(got[~hit], clean[~hit])
+        # single tokens behind it
+        for pos, nan in ((40, True), (39, False)):
+            pool = ops.Kv4Pages.empty(pages, kv_heads, 16, hd, DEV)
+            _step(layer, worse[: pos + 1], [pos + 1], [0], tables[:1], pool, dtype)
+            one = _step(layer, worse[pos : pos + 1], [1], [pos], tables[:1], pool, dtype).view(heads, hd)
+            assert bool(torch.isnan(one[group * 2 : group * 2 + 2]).all()) == nan and bool(torch.isfinite(one[2 - group * 2 : 4 - group * 2]).all())
+
+
+@pytest.mark.parametrize("hd", [96, 128])
+def test_pages_beyond_4_gib(hd):
+    """The same step in pages at a small pool's beginning and at the end of a pool of more than 2^32 bytes: the same bits."""
+    ops, layer = _ops(), _layer(hd, heads=8, kv_heads=8)
+    lens, starts = [40, 1, 1], [0, 0, 100]
+    per_page = 8 * 2 * (8 * hd + 64)
+    pages = 2**32 // per_page + 50
+    small, _ = oracle.scattered_tables([3, 1, 7], 0, 1)
+    far = torch.where(small >= 0, pages - 1 - small, small)
+    results = []
+    for tables, n in ((small, 11), (far, pages)):
+        pool = ops.Kv4Pages.empty(n, 8, 16, hd, DEV)
+        _step(layer, _rand((100, 24 * hd), 4), [100], [0], tables[2:], pool, torch.bfloat16)  # what the last request has
+        out = _step(layer, _rand((42, 24 * hd), 5), lens, starts, tables, pool, torch.bfloat16)
+        where = (torch.arange(101, dtype=torch.int32, device=DEV), torch.full((101,), 2, dtype=torch.int32, device=DEV), tables.to(DEV))
+        results.append((out, *ops.kv4_read(pool, *where)))
+        assert bool(pool.pool[int(tables.max())].any())
+        del pool
+    assert all(torch.equal(a, b) for a, b in zip(*results)) and bool(results[0][1].any())
+
+
+def test_on_another_stream():
+    ops, layer = _ops(), _layer(64)
+    lens, starts = [50, 1], [0, 300]
+    tables, pages = oracle.scattered_tables([4, 19], 1, 2)
+    qkv, x = _rand((51, 8 * 64), 1), _rand((300, 8 * 64), 2)
+    results = []
+    for stream in (torch.cuda.current_stream(), torch.cuda.Stream()):
+        stream.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(stream):
+            pool = ops.Kv4Pages.empty(pages, 2, 16, 64, DEV)
+            _step(layer, x, [300], [0], tables[1:], pool, torch.bfloat16)
+            out = _step(layer, qkv, lens, starts, tables, pool, torch.bfloat16)
+            rows = ops.int8_rows(out)
+            results.append((out, ops.linear_int8(rows, ops.Int8Weight.from_float(_rand((300, 256), 3).to(DEV)))))
+        stream.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(*results))
+
+
+@pytest.mark.parametrize("rows,splits", [(False, 1), (False, 3), (True, 1), (True, 4)])
+def test_tokens_that_no_tile_describes_are_left_alone(rows, splits):
+    """A step of a fixed shape: tiles without tokens among others, rows behind the last."""
+    ops = _ops()
+    pool, keys, values, _ = _pool(8, 2, 16, 64, 1)
+    table = torch.arange(8, dtype=torch.int32, device=DEV).view(1, 8)
+    q = _rand((60, 256), 2).bfloat16().to(DEV)
+    n = 1 if rows else 40
+    live = [[0, 0, 5, 1, 90, 0, 3, 0]] if rows else [[0, 0, 5, 40, 90, 0, 0, 0], [0, 32, 5, 40, 90, 0, 0, -1]]
+    none = [[0, 0, 0, 0, 0, 0, 3, -1]]
+    tiles = torch.tensor(none + live + none * 3, dtype=torch.int32, device=DEV)
+    columns = tiles.shape[0] * (1 if rows else 32) * 4
+    work = tuple(torch.full((columns * splits * w,), math.nan, device=DEV) for w in (64, 1)) if splits > 1 else None
+    out = torch.full((60, 256), 7.0, dtype=torch.bfloat16, device=DEV)
+    ops.attention_kv4(q, out, pool, tiles, table, 4, 2, 64, 0.125, rows, splits=splits, workspace=work, groups=512)
+    assert bool((out[:5] == 7).all()) and bool((out[5 + n :] == 7).all())
+    want, _ = oracle.attention(q[5 : 5 + n].cpu().double().view(n, 4, 64), keys, values, [n], [90 - n], table.cpu(), 16, 4, 2, 0.125)
+    # (weights in float16, 2^-11 of values of up to 20, and the result's rounding)
+    assert float((out[5 : 5 + n].cpu().double().view(n, 4, 64) - want).abs().max()) <= 20 * (2.0**-11 + 2.0**-8)
