@@ -15,8 +15,9 @@
 // Queries are float16 on their way in, scaled by a power of two of their own so that the largest lies at 256: what is 2^-22 of it is exact.  Weights are
 // rounded to float16 (2^-12 of themselves).  PARTS 2: queries and weights as the sum of two float16 values each, two products for one.
 //
-// The soft-max's reference R is one number a column for weights and steps together: R >= (largest score so far) + (exponent of the steps seen) - 8, so
-// that p step, p = 2^(s - R), fits float16 whatever the steps' size, and is only raised when that no longer holds (then every sum shrinks).
+// The soft-max's reference R is one number a column for weights and steps together: R >= (score + log2 of its value's step) - 8 of every key so far, so
+// that p step, p = 2^(s - R), fits float16 whatever the steps' size, and is only raised when that no longer holds (then every sum shrinks).  (Key by key: by the largest score and the largest step
+// apart, a value of great size whose key has next to no weight would cost the others their bits; that costs a portion 5%.)
 // It knows of the keys that the column sees, and of no others.
 #pragma once
 
@@ -35,6 +36,8 @@ __device__ __forceinline__ f16x8 as_f16x8(uint32_t a, uint32_t b, uint32_t c, ui
 // two codes of a dword as 2^-24 u, and as 2^-20 u
 __device__ __forceinline__ uint32_t kv4_ones(uint32_t w) { return w & 0x000f000fu; }
 __device__ __forceinline__ uint32_t kv4_sixteens(uint32_t w) { return w & 0x00f000f0u; }
+// log2 of a mark's step + 127, up to 0.09 below it; at least 63 (of smaller steps is lost what float16 does not hold)
+__device__ __forceinline__ float kv4_log(uint32_t mark) { return (float)max(mark, 63u << 23) * 0x1p-23f; }
 __device__ __forceinline__ float quarters_max(float v) {
   v = fmaxf(v, __shfl_xor(v, 16, NS_WAVE));
   return fmaxf(v, __shfl_xor(v, 32, NS_WAVE));
@@ -177,27 +180,22 @@ struct Kv4Wave {
     for (int i = 0; i < 2; ++i) m[i] = *reinterpret_cast<const u32x4*>(p.v + 8 * HD + 32 * of_values + 16 * i);
   }
 
-  // From the products of 8 keys with a column of tile c to its weights, in p.  ``v_mark``: steps for values as bits (what is below counts for nothing), ``most_of`` the largest.
-  __device__ __forceinline__ void soften(int c, const f32x4v* d, const float* k_step, const float* k_low, const float* v_step, const float* v_low, const uint32_t* v_mark, uint32_t most_of, int k0,
-                                         bool mask, f16x8* p) {
-    float s[8], top = -INFINITY;
-    uint32_t most = most_of;
+  // From the products of 8 keys with a column of tile c to its weights, in p.  ``v_log``: about log2 of the keys' steps for values, + 127.
+  __device__ __forceinline__ void soften(int c, const f32x4v* d, const float* k_step, const float* k_low, const float* v_step, const float* v_low, const float* v_log, int k0, bool mask,
+                                         f16x8* p) {
+    float s[8], reach = -INFINITY;
 #pragma unroll
     for (int e = 0; e < 8; ++e) s[e] = fmaf(k_step[e], d[e / 4][e % 4], k_low[e] * qsum[c]);
     if (mask) {
-      most = 0;
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         const int key = k0 + 8 * t + e;
-        const bool seen = key <= kpos[c] && key >= kfirst[c];
-        s[e] = seen ? s[e] : -INFINITY;
-        most = max(most, seen ? v_mark[e] : 0u);
+        s[e] = key <= kpos[c] && key >= kfirst[c] ? s[e] : -INFINITY;
       }
     }
 #pragma unroll
-    for (int e = 0; e < 8; ++e) top = fmaxf(top, s[e]);
-    // the exponent above the largest step, at least -64 (smaller ones lose what float16 does not hold of them)
-    const float reach = top * unscale[c] + fmaxf((float)(int)(most >> 23) - 126.f, -64.f);
+    for (int e = 0; e < 8; ++e) reach = fmaxf(reach, fmaf(s[e], unscale[c], v_log[e]));
+    reach -= 127.f;
     if (__any(reach > R[c] + KV4_SLACK)) {
       const float want = quarters_max(reach), next = want > R[c] + KV4_SLACK ? want : R[c], base = next == -INFINITY ? 0.f : next;
       const float shrink = __builtin_amdgcn_exp2f(R[c] - base);
@@ -247,7 +245,7 @@ struct Kv4Wave {
     __builtin_amdgcn_sched_barrier(0);
     f16x8 p[CT][PARTS];
     float k_step[8], k_low[8], v_step[8], v_low[8];
-    uint32_t v_mark[8], most_of = 0;
+    float v_log[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
       const uint32_t km = b.km[e / 4][e % 4], vm = b.vm[e / 4][e % 4];
@@ -255,8 +253,7 @@ struct Kv4Wave {
       k_low[e] = kv4_low(km);
       v_step[e] = kv4_step(vm);
       v_low[e] = kv4_low(vm);
-      v_mark[e] = vm;
-      most_of = max(most_of, vm);
+      v_log[e] = kv4_log(vm);
     }
     load_marks(b.km, then, 0);
     load_marks(b.vm, then, 1);
@@ -271,7 +268,7 @@ struct Kv4Wave {
 #pragma unroll
           for (int h = 0; h < PARTS; ++h) d[a] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ka[a][g], q[c][h][g], d[a], 0, 0, 0);
       }
-      soften(c, d, k_step, k_low, v_step, v_low, v_mark, most_of, k0, mask, p[c]);
+      soften(c, d, k_step, k_low, v_step, v_low, v_log, k0, mask, p[c]);
       __builtin_amdgcn_sched_barrier(0);
     }
     // values as operands, four channels of each 64 a lane
@@ -440,9 +437,9 @@ __device__ __forceinline__ void kv4_columns_out(const Wave& w, const Kv4AttnPara
 }
 
 // Portions: a wave 16 CT tokens of a head, four waves a workgroup that share nothing but their place.
-// Bound by vector instructions: a block of 32 keys and 32 columns of 128 channels has 32 matrix instructions (512 cycles) and about 300 others (1,350), of which 112 make operands of the
-// codes and 16 are exponentials; they are under way 73% of the time.  2,048 tokens at 16,000 keys: 776 us, 736 TFLOP/s; 2,048 at none 69 us.  Four tiles of columns a wave (each operand made
-// for twice as many) leave one wave a SIMD and nothing to fill its waits: 1,203 and 149 us.  Operands made by four waves for each other, by way of LDS, with a barrier a block: 828 and 90.
+// Bound by vector instructions: a block of 32 keys and 32 columns of 128 channels has 32 matrix instructions (512 cycles) and about 320 others (1,430), of which 112 make operands of the
+// codes and 16 are exponentials; they are under way 73% of the time.  2,048 tokens at 16,000 keys: 809 us, 706 TFLOP/s; 2,048 at none 73 us.  Four tiles of columns a wave (each operand made
+// for twice as many) leave one wave a SIMD and nothing to fill its waits: 1,203 and 149 us.  Operands made by four waves for each other, by way of LDS, with a barrier a block: 828 and 90, where these took 772 and 75.
 template <typename T, int HD, int CT, int PARTS>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void attn_kv4_tiles_kernel(const Kv4AttnParams a) {
   typedef Kv4Wave<T, HD, CT, PARTS> Wave;

@@ -1497,7 +1497,7 @@ def kv4_read(pages: Kv4Pages, positions: torch.Tensor, token_req: torch.Tensor, 
     return k, v
 
 
-def _check_kv4_attn(q, out, pages: Kv4Pages, heads: int, kv_heads: int, head_dim: int, window: int, splits: int, workspace, cols: int, what: str):
+def _check_kv4_attn(q, out, pages: Kv4Pages, heads: int, kv_heads: int, head_dim: int, scale: float, window: int, splits: int, workspace, cols: int, what: str):
     _gpu(q, out)
     if heads < 1 or kv_heads < 1 or heads % kv_heads:
         raise KernelRefused(f"{what}: {heads} heads are not a multiple of {kv_heads} key/value heads")
@@ -1508,8 +1508,8 @@ def _check_kv4_attn(q, out, pages: Kv4Pages, heads: int, kv_heads: int, head_dim
         raise KernelRefused(f"{what}: q must be [tokens, at least {heads * head_dim}]")
     if out.shape != (n, heads * head_dim) or out.dtype != q.dtype or not out.is_contiguous():
         raise KernelRefused(f"{what}: out must be contiguous [{n}, {heads * head_dim}] of q's dtype")
-    if window < 0 or not 1 <= splits <= 64:
-        raise KernelRefused(f"{what}: a window is not negative, ranges of keys are 1 to 64")
+    if window < 0 or not 1 <= splits <= 64 or not 0 < scale < math.inf:
+        raise KernelRefused(f"{what}: a window is not negative, ranges of keys are 1 to 64, the scale is positive")
     if splits == 1:
         return None, None
     if workspace is None:
@@ -1547,7 +1547,7 @@ def attention_kv4(q, out, pages: Kv4Pages, tiles, block_table, heads: int, kv_he
     if form not in ((4, 8) if rows else (16,) if q.dtype == torch.float32 else (16, 32)):
         raise KernelRefused("attention_kv4: a workgroup has 4 or 8 waves for single tokens; a wave takes 16 tokens of a portion, of bfloat16 also 32")
     n_tiles = tiles.shape[0]
-    po, pl = _check_kv4_attn(q, out, pages, heads, kv_heads, head_dim, window, splits, workspace, n_tiles * (1 if rows else 32) * heads, "attention_kv4")
+    po, pl = _check_kv4_attn(q, out, pages, heads, kv_heads, head_dim, scale, window, splits, workspace, n_tiles * (1 if rows else 32) * heads, "attention_kv4")
     _check(_entry("ns_attn_kv4", "ppppipppiiiiiiiiiiifip")(out.data_ptr(), _address(po), _address(pl), q.data_ptr(), q.stride(0), pages.pool.data_ptr(), tiles.data_ptr(),
                                                            block_table.data_ptr(), block_table.stride(0), n_tiles, heads, kv_heads, head_dim, pages.page, 1 if rows else 0, form,
                                                            splits, groups, window, scale, _dtype_code(q), _stream()), "attention_kv4")
@@ -1562,7 +1562,7 @@ def attention_kv4_plain(q, out, pages: Kv4Pages, token_req, positions, block_tab
     n = _check_kv4(pages, positions, token_req, block_table, kv_heads, head_dim, "attention_kv4_plain")
     if n != q.shape[0]:
         raise KernelRefused("attention_kv4_plain: positions and token_req are per row of q")
-    po, pl = _check_kv4_attn(q, out, pages, heads, kv_heads, head_dim, window, splits, workspace, n * heads, "attention_kv4_plain")
+    po, pl = _check_kv4_attn(q, out, pages, heads, kv_heads, head_dim, scale, window, splits, workspace, n * heads, "attention_kv4_plain")
     _check(build.core().ns_attn_kv4_plain(_ptr(out), _ptr(po), _ptr(pl), _ptr(q), c_int(q.stride(0)), _ptr(pages.pool), _ptr(token_req), _ptr(positions), _ptr(block_table),
                                           c_int(block_table.stride(0)), c_int(n), c_int(heads), c_int(kv_heads), c_int(head_dim), c_int(pages.page), c_int(splits), c_int(window),
                                           c_float(scale), c_int(_dtype_code(q)), _stream()), "attention_kv4_plain")

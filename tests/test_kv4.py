@@ -86,7 +86,7 @@ def test_write_refuses(monkeypatch, change):
 
 @pytest.mark.parametrize("change", [
     dict(heads=3), dict(kv_heads=4), dict(head_dim=64), dict(q=torch.zeros(3, 100)), dict(q=torch.zeros(128, 3).t()), dict(out=torch.zeros(3, 64)),
-    dict(out=torch.zeros(3, 128).bfloat16()), dict(out=torch.zeros(3, 200)[:, :128]), dict(window=-1), dict(splits=0), dict(splits=65), dict(splits=2),
+    dict(out=torch.zeros(3, 128).bfloat16()), dict(out=torch.zeros(3, 200)[:, :128]), dict(window=-1), dict(splits=0), dict(splits=65), dict(splits=2), dict(scale=0.0), dict(scale=float("inf")),
     dict(splits=2, workspace=(torch.zeros(8), torch.zeros(24))), dict(splits=2, workspace=(torch.zeros(768), torch.zeros(23))), dict(token_req=torch.zeros(4, dtype=torch.int32)),
     dict(positions=torch.zeros(2, dtype=torch.int32), token_req=torch.zeros(2, dtype=torch.int32)),
     dict(q=torch.zeros(3, 128, dtype=torch.float16), out=torch.zeros(3, 128, dtype=torch.float16))])
@@ -103,7 +103,7 @@ def test_attention_refuses(monkeypatch, change):
     dict(heads=3), dict(kv_heads=4), dict(head_dim=128), dict(pages=ops.Kv4Pages.empty(2, 2, 8, 96, "cpu"), head_dim=96, q=torch.zeros(3, 384), out=torch.zeros(3, 384)),
     dict(pages=torch.zeros(2, 2, 1, 576, dtype=torch.uint8)), dict(q=torch.zeros(3, 200)), dict(out=torch.zeros(3, 200)), dict(out=torch.zeros(3, 256).bfloat16()), dict(q=torch.zeros(256)),
     dict(tiles=torch.zeros((2, 8), dtype=torch.int64)), dict(tiles=torch.zeros((2, 6), dtype=torch.int32)), dict(tiles=torch.zeros(8, dtype=torch.int32)),
-    dict(block_table=torch.zeros((1, 2))), dict(window=-1), dict(splits=0), dict(splits=65), dict(splits=2), dict(groups=0), dict(form=5), dict(form=16), dict(rows=False, form=8),
+    dict(block_table=torch.zeros((1, 2))), dict(window=-1), dict(splits=0), dict(splits=65), dict(splits=2), dict(groups=0), dict(scale=0.0), dict(scale=-1.0), dict(scale=float("nan")), dict(form=5), dict(form=16), dict(rows=False, form=8),
     dict(rows=False, form=32), dict(splits=2, workspace=(torch.zeros(2 * 4 * 2 * 64 - 1), torch.zeros(16))), dict(splits=2, rows=False, workspace=(torch.zeros(2 * 4 * 2 * 64), torch.zeros(16))),
     dict(splits=2, workspace=(torch.zeros(1024).bfloat16(), torch.zeros(16)))])
 def test_attention_by_tiles_refuses(monkeypatch, change):

@@ -347,3 +347,35 @@ def test_tokens_that_no_tile_describes_are_left_alone(rows, splits):
     want, _ = oracle.attention(q[5 : 5 + n].cpu().double().view(n, 4, 64), keys, values, [n], [90 - n], table.cpu(), 16, 4, 2, 0.125)
     # (weights in float16, 2^-11 of values of up to 20, and the result's rounding)
     assert float((out[5 : 5 + n].cpu().double().view(n, 4, 64) - want).abs().max()) <= 20 * (2.0**-11 + 2.0**-8)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("lens,starts", [([1], [90]), ([20], [71]), ([1], [3000])])
+def test_values_of_a_key_without_weight_cost_the_others_nothing(lens, starts, dtype):
+    """One key's values, and their step, are 2^40 times the others', and its score is so far below them that its weight is 2^-60 or less: the result is that of the others alone, to their own
+    tolerance."""
+    from nanospec_amd.parts.attention import kv4_attention
+
+    ops, hd, page = _ops(), 64, 16
+    held = lens[0] + starts[0]
+    tables, pages = oracle.scattered_tables([-(-held // page)], 1, 1)
+    gen = torch.Generator().manual_seed(5)
+    k = 0.1 * torch.randn((pages, 1, page, hd), generator=gen, dtype=torch.float64)
+    v = torch.randn((pages, 1, page, hd), generator=gen, dtype=torch.float64)
+    at = (int(tables[0, 40 // page]), 0, 40 % page)
+    k[at], v[at] = -8.0, v[at] * 2.0**40
+    made, sides = [], []
+    for x in (k, v):
+        c, s, low = oracle.quantised(x)
+        sides.append(s * c + low)
+        made += [c.to(torch.uint8).to(DEV), s[..., 0].bfloat16().to(DEV), low[..., 0].bfloat16().to(DEV)]
+    pool = ops.Kv4Pages.from_codes(*made)
+    q = (1 + 0.1 * _rand((lens[0], 4 * hd), 3)).to(dtype)  # the key's score is about -8 * 64 / 8 = -64, or 92 octaves
+    ctx = oracle.batch_context(lens, starts, tables, DEV)
+    out = torch.empty((lens[0], 4 * hd), dtype=dtype, device=DEV)
+    kv4_attention(ctx, q.to(DEV), out, pool, ctx.block_tables[0], 4, 1, hd, hd**-0.5)
+    want, size = oracle.attention(q.double().view(-1, 4, hd), *sides, lens, starts, tables, page, 4, 1, hd**-0.5)
+    alone = sides[1].clone()
+    alone[at] = 0
+    tol = tolerance(dtype, want, size, hd, held, float(alone.abs().max()) / 4, float(alone.abs().max())) + 2.0**-40
+    assert bool(((out.cpu().double().view(-1, 4, hd) - want).abs() <= tol).all())
