@@ -111,12 +111,15 @@ __global__ __launch_bounds__(256) void attn_kv4_plain_kernel(const Kv4AttnParams
   if (a.splits > 1 && threadIdx.x == 0) a.part_l[(size_t)blockIdx.x * a.splits + split] = bad ? NAN : top + log2f(total);
 }
 
-// Joining the ranges of a column: out = sum_s o_s 2^(l_s - max l) / sum_s 2^(l_s - max l).  One wave a column; a range whose weight is no number makes it so.
+// Joining the ranges of a column: out = sum_s o_s 2^(l_s - max l) / sum_s 2^(l_s - max l).  A workgroup a column, a wave eight ranges of it and every 32nd eight behind them (2 rows of 64 heads in 32
+// ranges each: 6.0 us, by one wave a column 9.2); a range whose weight is no number makes it so.
 // ``tile_tokens`` 0: columns are (token, head); otherwise (tile, token of the tile, head), and of a tile with fewer tokens nothing is written.
+#define KV4_JOIN_WAVES 4
 template <typename T>
-__global__ __launch_bounds__(64) void attn_kv4_join_kernel(const Kv4AttnParams a, int tile_tokens) {
+__global__ __launch_bounds__(KV4_JOIN_WAVES * NS_WAVE) void attn_kv4_join_kernel(const Kv4AttnParams a, int tile_tokens) {
+  __shared__ float sums[KV4_JOIN_WAVES][KV4_MAX_HD];
   const size_t col = blockIdx.x;
-  const int lane = threadIdx.x, head = col % a.heads;
+  const int lane = threadIdx.x % NS_WAVE, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / NS_WAVE), waves = blockDim.x / NS_WAVE, head = col % a.heads;
   size_t row = col / a.heads;
   if (tile_tokens) {
     const int* info = a.tiles + row / tile_tokens * 8;
@@ -125,12 +128,12 @@ __global__ __launch_bounds__(64) void attn_kv4_join_kernel(const Kv4AttnParams a
     row = info[2] + token;
   }
   const float* from = a.part_o + col * a.splits * a.hd;
-  // the first eight results are asked for before it is known which count
+  // a wave's first eight results are asked for before it is known which count
   float x[4][8];
 #pragma unroll
   for (int i = 0; i < 4; ++i)
 #pragma unroll
-    for (int s = 0; s < 8; ++s) x[i][s] = lane + 64 * i < a.hd && s < a.splits ? from[(size_t)s * a.hd + lane + 64 * i] : 0.f;
+    for (int s = 0; s < 8; ++s) x[i][s] = lane + 64 * i < a.hd && 8 * wave + s < a.splits ? from[(size_t)(8 * wave + s) * a.hd + lane + 64 * i] : 0.f;
   const float ls = lane < a.splits ? a.part_l[col * a.splits + lane] : -INFINITY;
   // (results are there from the first on; where there is none the row has been written whole)
   const int used = __popcll(__ballot(ls != -INFINITY));
@@ -143,17 +146,28 @@ __global__ __launch_bounds__(64) void attn_kv4_join_kernel(const Kv4AttnParams a
     if (64 * i >= a.hd) break;
     float o = 0.f;
 #pragma unroll
-    for (int s = 0; s < 8; ++s) o += s < used ? x[i][s] * __shfl(weight, s, NS_WAVE) : 0.f;
-    for (int s0 = 8; s0 < used; s0 += 8) {  // eight results' loads on their way at a time
+    for (int s = 0; s < 8; ++s) o += 8 * wave + s < used ? x[i][s] * __shfl(weight, 8 * wave + s, NS_WAVE) : 0.f;
+    for (int s0 = 8 * (wave + waves); s0 < used; s0 += 8 * waves) {  // eight results' loads on their way at a time
       float more[8];
 #pragma unroll
       for (int s = 0; s < 8; ++s) more[s] = c < a.hd ? from[(size_t)min(s0 + s, used - 1) * a.hd + c] : 0.f;
 #pragma unroll
       for (int s = 0; s < 8; ++s) o += s0 + s < used ? more[s] * __shfl(weight, (s0 + s) & 63, NS_WAVE) : 0.f;
     }
-    if (c < a.hd) ((T*)a.out)[(row * a.heads + head) * a.hd + c] = from_f<T>(o / total);
+    if (waves > 1)
+      sums[wave][c] = o;
+    else if (c < a.hd)
+      ((T*)a.out)[(row * a.heads + head) * a.hd + c] = from_f<T>(o / total);
+  }
+  if (waves == 1) return;
+  __syncthreads();
+  for (int c = threadIdx.x; c < a.hd; c += blockDim.x) {
+    float o = sums[0][c];
+    for (int v = 1; v < waves; ++v) o += sums[v][c];
+    ((T*)a.out)[(row * a.heads + head) * a.hd + c] = from_f<T>(o / total);
   }
 }
+static unsigned kv4_join_threads(int splits) { return (unsigned)min((splits + 7) / 8, KV4_JOIN_WAVES) * NS_WAVE; }
 
 template <typename T>
 static void launch_plain(const Kv4AttnParams& a, int tokens, hipStream_t stream) {
@@ -164,7 +178,7 @@ static void launch_plain(const Kv4AttnParams& a, int tokens, hipStream_t stream)
     case 3: attn_kv4_plain_kernel<T, 3><<<grid, 256, 0, stream>>>(a); break;
     default: attn_kv4_plain_kernel<T, 4><<<grid, 256, 0, stream>>>(a);
   }
-  if (a.splits > 1) attn_kv4_join_kernel<T><<<(unsigned)(tokens * a.heads), 64, 0, stream>>>(a, 0);
+  if (a.splits > 1) attn_kv4_join_kernel<T><<<(unsigned)(tokens * a.heads), kv4_join_threads(a.splits), 0, stream>>>(a, 0);
 }
 
 extern "C" int ns_attn_kv4_plain(void* out, void* part_o, void* part_l, const void* q, int q_stride, const void* pool, const int* token_req, const int* positions,
@@ -209,7 +223,7 @@ static int launch_tiles(const Kv4AttnParams& a, int rows, int form, hipStream_t 
   if (a.splits > 1) {
     const long long cols = (long long)a.n_tiles * (rows ? 1 : KV4_TILE_TOKENS) * a.heads;
     if (cols > 0x7fffffff) return NS_ERR_UNSUPPORTED;
-    attn_kv4_join_kernel<T><<<(unsigned)cols, 64, 0, stream>>>(a, rows ? 1 : KV4_TILE_TOKENS);
+    attn_kv4_join_kernel<T><<<(unsigned)cols, kv4_join_threads(a.splits), 0, stream>>>(a, rows ? 1 : KV4_TILE_TOKENS);
   }
   return ns_launch_status();
 }

@@ -109,7 +109,7 @@ __global__ void int8_rows_kernel(const Int8RowsParams p) {
 template <typename T, int SRC, int V>
 static int launch_rows(const Int8RowsParams& p, int rows, hipStream_t stream) {
   const int pieces = p.k / V;
-  // (a wave for little, 1,024 threads for the widest rows: as many pieces a thread as there must be)
+  // (a wave for little, 1,024 threads for the widest rows: as many pieces a thread as there must be; four of fewer threads are no faster with many rows: 2,048 of 4,096 10.8 us and 10.7)
   const int chunks = (pieces + 1023) / 1024;
   int threads = (pieces + chunks - 1) / chunks;
   threads = (threads + 63) / 64 * 64;
