@@ -111,15 +111,14 @@ __global__ __launch_bounds__(256) void attn_kv4_plain_kernel(const Kv4AttnParams
   if (a.splits > 1 && threadIdx.x == 0) a.part_l[(size_t)blockIdx.x * a.splits + split] = bad ? NAN : top + log2f(total);
 }
 
-// Joining the ranges of a column: out = sum_s o_s 2^(l_s - max l) / sum_s 2^(l_s - max l).  A workgroup a column, a wave eight ranges of it and every 32nd eight behind them (2 rows of 64 heads in 32
-// ranges each: 6.0 us, by one wave a column 9.2); a range whose weight is no number makes it so.
+// Joining the ranges of a column: out = sum_s o_s 2^(l_s - max l) / sum_s 2^(l_s - max l).  A workgroup a column: a wave, or, of few columns in many ranges, four that take eight ranges each in turn (2 rows of 64 heads in 32
+// ranges each: 6.0 us, by a wave each 9.2); a range whose weight is no number makes it so.
 // ``tile_tokens`` 0: columns are (token, head); otherwise (tile, token of the tile, head), and of a tile with fewer tokens nothing is written.
-#define KV4_JOIN_WAVES 4
-template <typename T>
-__global__ __launch_bounds__(KV4_JOIN_WAVES * NS_WAVE) void attn_kv4_join_kernel(const Kv4AttnParams a, int tile_tokens) {
-  __shared__ float sums[KV4_JOIN_WAVES][KV4_MAX_HD];
+template <typename T, int WAVES>
+__global__ __launch_bounds__(WAVES * NS_WAVE) void attn_kv4_join_kernel(const Kv4AttnParams a, int tile_tokens) {
+  __shared__ float sums[WAVES][WAVES > 1 ? KV4_MAX_HD : 1];
   const size_t col = blockIdx.x;
-  const int lane = threadIdx.x % NS_WAVE, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / NS_WAVE), waves = blockDim.x / NS_WAVE, head = col % a.heads;
+  const int lane = threadIdx.x % NS_WAVE, wave = WAVES > 1 ? __builtin_amdgcn_readfirstlane(threadIdx.x / NS_WAVE) : 0, head = col % a.heads;
   size_t row = col / a.heads;
   if (tile_tokens) {
     const int* info = a.tiles + row / tile_tokens * 8;
@@ -147,27 +146,35 @@ __global__ __launch_bounds__(KV4_JOIN_WAVES * NS_WAVE) void attn_kv4_join_kernel
     float o = 0.f;
 #pragma unroll
     for (int s = 0; s < 8; ++s) o += 8 * wave + s < used ? x[i][s] * __shfl(weight, 8 * wave + s, NS_WAVE) : 0.f;
-    for (int s0 = 8 * (wave + waves); s0 < used; s0 += 8 * waves) {  // eight results' loads on their way at a time
+    for (int s0 = 8 * (wave + WAVES); s0 < used; s0 += 8 * WAVES) {  // eight results' loads on their way at a time
       float more[8];
 #pragma unroll
       for (int s = 0; s < 8; ++s) more[s] = c < a.hd ? from[(size_t)min(s0 + s, used - 1) * a.hd + c] : 0.f;
 #pragma unroll
       for (int s = 0; s < 8; ++s) o += s0 + s < used ? more[s] * __shfl(weight, (s0 + s) & 63, NS_WAVE) : 0.f;
     }
-    if (waves > 1)
+    if constexpr (WAVES > 1)
       sums[wave][c] = o;
     else if (c < a.hd)
       ((T*)a.out)[(row * a.heads + head) * a.hd + c] = from_f<T>(o / total);
   }
-  if (waves == 1) return;
+  if constexpr (WAVES == 1) return;
   __syncthreads();
   for (int c = threadIdx.x; c < a.hd; c += blockDim.x) {
     float o = sums[0][c];
-    for (int v = 1; v < waves; ++v) o += sums[v][c];
+#pragma unroll
+    for (int v = 1; v < WAVES; ++v) o += sums[v][c];
     ((T*)a.out)[(row * a.heads + head) * a.hd + c] = from_f<T>(o / total);
   }
 }
-static unsigned kv4_join_threads(int splits) { return (unsigned)min((splits + 7) / 8, KV4_JOIN_WAVES) * NS_WAVE; }
+template <typename T>
+static void launch_join(const Kv4AttnParams& a, unsigned columns, int tile_tokens, hipStream_t stream) {
+  // (many columns fill the card with a wave each: 21,000 of 9 ranges 24 us, with four 47)
+  if (a.splits <= 8 || columns > 4096)
+    attn_kv4_join_kernel<T, 1><<<columns, NS_WAVE, 0, stream>>>(a, tile_tokens);
+  else
+    attn_kv4_join_kernel<T, 4><<<columns, 4 * NS_WAVE, 0, stream>>>(a, tile_tokens);
+}
 
 template <typename T>
 static void launch_plain(const Kv4AttnParams& a, int tokens, hipStream_t stream) {
@@ -178,7 +185,7 @@ static void launch_plain(const Kv4AttnParams& a, int tokens, hipStream_t stream)
     case 3: attn_kv4_plain_kernel<T, 3><<<grid, 256, 0, stream>>>(a); break;
     default: attn_kv4_plain_kernel<T, 4><<<grid, 256, 0, stream>>>(a);
   }
-  if (a.splits > 1) attn_kv4_join_kernel<T><<<(unsigned)(tokens * a.heads), kv4_join_threads(a.splits), 0, stream>>>(a, 0);
+  if (a.splits > 1) launch_join<T>(a, (unsigned)(tokens * a.heads), 0, stream);
 }
 
 extern "C" int ns_attn_kv4_plain(void* out, void* part_o, void* part_l, const void* q, int q_stride, const void* pool, const int* token_req, const int* positions,
@@ -223,7 +230,7 @@ static int launch_tiles(const Kv4AttnParams& a, int rows, int form, hipStream_t 
   if (a.splits > 1) {
     const long long cols = (long long)a.n_tiles * (rows ? 1 : KV4_TILE_TOKENS) * a.heads;
     if (cols > 0x7fffffff) return NS_ERR_UNSUPPORTED;
-    attn_kv4_join_kernel<T><<<(unsigned)cols, kv4_join_threads(a.splits), 0, stream>>>(a, rows ? 1 : KV4_TILE_TOKENS);
+    launch_join<T>(a, (unsigned)cols, rows ? 1 : KV4_TILE_TOKENS, stream);
   }
   return ns_launch_status();
 }
