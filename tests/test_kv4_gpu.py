@@ -379,3 +379,25 @@ def test_values_of_a_key_without_weight_cost_the_others_nothing(lens, starts, dt
     alone[at] = 0
     tol = tolerance(dtype, want, size, hd, held, float(alone.abs().max()) / 4, float(alone.abs().max())) + 2.0**-40
     assert bool(((out.cpu().double().view(-1, 4, hd) - want).abs() <= tol).all())
+
+
+@pytest.mark.parametrize("rows,tokens,heads,kv_heads,hd", [(False, 150, 32, 8, 64), (False, 40, 4, 2, 128), (True, 3, 4, 2, 64), (True, 200, 32, 8, 128)])
+def test_any_number_of_ranges(rows, tokens, heads, kv_heads, hd):
+    """Few columns and many, joined from 2 to 64 ranges, some of them empty: the result of one range, but for weights rounded against another reference (2^-11 of values of up to 20) and the
+    result's own rounding."""
+    ops = _ops()
+    pool, _, _, _ = _pool(80, kv_heads, 16, hd, 3)
+    table = torch.arange(80, dtype=torch.int32, device=DEV).view(1, 80)
+    q = _rand((tokens, heads * hd), 2).bfloat16().to(DEV)
+    if rows:
+        tiles = torch.tensor([[0, 0, i, 1, 1280 - 6 * i, 0, 8 * tokens, 0] for i in range(tokens)], dtype=torch.int32, device=DEV)
+    else:
+        tiles = torch.tensor([[0, t0, 0, tokens, 1270, 0, 0, -1] for t0 in range(0, tokens, 32)], dtype=torch.int32, device=DEV)
+    results = []
+    for splits in (1, 2, 8, 9, 33, 64):
+        columns = tiles.shape[0] * (1 if rows else 32) * heads
+        work = tuple(torch.full((columns * splits * w,), math.nan, device=DEV) for w in (hd, 1)) if splits > 1 else None
+        out = torch.full((tokens, heads * hd), 7.0, dtype=torch.bfloat16, device=DEV)
+        ops.attention_kv4(q, out, pool, tiles, table, heads, kv_heads, hd, hd**-0.5, rows, splits=splits, workspace=work, groups=1 << 20)
+        results.append(out.float())
+    assert all(float((r - results[0]).abs().max()) <= 20 * (2 * 2.0**-11 + 2 * 2.0**-8) for r in results[1:])
