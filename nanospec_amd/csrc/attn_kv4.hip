@@ -62,7 +62,7 @@ __global__ __launch_bounds__(256) void attn_kv4_plain_kernel(const Kv4AttnParams
     const float top = fmaxf(m, wave_max(s)), base = top == -INFINITY ? 0.f : top, shrink = exp2f(m - base);
     const float p = exp2f(s - base), ps = seen ? p * kv4_step(vm) : 0.f;
     l = l * shrink + p;
-    z = z * shrink + (seen ? p * kv4_low(vm) : 0.f);
+    z = z * shrink + (seen ? p * fmaf(8.f, kv4_step(vm), kv4_low(vm)) : 0.f);  // (codes less 8: the two sums would be many times their own)
     m = top;
 #pragma unroll
     for (int c = 0; c < CH; ++c) acc[c] *= shrink;
@@ -77,7 +77,7 @@ __global__ __launch_bounds__(256) void attn_kv4_plain_kernel(const Kv4AttnParams
         const uint4 w = *reinterpret_cast<const uint4*>(vr + ch / 4 * 16);
         const uint32_t d[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
-        for (int e = 0; e < 8; ++e) acc[c] = fmaf(__shfl(ps, 8 * o + e, NS_WAVE), (float)(d[e / 2] >> (16 * (e % 2) + 4 * (ch % 4)) & 15u), acc[c]);
+        for (int e = 0; e < 8; ++e) acc[c] = fmaf(__shfl(ps, 8 * o + e, NS_WAVE), (float)((int)(d[e / 2] >> (16 * (e % 2) + 4 * (ch % 4)) & 15u) - 8), acc[c]);
       }
     }
   }
@@ -208,24 +208,24 @@ extern "C" int ns_attn_kv4_plain(void* out, void* part_o, void* part_l, const vo
 
 #include "attn_kv4_mfma.h"
 
-template <typename T, int HD, int PARTS>
+template <typename T, int HD, bool EXACT>
 static int launch_tiles(const Kv4AttnParams& a, int rows, int form, hipStream_t stream) {
   const int group = a.heads / a.kv_heads;
   if (rows) {
     if (a.n_tiles > 65535) return NS_ERR_UNSUPPORTED;
     const dim3 grid((unsigned)(a.kv_heads * ((group + 15) / 16)), (unsigned)a.n_tiles, (unsigned)a.splits);
     if (form == 8)
-      attn_kv4_rows_kernel<T, HD, PARTS, 8><<<grid, 512, 0, stream>>>(a);
+      attn_kv4_rows_kernel<T, HD, EXACT, 8><<<grid, 512, 0, stream>>>(a);
     else
-      attn_kv4_rows_kernel<T, HD, PARTS, 4><<<grid, 256, 0, stream>>>(a);
+      attn_kv4_rows_kernel<T, HD, EXACT, 4><<<grid, 256, 0, stream>>>(a);
   } else {
     const long long items = (long long)a.n_tiles * a.splits * a.heads * (KV4_TILE_TOKENS / form);
     if (items > 0x7fffffff - 4) return NS_ERR_UNSUPPORTED;
     const unsigned grid = (unsigned)((items + 3) / 4);
-    if constexpr (PARTS == 1) {
-      if (form == 32) attn_kv4_tiles_kernel<T, HD, 2, PARTS><<<grid, 256, 0, stream>>>(a);
+    if constexpr (!EXACT) {
+      if (form == 32) attn_kv4_tiles_kernel<T, HD, 2, EXACT><<<grid, 256, 0, stream>>>(a);
     }
-    if (form == 16) attn_kv4_tiles_kernel<T, HD, 1, PARTS><<<grid, 256, 0, stream>>>(a);
+    if (form == 16) attn_kv4_tiles_kernel<T, HD, 1, EXACT><<<grid, 256, 0, stream>>>(a);
   }
   if (a.splits > 1) {
     const long long cols = (long long)a.n_tiles * (rows ? 1 : KV4_TILE_TOKENS) * a.heads;
@@ -250,7 +250,7 @@ extern "C" int ns_attn_kv4(void* out, void* part_o, void* part_l, const void* q,
   const Kv4AttnParams a{out, (float*)part_o, (float*)part_l, q, (const uint8_t*)pool, tiles, nullptr, nullptr, block_table, q_stride, table_stride, n_tiles, heads, kv_heads,
                         hd, page, splits, window, groups, scale * 1.4426950408889634f,
                         ((uintptr_t)q & 15) == 0 && q_stride % (dtype == NS_DTYPE_F32 ? 4 : 8) == 0};
-  if (dtype == NS_DTYPE_F32) return hd == 64 ? launch_tiles<float, 64, 2>(a, rows, form, stream) : launch_tiles<float, 128, 2>(a, rows, form, stream);
-  if (dtype == NS_DTYPE_BF16) return hd == 64 ? launch_tiles<bf16_t, 64, 1>(a, rows, form, stream) : launch_tiles<bf16_t, 128, 1>(a, rows, form, stream);
+  if (dtype == NS_DTYPE_F32) return hd == 64 ? launch_tiles<float, 64, true>(a, rows, form, stream) : launch_tiles<float, 128, true>(a, rows, form, stream);
+  if (dtype == NS_DTYPE_BF16) return hd == 64 ? launch_tiles<bf16_t, 64, false>(a, rows, form, stream) : launch_tiles<bf16_t, 128, false>(a, rows, form, stream);
   return NS_ERR_UNSUPPORTED;
 }

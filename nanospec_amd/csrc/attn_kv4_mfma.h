@@ -13,9 +13,12 @@
 //   s = step (q . u) + low sum(q):      two operations a score, as both are a key's
 //   out = sum p step u + sum p low:     p step is the weight in the second product, the rest a sum of numbers
 // Queries are float16 on their way in, scaled by a power of two of their own so that the largest lies at 256: what is 2^-22 of it is exact.  Weights are
-// rounded to float16 (2^-12 of themselves).  PARTS 2: queries and weights as the sum of two float16 values each, two products for one.
+// rounded to float16 (2^-12 of themselves).
+// float32 (EXACT) takes the 32-bit matrix instructions, with codes as the numbers 16 (u - 8), bytes that a mask and a sign bit make, low + 8 step in the place of low, and everything in 32 bits.  (Queries and weights as two
+// float16 values each were faster and 1e-4 of the result off at 4,000 keys: the two sums above are many times what is left of them, and the instruction cuts off what lies below its largest product, always
+// downwards; bfloat16 does not see that.)
 //
-// The soft-max's reference R is one number a column for weights and steps together: R >= (score + log2 of its value's step) - 8 of every key so far, so
+// The soft-max's reference R is one number a column for weights and steps together: R >= (score + log2 of its value's step) - 15 of every key so far, so
 // that p step, p = 2^(s - R), fits float16 whatever the steps' size, and is only raised when that no longer holds (then every sum shrinks).  (Key by key: by the largest score and the largest step
 // apart, a value of great size whose key has next to no weight would cost the others their bits; that costs a portion 5%.)
 // It knows of the keys that the column sees, and of no others.
@@ -29,7 +32,8 @@ typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 
 #define KV4_TILE_INTS 8
 #define KV4_TILE_TOKENS 32  // of a portion's tile
-#define KV4_SLACK 8.f
+#define KV4_TOP 7.f    // log2 of the largest weight times step where the reference is raised to it, so that of small ones float16's subnormal numbers cost as little as may be ...
+#define KV4_SLACK 8.f  // ... and how far above that another may come before it is raised again: 2^15 is below float16's largest
 #define KV4_RANGE_BLOCKS 8  // of 32 keys: the fewest of a range of a single token's keys
 
 __device__ __forceinline__ f16x8 as_f16x8(uint32_t a, uint32_t b, uint32_t c, uint32_t d) { return __builtin_bit_cast(f16x8, u32x4{a, b, c, d}); }
@@ -38,6 +42,9 @@ __device__ __forceinline__ uint32_t kv4_ones(uint32_t w) { return w & 0x000f000f
 __device__ __forceinline__ uint32_t kv4_sixteens(uint32_t w) { return w & 0x00f000f0u; }
 // log2 of a mark's step + 127, up to 0.09 below it; at least 63 (of smaller steps is lost what float16 does not hold)
 __device__ __forceinline__ float kv4_log(uint32_t mark) { return (float)max(mark, 63u << 23) * 0x1p-23f; }
+// the upper codes of a dword's bytes as signed bytes 16 (u - 8), and one of them as a number
+__device__ __forceinline__ uint32_t kv4_signed(uint32_t w) { return (w & 0xf0f0f0f0u) ^ 0x80808080u; }
+__device__ __forceinline__ float kv4_byte(uint32_t w, int y) { return (float)(int8_t)(w >> (8 * y)); }
 __device__ __forceinline__ float quarters_max(float v) {
   v = fmaxf(v, __shfl_xor(v, 16, NS_WAVE));
   return fmaxf(v, __shfl_xor(v, 32, NS_WAVE));
@@ -55,13 +62,14 @@ struct Kv4Block {
   u32x4 km[2], vm[2];      // its octet's marks
 };
 
-// CT: tiles of 16 columns.  PARTS: 1 for bfloat16, 2 for float32.
-template <typename T, int HD, int CT, int PARTS>
+// CT: tiles of 16 columns.  EXACT: float32.
+template <typename T, int HD, int CT, bool EXACT>
 struct Kv4Wave {
   static constexpr int NG = HD / 32, NB = HD / 64;
   static constexpr int REC = 8 * HD + 64;
-  f16x8 q[CT][PARTS][NG];
-  float qsum[CT], unscale[CT];  // sum of the scaled queries, times 2^-24 as the products are; what a score is multiplied with: the scale, log2(e), the queries' own scale and the 2^-24 taken off
+  f16x8 q[CT][EXACT ? 1 : NG];
+  float q32[EXACT ? CT : 1][EXACT ? NG : 1][8];
+  float qsum[CT], unscale[CT];  // sum of the scaled queries, times 2^-24 as the products are; what a score is multiplied with: the scale, log2(e), the queries' own scale and the 2^-24 taken off (EXACT: neither)
   float R[CT], l[CT], z[CT];
   f32x4v o[CT][NB][4];
   int lane, col, t;
@@ -104,6 +112,16 @@ struct Kv4Wave {
 #pragma unroll
         for (int e = 0; e < 8; ++e) x[g][e] = to_f(from[32 * g + 8 * t + e]);
     }
+    if constexpr (EXACT) {
+      float sum = 0.f;
+#pragma unroll
+      for (int g = 0; g < NG; ++g)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) q32[c][g][e] = x[g][e], sum += x[g][e];
+      qsum[c] = quarters_sum(sum);
+      unscale[c] = scale_log2;
+      return;
+    }
 #pragma unroll
     for (int g = 0; g < NG; ++g)
 #pragma unroll
@@ -117,18 +135,16 @@ struct Kv4Wave {
     float sum = 0.f;
 #pragma unroll
     for (int g = 0; g < NG; ++g) {
-      f16x8 hi, lo;
+      f16x8 hi;
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         // channels 2, 3, 6, 7 of the eight meet codes times 16
         const float y = x[g][e] * by, s = e & 2 ? y * 0.0625f : y;
         hi[e] = (_Float16)s;
-        lo[e] = (_Float16)(s - (float)hi[e]);
         // what a lowest value meets are the queries as they are multiplied
-        sum += PARTS == 1 ? (e & 2 ? 16.f * (float)hi[e] : (float)hi[e]) : y;
+        sum += e & 2 ? 16.f * (float)hi[e] : (float)hi[e];
       }
-      q[c][0][g] = hi;
-      if constexpr (PARTS == 2) q[c][1][g] = lo;
+      q[c][g] = hi;
     }
     qsum[c] = quarters_sum(sum) * 0x1p-24f;
   }
@@ -182,7 +198,7 @@ struct Kv4Wave {
 
   // From the products of 8 keys with a column of tile c to its weights, in p.  ``v_log``: about log2 of the keys' steps for values, + 127.
   __device__ __forceinline__ void soften(int c, const f32x4v* d, const float* k_step, const float* k_low, const float* v_step, const float* v_low, const float* v_log, int k0, bool mask,
-                                         f16x8* p) {
+                                         float* p) {
     float s[8], reach = -INFINITY;
 #pragma unroll
     for (int e = 0; e < 8; ++e) s[e] = fmaf(k_step[e], d[e / 4][e % 4], k_low[e] * qsum[c]);
@@ -195,7 +211,7 @@ struct Kv4Wave {
     }
 #pragma unroll
     for (int e = 0; e < 8; ++e) reach = fmaxf(reach, fmaf(s[e], unscale[c], v_log[e]));
-    reach -= 127.f;
+    reach -= 127.f + KV4_TOP;
     if (__any(reach > R[c] + KV4_SLACK)) {
       const float want = quarters_max(reach), next = want > R[c] + KV4_SLACK ? want : R[c], base = next == -INFINITY ? 0.f : next;
       const float shrink = __builtin_amdgcn_exp2f(R[c] - base);
@@ -222,28 +238,27 @@ struct Kv4Wave {
       for (int e = 0; e < 8; ++e) z[c] = fmaf(w[e], v_low[e], z[c]);
     }
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const float ps = w[e] * v_step[e];
-      p[0][e] = (_Float16)ps;
-      if constexpr (PARTS == 2) p[1][e] = (_Float16)(ps - (float)p[0][e]);
-    }
+    for (int e = 0; e < 8; ++e) p[e] = w[e] * v_step[e];
   }
 
   // The 32 keys from k0 on.  ``mask``: some column may not see all of them.  What has been used of the block is loaded anew, from ``then``, at once: a load has most
   // of a block's time to arrive, and there is one set of registers for them.
   __device__ __forceinline__ void block(Kv4Block<HD>& b, int k0, bool mask, const At& then) {
     // keys as operands
-    f16x8 ka[2][NG];
+    f16x8 ka[2][EXACT ? 1 : NG];
+    uint32_t kw[2][EXACT ? NG : 1];
 #pragma unroll
     for (int a = 0; a < 2; ++a)
 #pragma unroll
       for (int g = 0; g < NG; ++g) {
         const uint32_t w = b.k[a][g], w8 = w >> 8;
-        ka[a][g] = as_f16x8(kv4_ones(w), kv4_sixteens(w), kv4_ones(w8), kv4_sixteens(w8));
+        if constexpr (EXACT)
+          kw[a][g] = w;
+        else
+          ka[a][g] = as_f16x8(kv4_ones(w), kv4_sixteens(w), kv4_ones(w8), kv4_sixteens(w8));
       }
     load_keys(b, then);
     __builtin_amdgcn_sched_barrier(0);
-    f16x8 p[CT][PARTS];
     float k_step[8], k_low[8], v_step[8], v_low[8];
     float v_log[8];
 #pragma unroll
@@ -254,9 +269,16 @@ struct Kv4Wave {
       v_step[e] = kv4_step(vm);
       v_low[e] = kv4_low(vm);
       v_log[e] = kv4_log(vm);
+      if constexpr (EXACT) {
+        k_low[e] = fmaf(8.f, k_step[e], k_low[e]);
+        v_low[e] = fmaf(8.f, v_step[e], v_low[e]);
+        k_step[e] *= 0.0625f;
+      }
     }
     load_marks(b.km, then, 0);
     load_marks(b.vm, then, 1);
+    f16x8 p[CT];
+    float p32[CT][8];
 #pragma unroll
     for (int c = 0; c < CT; ++c) {
       f32x4v d[2];
@@ -264,17 +286,47 @@ struct Kv4Wave {
       for (int a = 0; a < 2; ++a) {
         d[a] = f32x4v{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int g = 0; g < NG; ++g)
+        for (int g = 0; g < NG; ++g) {
+          if constexpr (EXACT) {
+            // bytes: channels 2, 6, 3, 7 of the eight, and 0, 4, 1, 5
+            const uint32_t upper = kv4_signed(kw[a][g]), lower = kv4_signed(kw[a][g] << 4);
 #pragma unroll
-          for (int h = 0; h < PARTS; ++h) d[a] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ka[a][g], q[c][h][g], d[a], 0, 0, 0);
+            for (int y = 0; y < 4; ++y) {
+              const int e = y % 2 * 4 + y / 2;
+              d[a] = __builtin_amdgcn_mfma_f32_16x16x4f32(kv4_byte(lower, y), q32[c][g][e], d[a], 0, 0, 0);
+              d[a] = __builtin_amdgcn_mfma_f32_16x16x4f32(kv4_byte(upper, y), q32[c][g][e + 2], d[a], 0, 0, 0);
+            }
+          } else {
+            d[a] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ka[a][g], q[c][g], d[a], 0, 0, 0);
+          }
+        }
       }
-      soften(c, d, k_step, k_low, v_step, v_low, v_log, k0, mask, p[c]);
+      soften(c, d, k_step, k_low, v_step, v_low, v_log, k0, mask, p32[c]);
+      if constexpr (!EXACT)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) p[c][e] = (_Float16)p32[c][e];
       __builtin_amdgcn_sched_barrier(0);
     }
     // values as operands, four channels of each 64 a lane
 #pragma unroll
     for (int n = 0; n < NB; ++n) {
       u32x4 w = b.v[n];
+      if constexpr (EXACT) {
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+          // bytes: channels 1 and 3 of key 2 x, then of 2 x + 1; channels 0 and 2
+          const uint32_t upper = kv4_signed(w[x]), lower = kv4_signed(w[x] << 4);
+#pragma unroll
+          for (int y = 0; y < 4; ++y)
+#pragma unroll
+            for (int c = 0; c < CT; ++c) {
+              f32x4v* to = o[c][n] + y % 2 * 2;
+              to[0] = __builtin_amdgcn_mfma_f32_16x16x4f32(kv4_byte(lower, y), p32[c][2 * x + y / 2], to[0], 0, 0, 0);
+              to[1] = __builtin_amdgcn_mfma_f32_16x16x4f32(kv4_byte(upper, y), p32[c][2 * x + y / 2], to[1], 0, 0, 0);
+            }
+        }
+        continue;
+      }
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         uint32_t r[4];
@@ -285,9 +337,7 @@ struct Kv4Wave {
         }
         const f16x8 va = as_f16x8(r[0], r[1], r[2], r[3]);
 #pragma unroll
-        for (int c = 0; c < CT; ++c)
-#pragma unroll
-          for (int h = 0; h < PARTS; ++h) o[c][n][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(va, p[c][h], o[c][n][i], 0, 0, 0);
+        for (int c = 0; c < CT; ++c) o[c][n][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(va, p[c], o[c][n][i], 0, 0, 0);
         if (i & 1) __builtin_amdgcn_sched_barrier(0);
       }
     }
@@ -315,16 +365,16 @@ struct Kv4Wave {
     low = quarters_sum(z[c]);
     return total == 0.f ? -INFINITY : R[c] + __log2f(total);
   }
-  __device__ __forceinline__ float sum_of(int c, int n, int e) const { return (e & 1 ? 0x1p20f : 0x1p24f) * o[c][n][e % 4][e / 4]; }
+  __device__ __forceinline__ float sum_of(int c, int n, int e) const { return (EXACT ? 0.0625f : e & 1 ? 0x1p20f : 0x1p24f) * o[c][n][e % 4][e / 4]; }
 };
 
 // Single tokens: a workgroup a (token, key/value head, 16 query heads of its group, range of keys), whose waves take blocks of 32 keys in turn and meet in LDS.  Ranges are even and as many
 // as give ``a.groups`` workgroups over all tokens: a row twice as long as others has twice as many.
 // Bound by memory where the rows are long and many (61 rows of 200 to 12,000 keys, 8 key/value heads of 128 channels: 94 us, 4.2 TB/s; 64 rows of 6,000: 5.3), by one workgroup's
 // chain of loads where they are few (a row of 1,000, in eight waves: 9.3 us).  Two blocks on their way at a time were slower everywhere (their registers cost a wave a SIMD).
-template <typename T, int HD, int PARTS, int WAVES>
+template <typename T, int HD, bool EXACT, int WAVES>
 __global__ __launch_bounds__(WAVES * 64) __attribute__((amdgpu_waves_per_eu(3))) void attn_kv4_rows_kernel(const Kv4AttnParams a) {
-  typedef Kv4Wave<T, HD, 1, PARTS> Wave;
+  typedef Kv4Wave<T, HD, 1, EXACT> Wave;
   __shared__ float outs[WAVES][16][HD + 4];
   __shared__ float weights[WAVES][16];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / NS_WAVE);
@@ -440,9 +490,9 @@ __device__ __forceinline__ void kv4_columns_out(const Wave& w, const Kv4AttnPara
 // Bound by vector instructions: a block of 32 keys and 32 columns of 128 channels has 32 matrix instructions (512 cycles) and about 320 others (1,430), of which 112 make operands of the
 // codes and 16 are exponentials; they are under way 73% of the time.  2,048 tokens at 16,000 keys: 809 us, 706 TFLOP/s; 2,048 at none 73 us.  Four tiles of columns a wave (each operand made
 // for twice as many) leave one wave a SIMD and nothing to fill its waits: 1,203 and 149 us.  Operands made by four waves for each other, by way of LDS, with a barrier a block: 828 and 90, where these took 772 and 75.
-template <typename T, int HD, int CT, int PARTS>
+template <typename T, int HD, int CT, bool EXACT>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void attn_kv4_tiles_kernel(const Kv4AttnParams a) {
-  typedef Kv4Wave<T, HD, CT, PARTS> Wave;
+  typedef Kv4Wave<T, HD, CT, EXACT> Wave;
   constexpr int TOKENS = 16 * CT, PIECES = KV4_TILE_TOKENS / TOKENS;  // of a wave; of a tile
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / NS_WAVE);
   // (late tiles see the most keys: they begin first)

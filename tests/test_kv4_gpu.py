@@ -165,14 +165,14 @@ def _pool(pages, kv_heads, page, hd, seed, spread=1.0, held=None):
 
 def tolerance(dtype, out, size, hd, keys, v_step, v_most):
     """How far attention may be off, for |out| and the sizes at hand (``size``: the largest sum of |q| |k| scale of a visible pair).
-    A score is at most 2 hd + 4 roundings of 2^-24 of ``size`` off (products and sums in 32 bits).  On the matrix cores queries are float16, one value for bfloat16, two for float32, scaled so that the
-    largest channel lies at 256 (or 16, where codes count sixteen times): a bfloat16 channel is exact but for what is below 2^-29 of the largest.  For bfloat16 70 roundings for every 8 channels are allowed.
+    A score is at most 2 hd + 4 roundings of 2^-24 of ``size`` off (products and sums in 32 bits).  bfloat16's queries are float16 on the matrix cores, scaled so that the
+    largest channel lies at 256 (or 16, where codes count sixteen times): exact but for what is below 2^-29 of the largest; 70 roundings for every 8 channels are allowed for them.
     The soft-max's weights are off by exp(2 delta) - 1 and the roundings of 2^x (2 units); bfloat16 rounds them to float16 on their way into the second product: 2^-11, and 2^-25 of the
     largest for those below the normal range, times keys; sums over the keys add 2^-24 each, of all that is summed (values and codes times steps: at most v_most + 8 steps)."""
     exact = dtype == torch.float32
     delta = size * 2.0**-24 * ((2 * hd + 4) if exact else max(2 * hd + 4, 70 * (hd / 8 + 2)))
     weight = math.expm1(2 * delta) + 2.0**-21 + (2.0**-22 if exact else 2.0**-11)
-    # (one part in float16 of a weight below 2^-14 of the largest is off by 2^-25; float32's second part by 2^-36 or less)
+    # (a weight in float16 below 2^-14 of the largest is off by 2^-25; in 32 bits by less than 2^-34)
     small = (2.0**-34 if exact else 2.0**-25) * min(keys, 2**14)
     sums = min(keys, 4096) * 2.0**-24
     return (v_most + 8 * v_step) * (weight + small + sums) + ROUND[dtype] * out.abs()
@@ -401,3 +401,13 @@ def test_any_number_of_ranges(rows, tokens, heads, kv_heads, hd):
         ops.attention_kv4(q, out, pool, tiles, table, heads, kv_heads, hd, hd**-0.5, rows, splits=splits, workspace=work, groups=1 << 20)
         results.append(out.float())
     assert all(float((r - results[0]).abs().max()) <= 20 * (2 * 2.0**-11 + 2 * 2.0**-8) for r in results[1:])
+
+
+@pytest.mark.parametrize("lens,starts", [([1, 1], [4000, 18000]), ([20], [6000])])
+@pytest.mark.parametrize("hd", [64, 96, 128])
+def test_float32_over_many_keys(hd, lens, starts):
+    """A mean of many values is many times smaller than they are, and than sums of codes apart from lowest values.  In 32 bits throughout, the error is a small part of it all the same: a score of size 4 is some
+    2^-24 sqrt(2 hd) of that off, 4e-6, and weights that are off by so much at random change a sum of the values at random by as much of itself; the exponential adds 2^-22, the sums, of blocks that are added up
+    by waves and ranges, 2^-24 for the root of their number.  Together under 1e-5 of the root mean square."""
+    got, want, _, _ = _attend((lens, starts), 4, 2, hd, 16, torch.float32, seed=hd, spread=0.3)
+    assert float((got - want).norm() / want.norm()) <= 1e-5
