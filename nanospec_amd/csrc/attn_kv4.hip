@@ -134,9 +134,10 @@ __global__ __launch_bounds__(WAVES * NS_WAVE) void attn_kv4_join_kernel(const Kv
 #pragma unroll
     for (int s = 0; s < 8; ++s) x[i][s] = lane + 64 * i < a.hd && 8 * wave + s < a.splits ? from[(size_t)(8 * wave + s) * a.hd + lane + 64 * i] : 0.f;
   const float ls = lane < a.splits ? a.part_l[col * a.splits + lane] : -INFINITY;
-  // (results are there from the first on; where there is none the row has been written whole)
-  const int used = __popcll(__ballot(ls != -INFINITY));
-  if (used == 0) return;
+  // (results are there up to the last that counts, those in front of a token's window of weight 0; where none counts the row has been written whole)
+  const uint64_t counts = __ballot(ls != -INFINITY);
+  if (counts == 0) return;
+  const int used = 64 - __clzll(counts);
   const float top = wave_max(ls), base = top == -INFINITY ? 0.f : top;
   const float weight = exp2f(ls - base), total = wave_sum(weight);
 #pragma unroll

@@ -411,3 +411,21 @@ def test_float32_over_many_keys(hd, lens, starts):
     by waves and ranges, 2^-24 for the root of their number.  Together under 1e-5 of the root mean square."""
     got, want, _, _ = _attend((lens, starts), 4, 2, hd, 16, torch.float32, seed=hd, spread=0.3)
     assert float((got - want).norm() / want.norm()) <= 1e-5
+
+
+@pytest.mark.parametrize("window", [1, 5, 31, 33, 70])
+@pytest.mark.parametrize("splits", [2, 5, 64])
+def test_ranges_that_a_window_hides(window, splits):
+    """Ranges of a portion's keys so short that some tokens' windows begin behind the first of them, and end in front of the last."""
+    ops = _ops()
+    pool, keys, values, v_step = _pool(20, 2, 16, 64, 3)
+    table = torch.arange(20, dtype=torch.int32, device=DEV).view(1, 20)
+    for dtype in (torch.bfloat16, torch.float32):
+        q = _rand((45, 256), 2).to(dtype)
+        tiles = torch.tensor([[0, 0, 0, 45, 300, 0, 0, -1], [0, 32, 0, 45, 300, 0, 0, -1]], dtype=torch.int32, device=DEV)
+        work = tuple(torch.full((2 * 32 * 4 * splits * w,), math.nan, device=DEV) for w in (64, 1))
+        out = torch.full((45, 256), 7.0, dtype=dtype, device=DEV)
+        ops.attention_kv4(q.to(DEV), out, pool, tiles, table, 4, 2, 64, 0.125, False, window=window, splits=splits, workspace=work)
+        want, size = oracle.attention(q.double().view(45, 4, 64), keys, values, [45], [255], table.cpu(), 16, 4, 2, 0.125, window)
+        tol = tolerance(dtype, want, size, 64, 300, v_step, float(values.abs().max()))
+        assert bool(((out.cpu().double().view(45, 4, 64) - want).abs() <= tol).all())
