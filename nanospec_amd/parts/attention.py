@@ -30,12 +30,13 @@ F32_RANGE_KEYS = 128  # keys of a range of a single token's row in 32-bit: two t
 # Attention over keys and values in 4 bits (us, 32 heads on 8 of 128 channels unless said otherwise)
 KV4_MAX_RANGES = 64  # of a row's keys
 KV4_RANGE_KEYS = 256  # the fewest keys of a single token's: with fewer a workgroup's beginning and end are longer than its blocks
-# The fewest keys of a range of a portion's, and the most where there are ranges at all (their lengths differ with the tiles': 666 tokens at 20,000 keys 440 in 2 ranges, 364 in 4, 347 in 6,
-# 339 in 8, 352 in 12; 512 at 8,000 158 in 2, 117 in 4, 128 in 6).  Ranges cost what joining their results takes: 2,048 tokens 69 in one range, 103 in two; 100 tokens at 1,000 keys 28 and, in 8, 19.
+# The fewest keys of a range of a portion's, and the most where there are ranges at all (their lengths differ with the tiles': 666 tokens at 20,000 keys 461 in 2 ranges, 380 in 4, 363 in 6,
+# 352 in 8, 364 in 12; 512 at 8,000 169 in 2, 122 in 4, 133 in 6).  Ranges cost what joining their results takes: 2,048 tokens 78 in one range, 103 in two; 100 tokens at 1,000 keys 31 and, in 8, 23.
 KV4_PORTION_KEYS = 128, 2560
 # The keys up to which a wave takes 16 tokens of a portion (three or four waves a SIMD, which hide each other's waits and end evenly) instead of 32 (two, each key made an operand once for
-# both halves).  2,048 tokens 69 and 81, 100 at 1,000 keys 19 and 23; 512 at 8,000 133 and 118, 2,048 at 16,000 888 and 778.
-KV4_NARROW_KEYS = 4096
+# both halves).  2,048 tokens 78 and 81 (of 64 channels 57 and 64), 100 at 1,000 keys 21 and 24; 512 at 2,000 54 and 53, 4,096 at none 238 and 218, 1,024 of 64 heads at 3,000 216 and 180, 512 at 8,000 138 and 122, 2,048 at
+# 16,000 933 and 811.
+KV4_NARROW_KEYS = 2048
 # Workgroups of four waves that single tokens' keys are cut for, for each compute unit.  Of 1, 2, 3 and 4: 8 rows of 4,000 keys 18.2, 17.6, 20.6, 21.4; 61 of 200 to 12,000 89, 93, 95, 90;
 # 2 of 100,000 (64 heads) 64, 62, 67, 70; one of 32,000 20, 24, 24, 24; 64 of 6,000 (64 channels) 67, 62, 62, 65.
 KV4_GROUPS_PER_UNIT = 2
