@@ -31,7 +31,7 @@ F32_RANGE_KEYS = 128  # keys of a range of a single token's row in 32-bit: two t
 KV4_MAX_RANGES = 64  # of a row's keys
 KV4_RANGE_KEYS = 256  # the fewest keys of a single token's: with fewer a workgroup's beginning and end are longer than its blocks
 # The fewest keys of a range of a portion's, and the most where there are ranges at all (their lengths differ with the tiles': 666 tokens at 20,000 keys 461 in 2 ranges, 380 in 4, 363 in 6,
-# 352 in 8, 364 in 12; 512 at 8,000 169 in 2, 122 in 4, 133 in 6).  Ranges cost what joining their results takes: 2,048 tokens 78 in one range, 103 in two; 100 tokens at 1,000 keys 31 and, in 8, 23.
+# 352 in 8, 364 in 12, and 390 in 9, whose waves come to 3.1 rounds of the card; 512 at 8,000 169 in 2, 122 in 4, 133 in 6).  Ranges cost what joining their results takes: 2,048 tokens 78 in one range, 103 in two; 100 tokens at 1,000 keys 31 and, in 8, 23.
 KV4_PORTION_KEYS = 128, 2560
 # The keys up to which a wave takes 16 tokens of a portion (three or four waves a SIMD, which hide each other's waits and end evenly) instead of 32 (two, each key made an operand once for
 # both halves).  2,048 tokens 78 and 81 (of 64 channels 57 and 64), 100 at 1,000 keys 21 and 24; 512 at 2,000 54 and 53, 4,096 at none 238 and 218, 1,024 of 64 heads at 3,000 216 and 180, 512 at 8,000 138 and 122, 2,048 at
@@ -263,9 +263,12 @@ def kv4_attention(ctx, q, out, pages, table, heads: int, kv_heads: int, head_dim
     if portions.shape[0]:
         tiles, longest = portions.shape[0], min(ctx.max_chunk_kv, span + TilePlan.TOKENS)
         wave_tokens = 16 if q.dtype == torch.float32 or longest <= KV4_NARROW_KEYS else TilePlan.TOKENS
-        # ranges until there are eight waves for each compute unit, if there are not without
-        waves, least, most = tiles * heads * (TilePlan.TOKENS // wave_tokens), *KV4_PORTION_KEYS
-        splits = 1 if waves >= 8 * units else max(1, min(KV4_MAX_RANGES, max(-(-8 * units // waves), -(-longest // most)), longest // least))
+        # ranges until there are eight waves for each compute unit, if there are not without, and as many of them as fill those rounds
+        waves, (least, most), full = tiles * heads * (TilePlan.TOKENS // wave_tokens), KV4_PORTION_KEYS, 8 * units
+        splits = 1
+        if waves < full:
+            rounds = max(1, round(waves * max(-(-full // waves), -(-longest // most)) / full))
+            splits = max(1, min(KV4_MAX_RANGES, rounds * full // waves, longest // least))
         ops.attention_kv4(q, out, pages, portions, table, heads, kv_heads, head_dim, scale, rows=False, window=window, splits=splits, form=wave_tokens,
                           workspace=workspace(tiles * TilePlan.TOKENS * heads, splits))
     if singles.shape[0]:
