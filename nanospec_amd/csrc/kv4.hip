@@ -38,9 +38,11 @@ __device__ __forceinline__ Kv4Row kv4_marks_of(const float* x, bool has, int W) 
   const float step = bf16_ceil(reach / 15.f);
   return {low, step < KV4_TINY ? 0.f : step};
 }
-// Divided, not times 1 / step: of short numbers (bfloat16 inputs) many lie half way between two codes exactly, and the quotient keeps that
-__device__ __forceinline__ uint32_t kv4_code(float x, const Kv4Row r) {
-  return r.step > 0.f ? (uint32_t)fminf(fmaxf(rintf((x - r.low) / r.step), 0.f), 15.f) : 0u;
+// Divided, not times 1 / step: of short numbers (bfloat16 inputs) many lie half way between two codes exactly, and the quotient keeps that.  With y = 1 / step rounded to nearest, and q a
+// quotient that is off by no more than its last bit, q + (a - q step) y is the quotient rounded to nearest (Markstein 1990): a reciprocal a row and three operations a value.
+__device__ __forceinline__ uint32_t kv4_code(float x, const Kv4Row r, float y) {
+  const float a = x - r.low, q = a * y;
+  return (uint32_t)fminf(fmaxf(rintf(fmaf(fmaf(-q, r.step, a), y, q)), 0.f), 15.f);
 }
 
 template <typename T>
@@ -154,7 +156,7 @@ struct Kv4WriteParams {
 
 // A workgroup a token; its groups of W lanes take the rows (queries, keys, values, as they lie in qkv) in turn, UNITS of them at once: all that a thread reads is on its way before the
 // token's angles are made and before anything is written (in place, the partners are each other's).
-// Bound by memory with many tokens (4,095 of 32 heads on 8 of 128 channels, 88 MB: 24 us, 3.6 TB/s; a row after the other 29), by one chain of loads with few.
+// Bound by memory with many tokens (4,095 of 32 heads on 8 of 128 channels, 88 MB: 23 us, 3.8 TB/s; a row after the other 29, with eight divisions a lane 24), by one chain of loads with few.
 template <typename T, bool WIDE, int UNITS>
 __global__ __launch_bounds__(256) void rope_kv4_kernel(const Kv4WriteParams p) {
   extern __shared__ __attribute__((aligned(16))) float cs[];  // cos[half] | sin[half] of this token's angles
@@ -193,14 +195,15 @@ __global__ __launch_bounds__(256) void rope_kv4_kernel(const Kv4WriteParams p) {
       }
       const Kv4Row m = kv4_marks_of(x, live, W);
       if (!live) continue;
+      const float y = m.step > 0.f ? 1.f / m.step : 0.f;  // (0: all codes are 0)
       const int h = r - (value ? keys : p.heads);
       uint8_t* to = p.pool + kv4_at(page, p.kv_heads, h, p.page / KV4_TOKENS, off / KV4_TOKENS) * record;
       if (value) {
         uint32_t lo = 0, hi = 0;
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          lo |= kv4_code(x[e], m) << (4 * e);
-          hi |= kv4_code(x[4 + e], m) << (4 * e);
+          lo |= kv4_code(x[e], m, y) << (4 * e);
+          hi |= kv4_code(x[4 + e], m, y) << (4 * e);
         }
         uint16_t* d = reinterpret_cast<uint16_t*>(to + kv4_values_at(p.hd) + 2 * o * 16 + j * 2);
         d[0] = (uint16_t)lo;
@@ -208,7 +211,7 @@ __global__ __launch_bounds__(256) void rope_kv4_kernel(const Kv4WriteParams p) {
       } else {
         uint32_t w = 0;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) w |= kv4_code(x[e], m) << (4 * (e / 2) + 16 * (e % 2));
+        for (int e = 0; e < 8; ++e) w |= kv4_code(x[e], m, y) << (4 * (e / 2) + 16 * (e % 2));
         reinterpret_cast<uint32_t*>(to + j * (p.hd / 2))[o % 4 * groups + o / 4] = w;
       }
       if (o == 0)
