@@ -1215,8 +1215,32 @@ class Int8Rows:
     nothing), ``scales`` float32 [rows], which stand for scale * code.  Made by ``int8_rows``, ``rmsnorm_int8`` and ``silu_mul_int8``, taken by ``linear_int8``."""
 
     def __init__(self, data: torch.Tensor, scales: torch.Tensor, k: int) -> None:
-        self.data, self.scales, self.k = data, scales, k
+        self._data, self._scales, self.k = data, scales, k
         self.shape = (scales.shape[0], k)
+        self.whole = None
+
+    @classmethod
+    def _made(cls, m: int, k: int, device, take) -> "Int8Rows":
+        """Room for m rows in one piece of memory (every tensor costs a step that is launched kernel by kernel a microsecond), scales behind the codes."""
+        self = cls.__new__(cls)
+        self._data = self._scales = None
+        self.k, self.kp, self.shape = k, int8_padded_k(k), (m, k)
+        self.codes_size = -(-m // 16) * 16 * self.kp
+        size = self.codes_size + 4 * m
+        self.whole = take((size,), torch.int8) if take is not None else torch.empty(size, dtype=torch.int8, device=device)
+        return self
+
+    @property
+    def data(self) -> torch.Tensor:
+        if self._data is None:
+            self._data = self.whole[: self.codes_size].view(-1, self.kp // 64, 4, 16, 16)
+        return self._data
+
+    @property
+    def scales(self) -> torch.Tensor:
+        if self._scales is None:
+            self._scales = self.whole[self.codes_size :].view(torch.float32)
+        return self._scales
 
     @classmethod
     def from_codes(cls, codes: torch.Tensor, scales: torch.Tensor) -> "Int8Rows":
@@ -1235,14 +1259,10 @@ def _int8_rows(x: torch.Tensor, k: int, src: int, take, what: str, resid=None, r
     stride, step = x.stride()
     if not 1 <= k <= INT8_MAX_K or width != (2 * k if src == 2 else k) or (m > 1 and stride < width) or (m and step != 1):
         raise KernelRefused(f"{what}: rows of up to {INT8_MAX_K} values with unit stride along a row; got {tuple(x.shape)}")
-    kp, code = int8_padded_k(k), _dtype_code(x)
-    shape = (-(-m // 16), kp // 64, 4, 16, 16)
-    if take is None:
-        rows = Int8Rows(torch.empty(shape, dtype=torch.int8, device=x.device), torch.empty(m, dtype=torch.float32, device=x.device), k)
-    else:
-        rows = Int8Rows(take(shape, torch.int8), take((m,), torch.float32), k)
-    _check(_entry("ns_int8_rows", "pppipppfiiiiip")(rows.data.data_ptr(), rows.scales.data_ptr(), x.data_ptr(), max(stride, width), _address(resid), _address(resid_out), _address(weight), eps,
-                                                   m, k, kp, src, code, _stream()), what)
+    code, rows = _dtype_code(x), Int8Rows._made(m, k, x.device, take)
+    at = rows.whole.data_ptr()
+    _check(_entry("ns_int8_rows", "pppipppfiiiiip")(at, at + rows.codes_size, x.data_ptr(), max(stride, width), _address(resid), _address(resid_out), _address(weight), eps, m, k, rows.kp, src,
+                                                   code, _stream()), what)
     return rows
 
 
@@ -1344,20 +1364,28 @@ def linear_int8(x: Int8Rows, w: Int8Weight, out: torch.Tensor | None = None, dty
     (shape, dtype) gives scratch (``ctx.arena.take``)."""
     if not isinstance(x, Int8Rows) or not isinstance(w, Int8Weight):
         raise KernelRefused("linear_int8 takes rows in 8 bits (int8_rows) and an Int8Weight")
-    data, scales = x.data, x.scales
-    _gpu(data, scales, w.data, out)
-    m, n = scales.shape[0], w.n
-    if x.k != w.k or data.shape != (-(-m // 16), w.kp // 64, 4, 16, 16) or data.dtype != torch.int8 or not data.is_contiguous() or scales.dim() != 1 or scales.dtype != torch.float32 or not scales.is_contiguous():
+    n = w.n
+    if x.k != w.k:
         raise KernelRefused(f"linear_int8: rows of {x.k}, a weight of {w.k}")
+    if x.whole is not None:
+        m, codes_at = x.shape[0], x.whole.data_ptr()
+        scales_at = codes_at + x.codes_size
+        _gpu(w.data, out)
+    else:
+        data, scales = x.data, x.scales
+        _gpu(data, scales, w.data, out)
+        m, codes_at, scales_at = scales.shape[0], data.data_ptr(), scales.data_ptr()
+        if data.shape != (-(-m // 16), w.kp // 64, 4, 16, 16) or data.dtype != torch.int8 or not data.is_contiguous() or scales.dim() != 1 or scales.dtype != torch.float32 or not scales.is_contiguous():
+            raise KernelRefused(f"linear_int8: rows of {x.k} in another layout")
     if out is None:
-        out = torch.empty((m, n), dtype=dtype, device=data.device)
+        out = torch.empty((m, n), dtype=dtype, device=w.data.device)
     stride, step = out.stride() if out.dim() == 2 else (0, 0)
     if out.shape != (m, n) or (m and step != 1) or (m > 1 and stride < n):
         raise KernelRefused(f"linear_int8: out must be [{m}, {n}] with unit stride along a row")
     code = _dtype_code(out)
     to, size, at = out.data_ptr(), out.element_size(), 0
     for columns, form, ranges in int8_plan(m, n, w.k, _units_of(out)) if m else ():
-        operands = (data.data_ptr(), scales.data_ptr(), w.data.data_ptr() + at * w.kp, w.scales.data_ptr() + 4 * at, m, columns, w.kp, max(stride, n))
+        operands = (codes_at, scales_at, w.data.data_ptr() + at * w.kp, w.scales.data_ptr() + 4 * at, m, columns, w.kp, max(stride, n))
         if form < 0:
             _check(_entry("ns_gemm_int8", "pppppiiiiiip")(to + at * size, *operands, -form, code, _stream()), "linear_int8")
         else:
