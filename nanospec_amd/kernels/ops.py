@@ -1233,7 +1233,7 @@ class Int8Rows:
     @property
     def data(self) -> torch.Tensor:
         if self._data is None:
-            self._data = self.whole[: self.codes_size].view(-1, self.kp // 64, 4, 16, 16)
+            self._data = self.whole[: self.codes_size].view(-(-self.shape[0] // 16), self.kp // 64, 4, 16, 16)
         return self._data
 
     @property
@@ -1370,7 +1370,7 @@ def linear_int8(x: Int8Rows, w: Int8Weight, out: torch.Tensor | None = None, dty
     if x.whole is not None:
         m, codes_at = x.shape[0], x.whole.data_ptr()
         scales_at = codes_at + x.codes_size
-        _gpu(w.data, out)
+        _gpu(x.whole, w.data, out)
     else:
         data, scales = x.data, x.scales
         _gpu(data, scales, w.data, out)

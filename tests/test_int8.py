@@ -20,6 +20,17 @@ def test_layout(n, k):
     assert int(w.data.abs().long().sum()) == int(codes.abs().long().sum())  # zeros everywhere else
 
 
+@pytest.mark.parametrize("m,k", [(0, 64), (1, 1), (16, 700), (17, 512)])
+def test_room_for_rows(m, k):
+    for take in (None, lambda shape, dtype: torch.empty(shape, dtype=dtype)):
+        rows = ops.Int8Rows._made(m, k, torch.device("cpu"), take)
+        rows.whole.copy_(torch.arange(rows.whole.numel()) % 100)
+        assert rows.data.shape == (-(-m // 16), ops.int8_padded_k(k) // 64, 4, 16, 16) and rows.scales.shape == (m,) and rows.codes().shape == (m, k)
+        assert rows.data.numel() + 4 * m == rows.whole.numel() and rows.scales.dtype == torch.float32
+        if m:
+            assert rows.scales.data_ptr() == rows.data.data_ptr() + rows.data.numel()
+
+
 def test_from_float_keeps_rows_apart():
     w = torch.tensor([[1.0, -2.0, 0.5], [0.0, 0.0, 0.0], [float("inf"), 1.0, 0.0], [float("nan"), 1.0, 0.0], [2.0**-110, 0.0, 0.0]])
     made = ops.Int8Weight.from_float(w)
