@@ -53,6 +53,19 @@ def _gpu(*tensors) -> None:
             raise KernelRefused("kernels run on GPU tensors only; there is no CPU path")
 
 
+def _one_gpu(*tensors) -> None:
+    """``_gpu``, and all of them on the current device, on whose stream the kernel will run."""
+    here = tensors[0].get_device()
+    if here < 0:
+        return _gpu(*tensors)
+    for t in tensors:
+        if t is not None and t.get_device() != here:
+            _gpu(t)
+            raise KernelRefused(f"tensors on {tensors[0].device} and {t.device}")
+    if here != (_device_index or torch.cuda.current_device)():
+        raise KernelRefused(f"tensors on {tensors[0].device}, which is not the current device")
+
+
 def _check(code: int, what: str) -> None:
     if code != 0:
         lib = build.core()
@@ -1269,7 +1282,7 @@ def _int8_rows(x: torch.Tensor, k: int, src: int, take, what: str, resid=None, r
 def int8_rows(x: torch.Tensor, take=None) -> Int8Rows:
     """Each row of ``x`` in 8 bits: scale = largest magnitude / 127 (a row of less than 2^-100 is zeros), code = the whole number next to x * (127 / largest magnitude), in 32-bit.  A row that
     holds an infinity or no number has the scale "no number", and so have its products; other rows do not see it.  ``take`` (shape, dtype) gives the memory (``ctx.arena.take``)."""
-    _gpu(x)
+    _one_gpu(x)
     if x.dim() != 2:
         raise KernelRefused("int8_rows takes [rows, K]")
     return _int8_rows(x, x.shape[1], 0, take, "int8_rows")
@@ -1281,7 +1294,7 @@ def rmsnorm_int8(weight: torch.Tensor, eps: float, resid: torch.Tensor | None = 
     src = resid if resid is not None else x
     if src is None:
         raise KernelRefused("rmsnorm_int8 needs resid or x")
-    _gpu(weight, resid, x, resid_out)
+    _one_gpu(weight, resid, x, resid_out)
     dim = weight.numel()
     for t in (resid, x, resid_out):
         if t is not None and (t.dim() != 2 or t.shape[1] != dim or not t.is_contiguous() or t.dtype != weight.dtype or t.shape != src.shape):
@@ -1294,7 +1307,7 @@ def rmsnorm_int8(weight: torch.Tensor, eps: float, resid: torch.Tensor | None = 
 
 def silu_mul_int8(gu: torch.Tensor, take=None) -> Int8Rows:
     """``silu_mul`` into 8 bits: silu(gu[:, :I]) * gu[:, I:] for gu [rows, 2 I], in 32-bit up to the codes."""
-    _gpu(gu)
+    _one_gpu(gu)
     if gu.dim() != 2 or gu.shape[1] % 2:
         raise KernelRefused("silu_mul_int8 takes [rows, 2 I]")
     return _int8_rows(gu, gu.shape[1] // 2, 2, take, "silu_mul_int8")
@@ -1370,10 +1383,10 @@ def linear_int8(x: Int8Rows, w: Int8Weight, out: torch.Tensor | None = None, dty
     if x.whole is not None:
         m, codes_at = x.shape[0], x.whole.data_ptr()
         scales_at = codes_at + x.codes_size
-        _gpu(x.whole, w.data, out)
+        _one_gpu(x.whole, w.data, out)
     else:
         data, scales = x.data, x.scales
-        _gpu(data, scales, w.data, out)
+        _one_gpu(data, scales, w.data, out)
         m, codes_at, scales_at = scales.shape[0], data.data_ptr(), scales.data_ptr()
         if data.shape != (-(-m // 16), w.kp // 64, 4, 16, 16) or data.dtype != torch.int8 or not data.is_contiguous() or scales.dim() != 1 or scales.dtype != torch.float32 or not scales.is_contiguous():
             raise KernelRefused(f"linear_int8: rows of {x.k} in another layout")
@@ -1478,7 +1491,7 @@ def _check_kv4(pages: Kv4Pages, positions, token_req, block_table, kv_heads: int
     """What the kernels over 4-bit pages assume of a step's tokens (as for ``_check_pages``, positions and requests are the batch builder's).  -> tokens"""
     if not isinstance(pages, Kv4Pages):
         raise KernelRefused(f"{what} takes 4-bit pages (Kv4Pages)")
-    _gpu(pages.pool, positions, token_req, block_table)
+    _one_gpu(pages.pool, positions, token_req, block_table)
     if pages.kv_heads != kv_heads or pages.head_dim != head_dim:
         raise KernelRefused(f"{what}: pages of {pages.kv_heads} heads of {pages.head_dim}, asked for {kv_heads} of {head_dim}")
     _i32(positions, "positions"), _i32(token_req, "token_req")
@@ -1500,11 +1513,11 @@ def rope_kv4_write(qkv: torch.Tensor, positions: torch.Tensor, token_req: torch.
     k rotated, and k and v of every head quantised in 32-bit (``Kv4Pages``) and written into the pages ``block_table[token_req[t], position // page]``.  A key or value that holds
     an infinity or no number, or reaches further than 2^100, is kept as no number: whoever sees it gets no number.  Two tokens at one place leave either."""
     n = _check_kv4(pages, positions, token_req, block_table, kv_heads, head_dim, "rope_kv4_write")
-    _gpu(qkv, inv_freq, q_out)
+    _one_gpu(qkv, inv_freq, q_out)
     width = (heads + 2 * kv_heads) * head_dim
-    if qkv.dim() != 2 or qkv.shape != (n, width) or (n and qkv.stride(1) != 1):
+    if qkv.dim() != 2 or qkv.shape != (n, width) or (n and qkv.stride(1) != 1) or (n > 1 and qkv.stride(0) < width):
         raise KernelRefused(f"rope_kv4_write: qkv must be [{n}, {width}]")
-    if q_out is not None and (q_out.shape != (n, heads * head_dim) or q_out.dtype != qkv.dtype or (n and q_out.stride(1) != 1)):
+    if q_out is not None and (q_out.shape != (n, heads * head_dim) or q_out.dtype != qkv.dtype or (n and q_out.stride(1) != 1) or (n > 1 and q_out.stride(0) < heads * head_dim)):
         raise KernelRefused(f"rope_kv4_write: q_out must be [{n}, {heads * head_dim}] of qkv's dtype")
     if rotary_dim % 2 or not 0 <= rotary_dim <= head_dim or inv_freq.dtype != torch.float32 or not inv_freq.is_contiguous() or inv_freq.numel() < rotary_dim // 2:
         raise KernelRefused("rope_kv4_write: the rotary part is an even number of a head's channels, inv_freq holds rotary_dim/2 float32 values")
@@ -1526,7 +1539,7 @@ def kv4_read(pages: Kv4Pages, positions: torch.Tensor, token_req: torch.Tensor, 
 
 
 def _check_kv4_attn(q, out, pages: Kv4Pages, heads: int, kv_heads: int, head_dim: int, scale: float, window: int, splits: int, workspace, cols: int, what: str):
-    _gpu(q, out)
+    _one_gpu(q, out)
     if heads < 1 or kv_heads < 1 or heads % kv_heads:
         raise KernelRefused(f"{what}: {heads} heads are not a multiple of {kv_heads} key/value heads")
     if pages.kv_heads != kv_heads or pages.head_dim != head_dim:
@@ -1543,7 +1556,7 @@ def _check_kv4_attn(q, out, pages: Kv4Pages, heads: int, kv_heads: int, head_dim
     if workspace is None:
         raise KernelRefused(f"{what}: ranges of keys need a workspace")
     po, pl = workspace
-    _gpu(po, pl)
+    _one_gpu(q, po, pl)
     if po.dtype != torch.float32 or pl.dtype != torch.float32 or not po.is_contiguous() or not pl.is_contiguous() or po.numel() < cols * splits * head_dim or pl.numel() < cols * splits:
         raise KernelRefused(f"{what}: workspace too small")
     return po, pl
@@ -1564,7 +1577,7 @@ def attention_kv4(q, out, pages: Kv4Pages, tiles, block_table, heads: int, kv_he
         raise KernelRefused("attention_kv4 takes 4-bit pages (Kv4Pages)")
     if not kv4_tiles_take(head_dim):
         raise KernelRefused(f"attention_kv4 takes head sizes 64 and 128, not {head_dim} (attention_kv4_plain takes it)")
-    _gpu(pages.pool, tiles, block_table)
+    _one_gpu(pages.pool, tiles, block_table)
     _i32(tiles, "tiles")
     _kv4_table(block_table, "attention_kv4")
     if tiles.dim() != 2 or tiles.shape[1] != TILE_INTS:

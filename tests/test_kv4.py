@@ -78,7 +78,8 @@ def _call(monkeypatch, **change):
     dict(positions=torch.zeros(3, dtype=torch.int64)), dict(positions=torch.zeros(6, dtype=torch.int32)[::2]), dict(token_req=torch.zeros(2, dtype=torch.int32)),
     dict(block_table=torch.zeros((1, 2))), dict(block_table=torch.zeros(2, dtype=torch.int32)), dict(block_table=torch.zeros((2, 3), dtype=torch.int32).t()),
     dict(inv_freq=torch.ones(15)), dict(inv_freq=torch.ones(16).double()), dict(rotary_dim=31), dict(rotary_dim=34), dict(kv_heads=1), dict(head_dim=64),
-    dict(pages=torch.zeros(2, 2, 1, 320, dtype=torch.uint8)), dict(q_out=torch.zeros(3, 64)), dict(q_out=torch.zeros(3, 128).bfloat16())])
+    dict(pages=torch.zeros(2, 2, 1, 320, dtype=torch.uint8)), dict(q_out=torch.zeros(3, 64)), dict(q_out=torch.zeros(3, 128).bfloat16()),
+    dict(qkv=torch.zeros(1, 256).expand(3, 256)), dict(q_out=torch.zeros(1, 128).expand(3, 128))])
 def test_write_refuses(monkeypatch, change):
     with pytest.raises(ops.KernelRefused):
         ops.rope_kv4_write(**_call(monkeypatch, **change))
@@ -118,6 +119,19 @@ def test_attention_by_tiles_refuses(monkeypatch, change):
 def test_tensors_on_the_cpu_are_refused():
     with pytest.raises(ops.KernelRefused, match="GPU"):
         ops.kv4_read(ops.Kv4Pages.empty(1, 1, 8, 32, "cpu"), torch.zeros(1, dtype=torch.int32), torch.zeros(1, dtype=torch.int32), torch.zeros((1, 1), dtype=torch.int32))
+
+
+def test_tensors_of_another_device_are_refused(monkeypatch):
+    from types import SimpleNamespace
+
+    on = lambda index: SimpleNamespace(is_cuda=True, get_device=lambda: index, device=f"cuda:{index}")
+    monkeypatch.setattr(ops, "_device_index", lambda: 1)
+    ops._one_gpu(on(1), None, on(1))
+    for tensors in ((on(0),), (on(0), on(0)), (on(1), None, on(0)), (on(0), on(1))):
+        with pytest.raises(ops.KernelRefused, match="tensors on"):
+            ops._one_gpu(*tensors)
+    with pytest.raises(ops.KernelRefused, match="GPU"):
+        ops._one_gpu(on(1), torch.zeros(1))
 
 
 # ------------------------------------------------------------------------------------------------ which models and engines take them
