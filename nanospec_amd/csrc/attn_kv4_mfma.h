@@ -12,11 +12,16 @@
 // numbers that are meant.  The queries' channels that meet codes times 16 carry a factor of 1/16, exactly; the outputs' channels that do are multiplied by it at the end.
 //   s = step (q . u) + low sum(q):      two operations a score, as both are a key's
 //   out = sum p step u + sum p low:     p step is the weight in the second product, the rest a sum of numbers
+// Of a lane's octet the last four keys have their codes turned round, 15 - u, and their weights' signs with them:
+//   sum p step u = sum over the first four p step u - sum over the last four p step (15 - u) + sum over the last four p (15 step),   15 step added to those keys' low
+// The sums of whole numbers, all positive, would grow with the keys, and a mean of many values is many times smaller: the instruction cuts off what lies some 20 bits below its largest product, towards zero, which of
+// such sums is always the same way (-1.2e-3 of the result over 400,000 keys).  So half of the products have the other sign, and what is cut off of them cancels (under 1e-4; one instruction for eight codes and one for
+// each of four keys, 1% of a portion's time; codes less 8 everywhere, an instruction for two codes, 9 to 17%).
 // Queries are float16 on their way in, scaled by a power of two of their own so that the largest lies at 256: what is 2^-22 of it is exact.  Weights are
 // rounded to float16 (2^-12 of themselves).
 // float32 (EXACT) takes the 32-bit matrix instructions, with codes as the numbers 16 (u - 8), bytes that a mask and a sign bit make, low + 8 step in the place of low, and everything in 32 bits.  (Queries and weights as two
-// float16 values each were faster and 1e-4 of the result off at 4,000 keys: the two sums above are many times what is left of them, and the instruction cuts off what lies below its largest product, always
-// downwards; bfloat16 does not see that.)
+// float16 values each were faster and 1e-4 of the result off at 4,000 keys: with all codes positive the two sums above are many times what is left of them, and the instruction cuts off what lies below its largest
+// product.)
 //
 // The soft-max's reference R is one number a column for weights and steps together: R >= (score + log2 of its value's step) - 15 of every key so far, so
 // that p step, p = 2^(s - R), fits float16 whatever the steps' size, and is only raised when that no longer holds (then every sum shrinks).  (Key by key: by the largest score and the largest step
@@ -269,6 +274,7 @@ struct Kv4Wave {
       v_step[e] = kv4_step(vm);
       v_low[e] = kv4_low(vm);
       v_log[e] = kv4_log(vm);
+      if (!EXACT && e >= 4) v_low[e] = fmaf(15.f, v_step[e], v_low[e]);
       if constexpr (EXACT) {
         k_low[e] = fmaf(8.f, k_step[e], k_low[e]);
         v_low[e] = fmaf(8.f, v_step[e], v_low[e]);
@@ -304,7 +310,7 @@ struct Kv4Wave {
       soften(c, d, k_step, k_low, v_step, v_low, v_log, k0, mask, p32[c]);
       if constexpr (!EXACT)
 #pragma unroll
-        for (int e = 0; e < 8; ++e) p[c][e] = (_Float16)p32[c][e];
+        for (int e = 0; e < 8; ++e) p[c][e] = (_Float16)(e >= 4 ? -p32[c][e] : p32[c][e]);
       __builtin_amdgcn_sched_barrier(0);
     }
     // values as operands, four channels of each 64 a lane
@@ -327,6 +333,7 @@ struct Kv4Wave {
         }
         continue;
       }
+      w[2] = ~w[2], w[3] = ~w[3];  // 15 - u
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         uint32_t r[4];
