@@ -6,10 +6,12 @@
 // (reference: model/attention.py:22-43 for what is computed, over pages in the model's precision)
 #include "kv4.h"
 
+#define KV4_WHOLE INFINITY  // in part_l: the column's result has been written, there is nothing to join.  (No range's own: its weight is a finite number or none.)
+
 struct Kv4AttnParams {
   void* out;        // [tokens, heads, hd]
   float* part_o;    // [columns][splits][hd]: a range's result          (splits > 1)
-  float* part_l;    // [columns][splits]: log2 of its weight, -inf of an empty range
+  float* part_l;    // [columns][splits]: log2 of its weight, -inf of an empty range, KV4_WHOLE
   const void* q;    // row t at q + t * q_stride, head h at + h * hd
   const uint8_t* pool;
   const int *tiles, *token_req, *positions, *block_table;
@@ -134,12 +136,12 @@ __global__ __launch_bounds__(WAVES * NS_WAVE) void attn_kv4_join_kernel(const Kv
 #pragma unroll
     for (int s = 0; s < 8; ++s) x[i][s] = lane + 64 * i < a.hd && 8 * wave + s < a.splits ? from[(size_t)(8 * wave + s) * a.hd + lane + 64 * i] : 0.f;
   const float ls = lane < a.splits ? a.part_l[col * a.splits + lane] : -INFINITY;
-  // (results are there up to the last that counts, those in front of a token's window of weight 0; where none counts the row has been written whole)
+  if (__any(ls == INFINITY)) return;  // written whole (KV4_WHOLE)
+  // (results are there up to the last that counts, those in front of a token's window of weight 0)
   const uint64_t counts = __ballot(ls != -INFINITY);
-  if (counts == 0) return;
-  const int used = 64 - __clzll(counts);
+  const int used = counts ? 64 - __clzll(counts) : 0;
   const float top = wave_max(ls), base = top == -INFINITY ? 0.f : top;
-  const float weight = exp2f(ls - base), total = wave_sum(weight);
+  const float weight = exp2f(ls - base), total = used ? wave_sum(weight) : 1.f;  // (no key has a weight: 0, as of one range)
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const int c = lane + 64 * i;

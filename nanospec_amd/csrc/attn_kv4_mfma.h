@@ -446,7 +446,7 @@ __global__ __launch_bounds__(WAVES * 64) __attribute__((amdgpu_waves_per_eu(3)))
 #pragma unroll
       for (int e = 0; e < 4; ++e) r[e] = from_f<T>(sum[e] * by);
       *reinterpret_cast<vec_t*>((T*)a.out + ((size_t)row * a.heads + head0 + c) * HD + ch) = r;
-      if (a.splits > 1 && ch == 0) a.part_l[pc] = -INFINITY;  // (the second kernel finds nothing to join and leaves the row alone)
+      if (a.splits > 1 && ch == 0) a.part_l[pc] = KV4_WHOLE;  // (the second kernel leaves the row alone)
     } else {
       *reinterpret_cast<f32x4v*>(a.part_o + pc * HD + ch) = sum * by;
       if (ch == 0) a.part_l[pc] = every_weight == 0.f ? -INFINITY : base + __log2f(every_weight);

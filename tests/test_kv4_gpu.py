@@ -429,3 +429,39 @@ def test_ranges_that_a_window_hides(window, splits):
         want, size = oracle.attention(q.double().view(45, 4, 64), keys, values, [45], [255], table.cpu(), 16, 4, 2, 0.125, window)
         tol = tolerance(dtype, want, size, 64, 300, v_step, float(values.abs().max()))
         assert bool(((out.cpu().double().view(45, 4, 64) - want).abs() <= tol).all())
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("hd", [64, 96, 128])
+def test_scores_below_32_bits_are_written_whatever_the_ranges(hd, dtype):
+    """A token whose scores all lie below float32's range (-8 hd 10^34 10^5) has zeros, whole and in any number of ranges, among tokens that have results."""
+    ops, heads, kv_heads, page, pages = _ops(), 4, 2, 16, 60
+    gen = torch.Generator().manual_seed(hd)
+    v = torch.randn((pages, kv_heads, page, hd), generator=gen, dtype=torch.float64)
+    c, s, low = oracle.quantised(v)
+    keys = (torch.zeros(v.shape, dtype=torch.uint8), torch.zeros(v.shape[:3]).bfloat16(), torch.full(v.shape[:3], -8.0).bfloat16())
+    pool = ops.Kv4Pages.from_codes(*(t.to(DEV) for t in (*keys, c.to(torch.uint8), s[..., 0].bfloat16(), low[..., 0].bfloat16())))
+    table = torch.arange(pages, dtype=torch.int32, device=DEV)[None]
+    n, held = 3, 900
+    q = torch.zeros((n, heads * hd), dtype=dtype, device=DEV)
+    q[1] = 1e34
+    live = (s * c + low).transpose(0, 1).reshape(kv_heads, -1, hd)
+    # equal keys: the mean of the values that a token sees
+    want = torch.stack([live[:, : held - n + i + 1].mean(1).repeat_interleave(heads // kv_heads, 0) for i in range(n)])
+    pos = torch.arange(held - n, held, dtype=torch.int32, device=DEV)
+    forms = [("plain", 0)] if hd == 96 else [("plain", 0), ("rows", 4), ("rows", 8), ("tiles", 16)] + [("tiles", 32)] * (dtype == torch.bfloat16)
+    for kind, form in forms:
+        for splits in (1, 2, 9, 40):
+            tiles = [[0, 0, i, 1, held - n + i + 1, 0, 90, 0] for i in range(n)] if kind == "rows" else [[0, 0, 0, n, held, 0, 0, -1]]
+            columns = (n if kind != "tiles" else 32) * heads
+            work = tuple(torch.full((columns * splits * w,), 3.0, device=DEV) for w in (hd, 1)) if splits > 1 else None
+            out = torch.full((n, heads * hd), 7.0, dtype=dtype, device=DEV)
+            if kind == "plain":
+                ops.attention_kv4_plain(q, out, pool, torch.zeros(n, dtype=torch.int32, device=DEV), pos, table, heads, kv_heads, hd, 1e5, splits=splits, workspace=work)
+            else:
+                ops.attention_kv4(q, out, pool, torch.tensor(tiles, dtype=torch.int32, device=DEV), table, heads, kv_heads, hd, 1e5, kind == "rows", splits=splits, workspace=work,
+                                  groups=1 << 20, form=form)
+            got = out.cpu().double().view(n, heads, hd)
+            assert bool((got[1] == 0).all()), (kind, form, splits)
+            # weights of 1 and sums of 900 in 32 bits (float16's 1 is exact, its products' cuts 2^-20 of codes up to 15 times steps), then the rounding
+            assert float((got[[0, 2]] - want[[0, 2]]).abs().max()) <= 2.0**-12 + ROUND[dtype] * float(want.abs().max()), (kind, form, splits)
