@@ -23,6 +23,7 @@ struct Kv4AttnParams {
 // ------------------------------------------------------------------------------------------------------------------------------------
 // Any head size that is a multiple of 32: a workgroup a (token, head, range of keys); its four waves take blocks of 64 keys in turn, a lane
 // a key for the scores, then a lane a channel (and up to four) for the values.  All arithmetic is plain 32-bit.
+#define KV4_PLAIN_TOP 32.f  // the largest weight is 2^-32, so that sums of weights times values fit 32 bits where the values do
 template <typename T, int CH>  // CH: channels of a lane, hd <= 64 CH
 __global__ __launch_bounds__(256) void attn_kv4_plain_kernel(const Kv4AttnParams a) {
   __shared__ float qs[KV4_MAX_HD];
@@ -62,7 +63,7 @@ __global__ __launch_bounds__(256) void attn_kv4_plain_kernel(const Kv4AttnParams
     const uint32_t km = reinterpret_cast<const uint32_t*>(rec + kv4_marks_at(hd))[j], vm = reinterpret_cast<const uint32_t*>(rec + kv4_marks_at(hd))[KV4_TOKENS + j];
     const float s = seen ? (kv4_step(km) * dot + kv4_low(km) * qsum) * a.scale_log2 : -INFINITY;
     const float top = fmaxf(m, wave_max(s)), base = top == -INFINITY ? 0.f : top, shrink = exp2f(m - base);
-    const float p = exp2f(s - base), ps = seen ? p * kv4_step(vm) : 0.f;
+    const float p = exp2f(s - base - KV4_PLAIN_TOP), ps = seen ? p * kv4_step(vm) : 0.f;
     l = l * shrink + p;
     z = z * shrink + (seen ? p * fmaf(8.f, kv4_step(vm), kv4_low(vm)) : 0.f);  // (codes less 8: the two sums would be many times their own)
     m = top;
@@ -141,7 +142,8 @@ __global__ __launch_bounds__(WAVES * NS_WAVE) void attn_kv4_join_kernel(const Kv
   const uint64_t counts = __ballot(ls != -INFINITY);
   const int used = counts ? 64 - __clzll(counts) : 0;
   const float top = wave_max(ls), base = top == -INFINITY ? 0.f : top;
-  const float weight = exp2f(ls - base), total = used ? wave_sum(weight) : 1.f;  // (no key has a weight: 0, as of one range)
+  // (shares: no sum of them times the ranges' results is larger than those; no key has a weight: 0, as of one range)
+  const float part = exp2f(ls - base), weight = used ? part / wave_sum(part) : 0.f;
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const int c = lane + 64 * i;
@@ -159,7 +161,7 @@ __global__ __launch_bounds__(WAVES * NS_WAVE) void attn_kv4_join_kernel(const Kv
     if constexpr (WAVES > 1)
       sums[wave][c] = o;
     else if (c < a.hd)
-      ((T*)a.out)[(row * a.heads + head) * a.hd + c] = from_f<T>(o / total);
+      ((T*)a.out)[(row * a.heads + head) * a.hd + c] = from_f<T>(o);
   }
   if constexpr (WAVES == 1) return;
   __syncthreads();
@@ -167,7 +169,7 @@ __global__ __launch_bounds__(WAVES * NS_WAVE) void attn_kv4_join_kernel(const Kv
     float o = sums[0][c];
 #pragma unroll
     for (int v = 1; v < WAVES; ++v) o += sums[v][c];
-    ((T*)a.out)[(row * a.heads + head) * a.hd + c] = from_f<T>(o / total);
+    ((T*)a.out)[(row * a.heads + head) * a.hd + c] = from_f<T>(o);
   }
 }
 template <typename T>

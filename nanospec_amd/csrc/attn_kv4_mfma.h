@@ -26,7 +26,7 @@
 // The soft-max's reference R is one number a column for weights and steps together: R >= (score + log2 of its value's step) - 15 of every key so far, so
 // that p step, p = 2^(s - R), fits float16 whatever the steps' size, and is only raised when that no longer holds (then every sum shrinks).  (Key by key: by the largest score and the largest step
 // apart, a value of great size whose key has next to no weight would cost the others their bits; that costs a portion 5%.)
-// It knows of the keys that the column sees, and of no others.
+// It knows of the keys that the column sees, and of no others.  (kv4_log has what is taken for a step that is next to nothing, or small beside its value.)
 #pragma once
 
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
@@ -45,8 +45,10 @@ __device__ __forceinline__ f16x8 as_f16x8(uint32_t a, uint32_t b, uint32_t c, ui
 // two codes of a dword as 2^-24 u, and as 2^-20 u
 __device__ __forceinline__ uint32_t kv4_ones(uint32_t w) { return w & 0x000f000fu; }
 __device__ __forceinline__ uint32_t kv4_sixteens(uint32_t w) { return w & 0x00f000f0u; }
-// log2 of a mark's step + 127, up to 0.09 below it; at least 63 (of smaller steps is lost what float16 does not hold)
-__device__ __forceinline__ float kv4_log(uint32_t mark) { return (float)max(mark, 63u << 23) * 0x1p-23f; }
+// log2 + 127, up to 0.09 below it, of a value's step, or of what its lowest value makes of that: weights go up to 2^15 over it, and sums of them, and of them times lowest values, are to fit 32 bits.  So it counts as at
+// least 2^-64 of the lowest value (2^79 a key; what a smaller step adds is below its last bit anyway), and as at least 2^-88 (2^103 a key, for 2^24 keys; steps go down to 2^-100, whose weights of 2^-5 and more float16
+// still holds).  A lowest value that is no number counts for nothing here.
+__device__ __forceinline__ float kv4_log(float step, float low) { return (float)__float_as_uint(fmaxf(fmaxf(step, fabsf(low) * 0x1p-64f), 0x1p-88f)) * 0x1p-23f; }
 // the upper codes of a dword's bytes as signed bytes 16 (u - 8), and one of them as a number
 __device__ __forceinline__ uint32_t kv4_signed(uint32_t w) { return (w & 0xf0f0f0f0u) ^ 0x80808080u; }
 __device__ __forceinline__ float kv4_byte(uint32_t w, int y) { return (float)(int8_t)(w >> (8 * y)); }
@@ -273,7 +275,7 @@ struct Kv4Wave {
       k_low[e] = kv4_low(km);
       v_step[e] = kv4_step(vm);
       v_low[e] = kv4_low(vm);
-      v_log[e] = kv4_log(vm);
+      v_log[e] = kv4_log(v_step[e], v_low[e]);
       if (!EXACT && e >= 4) v_low[e] = fmaf(15.f, v_step[e], v_low[e]);
       if constexpr (EXACT) {
         k_low[e] = fmaf(8.f, k_step[e], k_low[e]);
@@ -431,24 +433,23 @@ __global__ __launch_bounds__(WAVES * 64) __attribute__((amdgpu_waves_per_eu(3)))
     for (int v = 0; v < WAVES; ++v) top = fmaxf(top, weights[v][c]);
     const float base = top == -INFINITY ? 0.f : top;
     f32x4v sum = {0.f, 0.f, 0.f, 0.f};
-    float every_weight = 0.f;
+    float every_weight = 0.f, x[WAVES];
 #pragma unroll
-    for (int v = 0; v < WAVES; ++v) {
-      const float x = __builtin_amdgcn_exp2f(weights[v][c] - base);
-      every_weight += x;
-      if (x != 0.f) sum += x * *reinterpret_cast<const f32x4v*>(&outs[v][c][ch]);
-    }
+    for (int v = 0; v < WAVES; ++v) x[v] = __builtin_amdgcn_exp2f(weights[v][c] - base), every_weight += x[v];
     const float by = every_weight == 0.f ? 0.f : 1.f / every_weight;
+#pragma unroll
+    for (int v = 0; v < WAVES; ++v)  // (a mean of means: no sum is larger than they are)
+      if (x[v] != 0.f) sum += (x[v] * by) * *reinterpret_cast<const f32x4v*>(&outs[v][c][ch]);
     const size_t pc = pc0 + (size_t)c * a.splits + split;
     if (whole) {
       typedef T vec_t __attribute__((ext_vector_type(4)));
       vec_t r;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) r[e] = from_f<T>(sum[e] * by);
+      for (int e = 0; e < 4; ++e) r[e] = from_f<T>(sum[e]);
       *reinterpret_cast<vec_t*>((T*)a.out + ((size_t)row * a.heads + head0 + c) * HD + ch) = r;
       if (a.splits > 1 && ch == 0) a.part_l[pc] = KV4_WHOLE;  // (the second kernel leaves the row alone)
     } else {
-      *reinterpret_cast<f32x4v*>(a.part_o + pc * HD + ch) = sum * by;
+      *reinterpret_cast<f32x4v*>(a.part_o + pc * HD + ch) = sum;
       if (ch == 0) a.part_l[pc] = every_weight == 0.f ? -INFINITY : base + __log2f(every_weight);
     }
   }

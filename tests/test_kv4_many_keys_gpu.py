@@ -100,3 +100,77 @@ def test_the_same_bits_again():
         _attend(2000, 5, 6, 2, 128, rows, splits, form, 4)
         again, _ = _attend(7001, 9 if rows else 45, 6, 2, 128, rows, splits, form, 3)
         assert torch.equal(first, again)
+
+
+def _of_values(v, dtype, hd, heads=4, kv_heads=1, tokens=20, seed=1):
+    """Every form's attention of the last ``tokens`` keys over values float64 [keys, hd], ordinary keys.  -> [(form, result)], 64 bits"""
+    import kv4_oracle as oracle
+    from nanospec_amd.kernels import ops
+
+    held, page = v.shape[0], 16
+    gen = torch.Generator().manual_seed(seed)
+    k = 0.5 * torch.randn((held, hd), generator=gen, dtype=torch.float64)
+    made, sides = [], []
+    for x in (k, v):
+        c, s, low = oracle.quantised(x.view(held // page, 1, page, hd))
+        sides.append((s * c + low).view(held, hd))
+        made += [c.to(torch.uint8).to(DEV), s[..., 0].bfloat16().to(DEV), low[..., 0].bfloat16().to(DEV)]
+    pool = ops.Kv4Pages.from_codes(*made)
+    table = torch.arange(held // page, dtype=torch.int32, device=DEV)[None]
+    q = torch.randn((tokens, heads * hd), generator=gen).to(dtype)
+    pos = torch.arange(held - tokens, held)
+    s = (q.double().view(tokens, heads, hd) @ sides[0].T * hd**-0.5).masked_fill((torch.arange(held)[None] > pos[:, None])[:, None], -math.inf)
+    want = torch.softmax(s, -1) @ sides[1]
+    got = []
+    kinds = [("plain", 0), ("rows", 4), ("rows", 8), ("tiles", 16)] + [("tiles", 32)] * (dtype == torch.bfloat16)
+    for kind, form in kinds if hd in (64, 128) else kinds[:1]:
+        for splits in (1, 3, 30):
+            columns = (tokens if kind != "tiles" else 32) * heads
+            work = tuple(torch.full((columns * splits * w,), math.nan, device=DEV) for w in (hd, 1)) if splits > 1 else None
+            out = torch.full((tokens, heads * hd), 7.0, dtype=dtype, device=DEV)
+            if kind == "plain":
+                ops.attention_kv4_plain(q.to(DEV), out, pool, torch.zeros(tokens, dtype=torch.int32, device=DEV), pos.int().to(DEV), table, heads, kv_heads, hd, hd**-0.5, splits=splits, workspace=work)
+            else:
+                tiles = [[0, 0, i, 1, held - tokens + i + 1, 0, tokens * held // 32, 0] for i in range(tokens)] if kind == "rows" else [[0, 0, 0, tokens, held, 0, 0, -1]]
+                ops.attention_kv4(q.to(DEV), out, pool, torch.tensor(tiles, dtype=torch.int32, device=DEV), table, heads, kv_heads, hd, hd**-0.5, kind == "rows", splits=splits, workspace=work,
+                                  groups=1 << 20, form=form)
+            got.append(((kind, form, splits), out.cpu().double().view(tokens, heads, hd)))
+    return got, want
+
+
+def _bound(dtype):
+    """bfloat16 as above; one key may have all the weight, and its rounding, 2^-12 at most, multiplies codes (8.8) where values are 4.6: 4.7e-4 for 4e-4.  float32: 1e-5, as over many keys."""
+    return 2.4e-3 if dtype == torch.bfloat16 else 1e-5
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("hd", [64, 96, 128])
+@pytest.mark.parametrize("size", [2.0**-99, 2.0**-70, 2.0**31, 2.0**50, 2.0**57, 2.0**90, -(2.0**100), 1.5 * 2.0**126])
+def test_values_all_alike(size, hd, dtype):
+    """Every key's value is a vector of one number (step 0), of any size that a page keeps: so is the mean."""
+    got, want = _of_values(torch.full((1024, hd), size, dtype=torch.float64), dtype, hd)
+    for form, out in got:
+        assert bool(((out / want - 1).abs() <= _bound(dtype)).all()), form
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("hd", [64, 96, 128])
+@pytest.mark.parametrize("low,high", [(-94, -94), (-80, -60), (95, 95), (-94, 94)])
+def test_values_of_any_size(low, high, hd, dtype):
+    """Values of steps from 2^-97 to 2^97, alike or mixed: the error in terms of the result is that of ordinary ones."""
+    gen = torch.Generator().manual_seed(hd)
+    v = torch.randn((1024, hd), generator=gen, dtype=torch.float64) * 2.0 ** torch.randint(low, high + 1, (1024, 1), generator=gen)
+    got, want = _of_values(v, dtype, hd)
+    for form, out in got:
+        assert float((out - want).norm() / want.norm()) <= _bound(dtype), form
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_great_lowest_values_beside_small_steps(dtype):
+    """Half of the keys' values lie about 2^40 with steps of 2^10, the others about 1."""
+    gen = torch.Generator().manual_seed(1)
+    v = torch.randn((1024, 64), generator=gen, dtype=torch.float64)
+    v[::2] = 2.0**40 + 2.0**13 * v[::2]
+    got, want = _of_values(v, dtype, 64)
+    for form, out in got:
+        assert float((out - want).norm() / want.norm()) <= _bound(dtype), form
