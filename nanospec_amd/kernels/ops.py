@@ -1425,7 +1425,8 @@ def kv4_takes(head_dim: int, page_size: int) -> bool:
 class Kv4Pages:
     """Pages of keys and values held in 4 bits.  The channels of a head's key (or value) of one token share a step and a lowest value,
     both bfloat16, rounded outwards: a code u of 0 to 15 stands for step * u + low.  ``pool`` is uint8 [pages, kv_heads, page / 8, record]: the records
-    of eight tokens of a head, 8 head_dim + 64 bytes (4.5 bits a value at head size 128, 5 at 64).  Pages of zeros stand for zeros."""
+    of eight tokens of a head, 8 head_dim + 64 bytes (4.5 bits a value at head size 128, 5 at 64).  Pages of zeros stand for zeros; places that no token has written to and nobody sees may hold anything.  Steps are finite and
+    not negative."""
 
     def __init__(self, pool: torch.Tensor, head_dim: int) -> None:
         record = 8 * head_dim + 64

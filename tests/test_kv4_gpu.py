@@ -465,3 +465,33 @@ def test_scores_below_32_bits_are_written_whatever_the_ranges(hd, dtype):
             assert bool((got[1] == 0).all()), (kind, form, splits)
             # weights of 1 and sums of 900 in 32 bits (float16's 1 is exact, its products' cuts 2^-20 of codes up to 15 times steps), then the rounding
             assert float((got[[0, 2]] - want[[0, 2]]).abs().max()) <= 2.0**-12 + ROUND[dtype] * float(want.abs().max()), (kind, form, splits)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("heads,kv_heads,hd,page", [(8, 2, 64, 8), (4, 1, 128, 32), (2, 2, 96, 16)])
+@pytest.mark.parametrize("fill", [0xFF, 0x7F, 0x80])
+def test_places_that_nobody_has_written_may_hold_anything(fill, heads, kv_heads, hd, page, dtype):
+    """A pool that was not cleared: steps and lowest values that are no numbers, infinite or below zero in all places behind a request's last key and in front of a window.  The bits are those over a pool of zeros."""
+    from nanospec_amd.parts.attention import kv4_attention
+
+    ops, layer = _ops(), _layer(hd, heads, kv_heads)
+    for lens, starts, window in (([1, 37, 1], [0, 0, 90], 0), ([1, 40], [3, 203], 50), ([1, 3], [700, 650], 0)):
+        tables, pages = oracle.scattered_tables([-(-(a + b) // page) for a, b in zip(lens, starts)], 2, 3)
+        results = []
+        for clear in (True, False):
+            pool = ops.Kv4Pages.empty(pages, kv_heads, page, hd, DEV)
+            if not clear:
+                pool.pool.fill_(fill)
+                if fill == 0x7F:  # infinite steps, lowest values of both kinds
+                    pool.pool[..., 8 * hd :] = torch.tensor([0x80, 0xFF, 0x80, 0x7F], dtype=torch.uint8, device=DEV).repeat(16)
+            for r, (m, s) in enumerate(zip(lens, starts)):  # what each has before this step, from its window on
+                first = max(0, s - window + 1) if window else 0
+                if s > first:
+                    before = (torch.arange(first, s, dtype=torch.int32, device=DEV), torch.full((s - first,), r, dtype=torch.int32, device=DEV), tables.to(DEV))
+                    ops.rope_kv4_write(_rand((s - first, (heads + 2 * kv_heads) * hd), r).to(device=DEV, dtype=dtype), *before, layer["inv"], pool, heads, kv_heads, hd, hd)
+            ctx = oracle.batch_context(lens, starts, tables, DEV)
+            qkv = _rand((sum(lens), (heads + 2 * kv_heads) * hd), 9).to(device=DEV, dtype=dtype)
+            ops.rope_kv4_write(qkv, ctx.positions, ctx.token_req, ctx.block_tables[0], layer["inv"], pool, heads, kv_heads, hd, hd)
+            out = torch.full((sum(lens), heads * hd), 7.0, dtype=dtype, device=DEV)
+            results.append(kv4_attention(ctx, qkv, out, pool, ctx.block_tables[0], heads, kv_heads, hd, hd**-0.5, window=window))
+        assert bool(torch.isfinite(results[0]).all()) and torch.equal(*results)
