@@ -443,8 +443,8 @@ __global__ __launch_bounds__(WAVES * 64) __attribute__((amdgpu_waves_per_eu(3)))
     for (int v = 0; v < WAVES; ++v) x[v] = __builtin_amdgcn_exp2f(weights[v][c] - base), every_weight += x[v];
     const float by = every_weight == 0.f ? 0.f : 1.f / every_weight;
 #pragma unroll
-    for (int v = 0; v < WAVES; ++v)  // (a mean of means: no sum is larger than they are)
-      if (x[v] != 0.f) sum += (x[v] * by) * *reinterpret_cast<const f32x4v*>(&outs[v][c][ch]);
+    for (int v = 0; v < WAVES; ++v)  // (a mean of means: no sum is larger than they are.  A wave without weight may hold no number: who sees such a value has none, however small its weight)
+      sum += (x[v] * by) * *reinterpret_cast<const f32x4v*>(&outs[v][c][ch]);
     const size_t pc = pc0 + (size_t)c * a.splits + split;
     if (whole) {
       typedef T vec_t __attribute__((ext_vector_type(4)));

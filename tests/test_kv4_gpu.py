@@ -495,3 +495,38 @@ def test_places_that_nobody_has_written_may_hold_anything(fill, heads, kv_heads,
             out = torch.full((sum(lens), heads * hd), 7.0, dtype=dtype, device=DEV)
             results.append(kv4_attention(ctx, qkv, out, pool, ctx.block_tables[0], heads, kv_heads, hd, hd**-0.5, window=window))
         assert bool(torch.isfinite(results[0]).all()) and torch.equal(*results)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("hd", [64, 96, 128])
+@pytest.mark.parametrize("what", ["key", "value"])
+def test_no_number_is_seen_however_small_its_weight(what, hd, dtype):
+    """The scores of 32 keys, all that a wave has, lie 2,000 below the others', far below any weight that 32 bits hold.  The value of one of them is no number, or its key: so is the result of whoever sees it."""
+    ops, heads, page, pages, held = _ops(), 4, 16, 8, 128
+    k = torch.zeros((pages, 1, page, hd), dtype=torch.float64)
+    v = _rand((pages, 1, page, hd), 1).double()
+    q = torch.ones((1, heads * hd), dtype=dtype, device=DEV)
+    table = torch.arange(pages, dtype=torch.int32, device=DEV)[None]
+    forms = [("plain", 0)] if hd == 96 else [("plain", 0), ("rows", 4), ("rows", 8), ("tiles", 16)] + [("tiles", 32)] * (dtype == torch.bfloat16)
+    for at in (0, 37, 94, 127):
+        bad = (at // page, 0, at % page)
+        kk, vv = k.clone(), v.clone()
+        kk[at // 32 * 2 : at // 32 * 2 + 2] = -2000.0 * hd**-0.5
+        (kk if what == "key" else vv)[bad] = math.nan
+        made = []
+        for x in (kk, vv):
+            c, s, low = oracle.quantised(x)
+            made += [c.to(torch.uint8).to(DEV), s[..., 0].bfloat16().to(DEV), low[..., 0].bfloat16().to(DEV)]
+        pool = ops.Kv4Pages.from_codes(*made)
+        for kind, form in forms:
+            for splits in (1, 2, 4):
+                columns = (1 if kind != "tiles" else 32) * heads
+                work = tuple(torch.full((columns * splits * w,), 3.0, device=DEV) for w in (hd, 1)) if splits > 1 else None
+                out = torch.full((1, heads * hd), 7.0, dtype=dtype, device=DEV)
+                if kind == "plain":
+                    ops.attention_kv4_plain(q, out, pool, torch.zeros(1, dtype=torch.int32, device=DEV), torch.tensor([held - 1], dtype=torch.int32, device=DEV), table, heads, 1, hd, hd**-0.5,
+                                            splits=splits, workspace=work)
+                else:
+                    tiles = torch.tensor([[0, 0, 0, 1, held, 0, 4 if kind == "rows" else 0, 0 if kind == "rows" else -1]], dtype=torch.int32, device=DEV)
+                    ops.attention_kv4(q, out, pool, tiles, table, heads, 1, hd, hd**-0.5, kind == "rows", splits=splits, workspace=work, groups=1 << 20, form=form)
+                assert bool(torch.isnan(out).all()), (at, kind, form, splits)
