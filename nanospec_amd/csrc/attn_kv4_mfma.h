@@ -40,6 +40,7 @@ typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 #define KV4_TOP 7.f    // log2 of the largest weight times step where the reference is raised to it, so that of small ones float16's subnormal numbers cost as little as may be ...
 #define KV4_SLACK 8.f  // ... and how far above that another may come before it is raised again: 2^15 is below float16's largest
 #define KV4_RANGE_BLOCKS 8  // of 32 keys: the fewest of a range of a single token's keys
+#define KV4_PORTION_BLOCKS 4  // ... and of a portion's (KV4_PORTION_KEYS of parts/attention.py)
 
 __device__ __forceinline__ f16x8 as_f16x8(uint32_t a, uint32_t b, uint32_t c, uint32_t d) { return __builtin_bit_cast(f16x8, u32x4{a, b, c, d}); }
 // two codes of a dword as 2^-24 u, and as 2^-20 u
@@ -460,16 +461,18 @@ __global__ __launch_bounds__(WAVES * 64) __attribute__((amdgpu_waves_per_eu(3)))
   }
 }
 
-// The results of a wave's columns, ``tokens`` tokens of a head from row ``row`` on, whole or as a range of theirs (``column``: its first token among all tiles').
+// The results of a wave's columns, ``tokens`` tokens of a head from row ``row`` on, ``whole`` or as a range of theirs (``column``: its first token among all tiles').
 template <typename T, int HD, int CT, class Wave>
-__device__ __forceinline__ void kv4_columns_out(const Wave& w, const Kv4AttnParams& a, int row, int tokens, int column, int head, int split) {
+__device__ __forceinline__ void kv4_columns_out(const Wave& w, const Kv4AttnParams& a, int row, int tokens, int column, int head, int split, bool whole) {
 #pragma unroll
   for (int c = 0; c < CT; ++c) {
     float total, low;
     const float weight = w.weight(c, total, low), inv = total == 0.f ? 0.f : 1.f / total;
     const int token = 16 * c + w.col;
     if (token >= tokens) continue;
-    if (a.splits == 1) {
+    const size_t pc = (((size_t)column + token) * a.heads + head) * a.splits + split;
+    if (whole) {
+      if (a.splits > 1 && w.t == 0) a.part_l[pc] = KV4_WHOLE;
       T* to_ = (T*)a.out + ((size_t)(row + token) * a.heads + head) * HD;
 #pragma unroll
       for (int nb = 0; nb < Wave::NB; ++nb) {
@@ -484,7 +487,6 @@ __device__ __forceinline__ void kv4_columns_out(const Wave& w, const Kv4AttnPara
         }
       }
     } else {
-      const size_t pc = (((size_t)column + token) * a.heads + head) * a.splits + split;
 #pragma unroll
       for (int nb = 0; nb < Wave::NB; ++nb)
 #pragma unroll
@@ -518,7 +520,13 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void a
   if (t0 >= n) return;
   const int tokens = min(TOKENS, n - t0), pos0 = kv - n + t0, last = pos0 + tokens - 1, shift = 31 - __clz(a.page) - 3;
   const int first = a.window ? max(0, pos0 - a.window + 1) : 0, first_of_last = a.window ? max(0, last - a.window + 1) : 0;
-  const int b0 = first / 32, blocks = last / 32 + 1 - b0, share = (blocks + a.splits - 1) / a.splits;
+  // (ranges are chosen on the host for the most keys that a portion may have, in a captured step those of its table; of fewer keys there are as many ranges as are worth joining)
+  const int b0 = first / 32, blocks = last / 32 + 1 - b0, share = a.splits == 1 ? blocks : max((blocks + a.splits - 1) / a.splits, KV4_PORTION_BLOCKS);
+  const int column = tile * KV4_TILE_TOKENS + piece * TOKENS;
+  if (split * share >= blocks) {  // nothing to do: neither queries nor keys are read, and no result is written
+    for (int i = threadIdx.x % NS_WAVE; i < tokens; i += NS_WAVE) a.part_l[(((size_t)column + i) * a.heads + head) * a.splits + split] = -INFINITY;
+    return;
+  }
   const int from = b0 + split * share, to = min(b0 + blocks, from + share);
   Wave w;
   w.init();
@@ -530,5 +538,5 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void a
     w.query(c, (const T*)a.q + (size_t)(row0 + t0 + token) * a.q_stride + head * HD, a.scale_log2, a.wide);
   }
   w.walk(from, to, 1, (first_of_last + 31) / 32, (pos0 + 1) / 32, first / 8, last / 8, a.block_table + (size_t)req * a.table_stride, a.pool, a.kv_heads, kvh, shift);
-  kv4_columns_out<T, HD, CT>(w, a, row0 + t0, tokens, (tile * KV4_TILE_TOKENS + piece * TOKENS), head, split);
+  kv4_columns_out<T, HD, CT>(w, a, row0 + t0, tokens, column, head, split, share >= blocks);
 }

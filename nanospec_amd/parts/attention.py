@@ -33,6 +33,9 @@ KV4_RANGE_KEYS = 256  # the fewest keys of a single token's: with fewer a workgr
 # The fewest keys of a range of a portion's, and the most where there are ranges at all (their lengths differ with the tiles': 666 tokens at 20,000 keys 461 in 2 ranges, 380 in 4, 363 in 6,
 # 352 in 8, 364 in 12, and 390 in 9, whose waves come to 3.1 rounds of the card; 512 at 8,000 169 in 2, 122 in 4, 133 in 6).  Ranges cost what joining their results takes: 2,048 tokens 78 in one range, 103 in two; 100 tokens at 1,000 keys 31 and, in 8, 23.
 KV4_PORTION_KEYS = 128, 2560
+# ... and the most rounds of the card that they come to, which bounds their results' memory (134 MB of heads of 128 channels) where a captured step's table, as wide as the longest request has needed, stands for its portions'
+# keys: of 4 rounds and of ranges of 2,560 keys 1,024 tokens at 100,000 2,293 and 2,465 (671 MB), 256 626 and 637, 512 at 50,000 626 and 648, 700 of 64 heads at 60,000 1,949 and 2,031
+KV4_PORTION_ROUNDS = 4
 # The keys up to which a wave takes 16 tokens of a portion (three or four waves a SIMD, which hide each other's waits and end evenly) instead of 32 (two, each key made an operand once for
 # both halves).  2,048 tokens 78 and 81 (of 64 channels 57 and 64), 100 at 1,000 keys 21 and 24; 512 at 2,000 54 and 53, 4,096 at none 238 and 218, 1,024 of 64 heads at 3,000 216 and 180, 512 at 8,000 138 and 122, 2,048 at
 # 16,000 933 and 811.
@@ -244,6 +247,16 @@ def f32_attention(ctx, q, out, cache, table, heads: int, kv_heads: int, head_dim
     return out
 
 
+def kv4_portion_ranges(tiles: int, heads: int, longest: int, wave_tokens: int, units: int) -> int:
+    """Into how many ranges the keys of portions are cut, at most (the kernel makes none of less than the fewest keys, whatever ``longest`` promised): until there are eight waves for each compute unit, if there are not
+    without, and as many as fill those rounds."""
+    waves, (least, most), full = tiles * heads * (TilePlan.TOKENS // wave_tokens), KV4_PORTION_KEYS, 8 * units
+    if waves >= full:
+        return 1
+    rounds = min(KV4_PORTION_ROUNDS, max(1, round(waves * max(-(-full // waves), -(-longest // most)) / full)))
+    return max(1, min(KV4_MAX_RANGES, rounds * full // waves, longest // least))
+
+
 def kv4_attention(ctx, q, out, pages, table, heads: int, kv_heads: int, head_dim: int, scale: float, window: int = 0) -> torch.Tensor:
     """Attention of the batch's tokens over pages of 4 bits (``ops.Kv4Pages``): head sizes 64 and 128 on the matrix cores, portions and single tokens by their tiles, others in plain
     32-bit arithmetic.  A batch without tiles has its tokens all in the latter."""
@@ -263,12 +276,7 @@ def kv4_attention(ctx, q, out, pages, table, heads: int, kv_heads: int, head_dim
     if portions.shape[0]:
         tiles, longest = portions.shape[0], min(ctx.max_chunk_kv, span + TilePlan.TOKENS)
         wave_tokens = 16 if q.dtype == torch.float32 or longest <= KV4_NARROW_KEYS else TilePlan.TOKENS
-        # ranges until there are eight waves for each compute unit, if there are not without, and as many of them as fill those rounds
-        waves, (least, most), full = tiles * heads * (TilePlan.TOKENS // wave_tokens), KV4_PORTION_KEYS, 8 * units
-        splits = 1
-        if waves < full:
-            rounds = max(1, round(waves * max(-(-full // waves), -(-longest // most)) / full))
-            splits = max(1, min(KV4_MAX_RANGES, rounds * full // waves, longest // least))
+        splits = kv4_portion_ranges(tiles, heads, longest, wave_tokens, units)
         ops.attention_kv4(q, out, pages, portions, table, heads, kv_heads, head_dim, scale, rows=False, window=window, splits=splits, form=wave_tokens,
                           workspace=workspace(tiles * TilePlan.TOKENS * heads, splits))
     if singles.shape[0]:

@@ -171,3 +171,22 @@ def test_caches_in_4_bits_refuse_what_is_not_built():
     assert storage.views[1] is storage.views[0] and storage.views[2] is None and storage.views[0].pages.pool.shape == (4, 2, 2, 8 * 64 + 64)
     with pytest.raises(ValueError, match="keeps no keys and values"):
         storage.kept(2, None, None, None)
+
+
+def test_ranges_of_portions_keep_within_their_memory():
+    """However long the keys are that a captured step's table has room for, the ranges' results come to a few rounds of the card: 4 rounds x 8 waves a unit x 32 tokens x the head's 32-bit sums."""
+    from nanospec_amd.parts import attention as att
+
+    units = 256
+    for tiles in (1, 2, 3, 17, 19, 33, 64, 100):
+        for heads in (4, 24, 32, 40, 64):
+            for longest in (2, 127, 512, 2048, 4096, 20000, 100_000, 131_072, 1 << 20):
+                for wave_tokens in (16, 32):
+                    splits = att.kv4_portion_ranges(tiles, heads, longest, wave_tokens, units)
+                    assert 1 <= splits <= 64 and (splits == 1 or longest // splits >= att.KV4_PORTION_KEYS[0])
+                    waves = tiles * heads * (32 // wave_tokens)
+                    assert splits == 1 or splits * waves <= att.KV4_PORTION_ROUNDS * 8 * units
+    # (17 and 33 tiles of 32 heads of 128 channels over 131,072 keys took 442 and 858 MiB)
+    assert all(tiles * 32 * 32 * 128 * 4 * att.kv4_portion_ranges(tiles, 32, 131_072, 32, units) <= 128 << 20 for tiles in (17, 33))
+    # as measured
+    assert [att.kv4_portion_ranges(t, 32, n, 32, units) for t, n in ((22, 20333), (16, 8512), (64, 2048))] == [8, 4, 1]

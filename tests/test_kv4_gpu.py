@@ -530,3 +530,60 @@ def test_no_number_is_seen_however_small_its_weight(what, hd, dtype):
                     tiles = torch.tensor([[0, 0, 0, 1, held, 0, 4 if kind == "rows" else 0, 0 if kind == "rows" else -1]], dtype=torch.int32, device=DEV)
                     ops.attention_kv4(q, out, pool, tiles, table, heads, 1, hd, hd**-0.5, kind == "rows", splits=splits, workspace=work, groups=1 << 20, form=form)
                 assert bool(torch.isnan(out).all()), (at, kind, form, splits)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("hd", [64, 128])
+def test_short_portions_in_a_captured_step_of_a_wide_table(hd, dtype):
+    """A captured step knows of its portions' keys only what its block tables have room for.  Of a short portion the ranges are as many as its keys are worth: the others leave nothing (but that they are empty), what is whole is
+    written at once, and the step, replayed with other lengths and work between, gives what 64 bits say."""
+    from nanospec_amd.engine.arena import Arena
+    from nanospec_amd.engine.context import BatchLayout, StepContext, fill_batch
+    from nanospec_amd.parts.attention import TILES, kv4_attention
+    import numpy as np
+
+    ops, heads, kv_heads, page, width = _ops(), 8, 2, 16, 8192
+    scale, n, reqs = hd**-0.5, 128, 3
+    layout = BatchLayout(n, reqs, 1, 1, width, plans=[(TILES, TILES.shape_captured(0, n, 2))])
+    tables = np.full((reqs, width), -1, dtype=np.int32)
+    tables[0, :200], tables[1, :200], tables[2, 0] = np.arange(200), np.arange(200, 400), 400
+    held = torch.ones(401, page, dtype=torch.bool)
+    pool, keys, values, _ = _pool(401, kv_heads, page, hd, hd, spread=0.3, held=held)
+    dev_buf = torch.zeros(layout.total, dtype=torch.int32, device=DEV)
+    host = torch.zeros(layout.total, dtype=torch.int32)
+    q, out = torch.zeros((n, heads * hd), dtype=dtype, device=DEV), torch.zeros((n, heads * hd), dtype=dtype, device=DEV)
+    context = lambda arena: StepContext(layout, dev_buf, arena, max_position=0, max_kv_len=width * page, captured=True)
+
+    def fill(lens, starts):
+        tail = n - sum(lens)
+        fill_batch(host.numpy(), layout, [0] * n, [*starts, 0], [*lens, tail], [0, 1, 2], [0], [tables], pad_tail=tail)
+        dev_buf.copy_(host)
+
+    run = lambda ctx: kv4_attention(ctx, q, out, pool, ctx.block_tables[0], heads, kv_heads, hd, scale)
+    fill([2, 2], [0, 0])
+    probe = Arena(torch.device(DEV))
+    run(context(probe))
+    torch.cuda.synchronize()
+    arena, stream = Arena(torch.device(DEV), nbytes=probe.high_water, fixed=True), torch.cuda.Stream()
+    graph = ops.Graph(stream)
+    with graph:
+        run(context(arena))
+    for lens, starts in (([2, 2], [0, 5]), ([100, 20], [0, 0]), ([64, 33], [9, 3000]), ([128 - 2, 2], [3000, 127]), ([60, 31], [450, 600])):
+        fill(lens, starts)
+        q.copy_(_rand((n, heads * hd), sum(starts)))
+        out.fill_(7.0)
+        for chunk in arena._chunks:
+            chunk.fill_(0xFF)  # no numbers
+        torch.randn(1000, device=DEV).sum().item()
+        stream.wait_stream(torch.cuda.current_stream())
+        graph.launch()
+        stream.synchronize()
+        m = sum(lens)
+        want, _ = oracle.attention(q[:m].cpu().double().view(m, heads, hd), keys, values, lens, starts, torch.from_numpy(tables), page, heads, kv_heads, scale)
+        got = out[:m].cpu().double().view(m, heads, hd)
+        # (by the norm: a bfloat16 result's rounding is 2.3e-3 at most, weights in float16 4.7e-4; 32 bits 1e-5)
+        assert float((got - want).norm() / want.norm()) <= (2.4e-3 if dtype == torch.bfloat16 else 1e-5), (lens, starts)
+        assert bool((out[m:] == 7).all())
+        # float32 results were left for the ranges that are joined alone: of portions of up to 128 keys for none
+        if max(a + b for a, b in zip(lens, starts)) <= 128:
+            assert all(bool(torch.isnan(c.view(torch.float32)[: c.numel() // 8]).all()) for c in arena._chunks)
