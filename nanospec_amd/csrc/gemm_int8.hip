@@ -259,7 +259,7 @@ static int launch_int8_few(const Int8Params& p, int blocks, hipStream_t stream) 
 // ``blocks``: row blocks of 16 of a workgroup's tile, 1, 2 or 4.
 extern "C" int ns_gemm_int8(void* out, const void* x, const float* xs, const void* w, const float* ws, int M, int N, int KP, int out_stride, int blocks, int dtype, hipStream_t stream) {
   if (M < 0 || N <= 0 || KP < 512 || KP % 256 || KP > INT8_MAX_K || out_stride < N || (blocks != 1 && blocks != 2 && blocks != 4)) return NS_ERR_BAD_ARG;
-  if ((((uintptr_t)x | (uintptr_t)w | (uintptr_t)ws) & 15) || (M + 15) / 16 > 65535) return NS_ERR_UNSUPPORTED;
+  if ((((uintptr_t)x | (uintptr_t)w | (uintptr_t)ws) & 15) || (M - 1) / (16 * blocks) >= 65535) return NS_ERR_UNSUPPORTED;  // (a grid's rows)
   if (M == 0) return NS_OK;
   const Int8Params p{out, (const int8_t*)x, (const int8_t*)w, xs, ws, M, N, KP, out_stride, 1, int8_quads(out, N, out_stride, dtype), 0};
   if (dtype == NS_DTYPE_F32) return launch_int8_few<float>(p, blocks, stream);

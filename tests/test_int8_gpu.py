@@ -232,3 +232,32 @@ def test_product_of_more_rows_than_a_grid_has_of_them(m, n, k):
     w = torch.randint(-127, 128, (n, k), generator=torch.Generator().manual_seed(2), dtype=torch.int8).to(DEV)
     y = ops.linear_int8(ops.Int8Rows.from_codes(codes, torch.ones(m, device=DEV)), ops.Int8Weight(w, torch.ones(n, device=DEV)), dtype=torch.float32)
     assert torch.equal(y, codes.float() @ w.float().T)
+
+
+@pytest.mark.parametrize("m,blocks", [(1_048_560, 1), (1_048_577, 2), (1_048_577, 4), (2_097_200, 4)])
+def test_few_columns_of_more_rows_than_16_times_a_grid(m, blocks):
+    """What the kernel for few rows takes goes by the rows of its workgroups: 65,535 times 16, 32 or 64 of them, one product by the plan's choice and one by each."""
+    ops = _ops()
+    n, k = 16, 64
+    codes = torch.randint(-127, 128, (m, k), generator=torch.Generator().manual_seed(1), dtype=torch.int8).to(DEV)
+    w = torch.randint(-127, 128, (n, k), generator=torch.Generator().manual_seed(2), dtype=torch.int8).to(DEV)
+    rows, weight = ops.Int8Rows.from_codes(codes, torch.ones(m, device=DEV)), ops.Int8Weight(w, torch.ones(n, device=DEV))
+    want = codes.float() @ w.float().T
+    assert torch.equal(ops.linear_int8(rows, weight, dtype=torch.float32), want)
+    plan, ops.int8_plan = ops.int8_plan, lambda m, n, k, units: ((n, -blocks, 1),)
+    try:
+        assert torch.equal(ops.linear_int8(rows, weight, dtype=torch.float32), want)
+    finally:
+        ops.int8_plan = plan
+
+
+def test_more_workgroups_of_rows_than_a_grid_has_are_refused():
+    ops = _ops()
+    m = 16 * 65535 + 1
+    rows, weight = ops.Int8Rows.from_codes(torch.zeros((m, 64), dtype=torch.int8, device=DEV), torch.ones(m, device=DEV)), ops.Int8Weight(torch.zeros((16, 64), dtype=torch.int8, device=DEV), torch.ones(16, device=DEV))
+    plan, ops.int8_plan = ops.int8_plan, lambda m, n, k, units: ((n, -1, 1),)
+    try:
+        with pytest.raises(ops.KernelRefused):
+            ops.linear_int8(rows, weight)
+    finally:
+        ops.int8_plan = plan
