@@ -18,7 +18,7 @@ import torch
 
 from ..kernels import ops
 from . import registry
-from .linear import Int8Linear, LinearWeight
+from .linear import Int8Linear, LinearWeight, check_inner_sizes
 from .needs import PagedNeed
 
 # How the matrix-core attention kernel is launched, from the counts of a step's batch and the size of the GPU
@@ -374,12 +374,17 @@ class Attention:
                                                    + 0.2 * torch.randn(shape, generator=gen, dtype=torch.float32, device=gen.device))
         return out
 
+    def check_products(self, products: str) -> None:
+        s = self.spec
+        if products == "int8" and s.general:
+            raise ValueError("an attention layer with options beyond a window has no products in 8-bit integers")
+        check_inner_sizes(products, "an attention layer", s.hidden, s.heads * s.v_dim)
+
     def load(self, get, dtype, device, layouts: str = "both", products: str = "model") -> None:
         s = self.spec
         plain = layouts == "both"
+        self.check_products(products)
         int8 = products == "int8"
-        if int8 and s.general:
-            raise ValueError("an attention layer with options beyond a window has no products in 8-bit integers")
         q, k, v, o = self._names
         rows = s.heads * s.head_dim + (s.kv_heads * (s.head_dim + (0 if s.value_is_key else s.v_dim)) if s.own_kv else 0)
         self.gate_at = rows  # the output gate's logits, if the layer has a gate, are the last columns of the first product

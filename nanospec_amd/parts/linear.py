@@ -33,6 +33,12 @@ LAYOUTS = ("both", "tiled")
 PRODUCTS = ("model", "int8")
 
 
+def check_inner_sizes(products: str, what: str, *inner: int) -> None:
+    """Whether products over these inner sizes run in ``products``, told from the sizes alone."""
+    if products == "int8" and max(inner) > ops.INT8_MAX_K:
+        raise ValueError(f"{what} has no products in 8-bit integers: they sum over up to {ops.INT8_MAX_K} values, not {max(inner)}")
+
+
 STREAM_ROWS = 16  # up to here the streaming kernel beats the library at the shapes measured
 GATED_WIDE_ROWS = 80  # up to here gate and up with the activation go through the 17-to-128-row kernel where the library's layout is kept too
 WIDE_HEAD_ROWS = 12  # above this many rows a wide 32-bit product (the head) is faster through the 17-to-64-row kernel

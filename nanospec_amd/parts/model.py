@@ -110,10 +110,15 @@ class DecoderModel:
         if products not in PRODUCTS:
             raise ValueError(f"products={products!r}: use one of {PRODUCTS}")
         if products == "int8":
-            for layer in self.layers:
+            for i, layer in enumerate(self.layers):
                 for part in (layer, getattr(layer, "mixer", None), getattr(layer, "ffn", None)):
                     if part is not None and not getattr(part, "takes_products", False):
-                        raise ValueError(f"products in 8-bit integers are not built for {type(part).__name__}")
+                        raise ValueError(f"products in 8-bit integers are not built for {type(part).__name__} (layer {i})")
+                    if hasattr(part, "check_products"):
+                        try:
+                            part.check_products(products)
+                        except ValueError as e:
+                            raise ValueError(f"layer {i}: {e}") from None
         full = self.wanted()
         wanted = {k: v[0] for k, v in full.items()}
         wsource.check(source, wanted, optional={spec.head_name} if spec.tie_head else frozenset(), unread_prefixes=spec.unread_prefixes)

@@ -37,7 +37,8 @@ Optional:
                                                   (which copies of a bfloat16 matrix to keep, ``parts.linear.LAYOUTS``)
   block, mixer, ffn
                takes_products = True: load(get, dtype, device, layouts, products) with products "model" | "int8"
-                                                  (what its products run in, ``parts.linear.PRODUCTS``)
+                                                  (what its products run in, ``parts.linear.PRODUCTS``);
+               check_products(products)           raises a ValueError, before anything is read, if they do not
   mixer        takes_int4_cache: bool; serve_int4_cache() is called before it is handed a cache in 4 bits
                                                   (``cache.storage.Int4View``), which its ``PagedNeed`` says it takes
 

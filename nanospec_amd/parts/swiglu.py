@@ -11,7 +11,7 @@ import torch
 
 from ..kernels import ops
 from . import registry
-from .linear import GatedWeights, Int8Gated, Int8Linear, LinearWeight
+from .linear import GatedWeights, Int8Gated, Int8Linear, LinearWeight, check_inner_sizes
 
 
 class SwiGLU:
@@ -44,15 +44,19 @@ class SwiGLU:
                         d + s.bias_suffix: ((s.hidden,), "bias")})
         return out
 
+    def check_products(self, products: str) -> None:
+        if products == "int8" and self.biased:
+            raise ValueError("a feed-forward with biases has no products in 8-bit integers")
+        check_inner_sizes(products, "a feed-forward", self.spec.hidden, self.spec.intermediate)
+
     def load(self, get, dtype, device, layouts: str = "both", products: str = "model") -> None:
         s = self.spec
         plain = layouts == "both"
         g, u, d = self._names
         to = lambda name: get(name).to(device=device, dtype=dtype)
+        self.check_products(products)
         self.reads_int8 = products == "int8"
         if self.reads_int8:
-            if self.biased:
-                raise ValueError("a feed-forward with biases has no products in 8-bit integers")
             self.gate_up, self.down = Int8Gated(to(g), to(u)), Int8Linear(to(d))
             return
         if self.biased:

@@ -120,3 +120,31 @@ def test_plans_of_more_rows_than_are_joined():
         for n, k in ((17, 32768), (64, 8192), (4096, 4096)):
             plan = ops.int8_plan(m, n, k, 256)
             assert all(ranges == 1 or m <= ops.INT8_JOIN_ROWS for _, _, ranges in plan)
+
+
+def test_models_refuse_layers_and_sizes_before_anything_is_read():
+    """Layers of the right kinds with options that have no products in 8-bit integers, and inner sizes that those do not sum over: by the layer's number, with nothing to read from."""
+    from nanospec_amd.config import LlamaConfig
+    from nanospec_amd.parts import DecoderModel
+    from tiny import TINY
+
+    cfg = TINY["A"]["cfg"]
+    fresh = lambda **change: DecoderModel(LlamaConfig.from_hf({**cfg, **change}).model_spec())
+    for change, what in ((dict(intermediate_size=32784), "layer 0: a feed-forward.*32768 values, not 32784"), (dict(hidden_size=32832), "layer 0: an attention layer.*not 32832"),
+                         (dict(num_attention_heads=2050, num_key_value_heads=2), "layer 0: an attention layer.*not 32800")):
+        with pytest.raises(ValueError, match=what):
+            fresh(**change).load(None, torch.float32, "cpu", products="int8")
+    net = fresh()
+    net.layers[1].ffn.biased = True
+    with pytest.raises(ValueError, match="layer 1: a feed-forward with biases"):
+        net.load(None, torch.float32, "cpu", products="int8")
+    import dataclasses
+
+    net = fresh()
+    net.layers[1].mixer.spec = dataclasses.replace(net.layers[1].mixer.spec, sink=True)
+    assert net.layers[1].mixer.spec.general
+    with pytest.raises(ValueError, match="layer 1: an attention layer with options"):
+        net.load(None, torch.float32, "cpu", products="int8")
+    # what these sizes are refused for is the products alone
+    with pytest.raises(AttributeError):
+        fresh(intermediate_size=32784).load(None, torch.float32, "cpu")
