@@ -37,6 +37,7 @@ class PagedView:
 class Int4View:
     group: int
     pages: Kv4Pages
+    products: dict  # of all of the storage's entries: mixer -> the product that it runs over this cache (others run their own)
 
 
 @dataclass
@@ -88,25 +89,34 @@ class CacheStorage:
         if kv_format not in KV_FORMATS:
             raise ValueError(f"kv_format={kv_format!r}: use one of {KV_FORMATS}")
         self.kv_format = kv_format
+        self.products: dict = {}
         if kv_format == "int4":
             check_int4(model, page_size)
-            model.serve_int4_cache()
-        # what a model keeps only to be faster makes room: where the pages do not fit beside it, or leave little for the steps
+        # what a model keeps only to be faster makes room, and what its layers would have for a cache in 4 bits: where the pages do not fit beside it, or leave little for the steps
         give_back = getattr(model, "give_back_second_copies", lambda: False)
         short = False
         try:
+            if kv_format == "int4":
+                self.products = model.serve_int4_cache() or {}
             self._allocate(model, num_pages, page_size, num_slots, dtype, device)
         except torch.OutOfMemoryError:
             short = True
         if short:  # (behind the handler, whose traceback holds what had been allocated)
+            products = self.products
             self.__dict__.clear()
-            self.kv_format = kv_format
+            self.kv_format, self.products = kv_format, products
+            self._one_order(model)
             give_back()
             self._allocate(model, num_pages, page_size, num_slots, dtype, device)
-        elif dtype == torch.float32 and torch.device(device).type == "cuda":  # (no other models have such copies)
+        elif (dtype == torch.float32 or self.products) and torch.device(device).type == "cuda":  # (no other models have such copies)
             free, total = torch.cuda.mem_get_info(device)
             if free + torch.cuda.memory_reserved(device) - torch.cuda.memory_allocated(device) < STEPS_SHARE * total:
+                self._one_order(model)
                 give_back()
+
+    def _one_order(self, model) -> None:
+        if self.kv_format == "int4" and getattr(model, "stream_one_order", lambda products: False)(self.products):
+            self.products.clear()  # (the views' too: the layers' own products are those)
 
     def _allocate(self, model, num_pages: list[int], page_size: int, num_slots: int, dtype, device) -> None:
         self.group_specs, needs, of_entry = plan_groups(model.cache_needs)
@@ -129,7 +139,7 @@ class CacheStorage:
                 return tuple(view_of(single) for single in need)
             if isinstance(need, PagedNeed):
                 g = needs.index(need)
-                view = Int4View(g, Kv4Pages(self.int4[g][taken[g]], need.head_dim)) if int4 else PagedView(g, self.k[g][taken[g]], self.v[g][taken[g]])
+                view = Int4View(g, Kv4Pages(self.int4[g][taken[g]], need.head_dim), self.products) if int4 else PagedView(g, self.k[g][taken[g]], self.v[g][taken[g]])
                 taken[g] += 1
                 return view
             if isinstance(need, StateNeed):

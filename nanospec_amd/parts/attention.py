@@ -10,6 +10,7 @@ all heads of a group with the keys cut into ranges that are joined afterwards.
 
 from __future__ import annotations
 
+import weakref
 from array import array
 from dataclasses import dataclass
 
@@ -310,6 +311,7 @@ class Attention:
         self.wo: LinearWeight | None = None
         self.qkv_bias = self.q_norm = self.k_norm = self.v_mix = None
         self.out_bias: torch.Tensor | None = None  # the output projection's bias; a block may add it itself (add_out_bias=False)
+        self._int4_product: weakref.ref | None = None  # see serve_int4_cache
         if spec.value_mix not in ("", "source", "mix"):
             raise ValueError(f"value_mix={spec.value_mix!r}: use '', 'source' or 'mix'")
         if (spec.bias or spec.whole_norm_eps is not None or spec.value_mix) and not spec.own_kv:
@@ -427,7 +429,7 @@ class Attention:
         self.reads_int8 = int8
         if int8:
             self.wqkv_rope = None
-            self.wqkv = self.wqkv_int4 = Int8Linear(wqkv)
+            self.wqkv = Int8Linear(wqkv)
             self.wo = Int8Linear(get(o).to(device=device, dtype=dtype))
             return
         # for few rows the stacked matrix is streamed by a kernel that rotates and writes the cache in its epilogue; it
@@ -439,17 +441,28 @@ class Attention:
         # (without the plain layout the stacked matrix is also kept tiled in its own row order, for more than 16 rows)
         self.wqkv = LinearWeight(wqkv, keep_plain=plain, tiled=self.wqkv_rope is None or not plain)
         self.wo = LinearWeight(get(o).to(device=device, dtype=dtype).contiguous(), keep_plain=plain)
-        self.wqkv_int4 = None
 
     @property
     def takes_int4_cache(self) -> bool:
         return not self.spec.general and self.spec.head_dim % 32 == 0
 
-    def serve_int4_cache(self) -> None:
-        """A stacked product that leaves q, k and v as they are: with 4-bit pages the rotation and the write are a kernel of their own, also for few rows.  (The copy that the kernel with
-        both in its epilogue streams has its rows in that kernel's order.)"""
-        if self.takes_int4_cache and self.wqkv_int4 is None:
-            self.wqkv_int4 = self.wqkv if self.wqkv_rope is None or self.wqkv.plain is None else LinearWeight(self.wqkv.plain)
+    def serve_int4_cache(self) -> "LinearWeight | None":
+        """A stacked product that leaves q, k and v as they are and streams its matrix for few rows: with 4-bit pages the rotation and the write are a kernel of their own, also there.  None where ``wqkv`` is that; beside a
+        copy for the kernel with both in its epilogue, whose rows lie in that kernel's order, one in the matrix' own order is made.  It belongs to the caches that are made for this layer: they share it, and it goes with the
+        last of them."""
+        if not self.takes_int4_cache or self.wqkv_rope is None or self.wqkv.plain is None:
+            return None
+        product = self._int4_product() if self._int4_product is not None else None
+        if product is None:
+            product = LinearWeight(self.wqkv.plain)
+            self._int4_product = weakref.ref(product)
+        return product
+
+    def stream_one_order(self, product: "LinearWeight | None" = None) -> None:
+        """Where there is no room for two copies of the stacked matrix for few rows: the one in its own order alone (``product``, which ``serve_int4_cache`` gave, or a new one) in the place of the other, for every cache."""
+        if self.takes_int4_cache and self.wqkv_rope is not None and self.wqkv.plain is not None:
+            self.wqkv_rope = None
+            self.wqkv = product if product is not None else LinearWeight(self.wqkv.plain)
 
     def cache_need(self):
         s = self.spec
@@ -486,7 +499,7 @@ class Attention:
                 raise ops.KernelRefused("this layer does not read keys and values in 4 bits")
             return self._forward_general(ctx, x, cache, owns_cache, out, residual, qkv, table, add_out_bias)
         if int4 is not None:
-            self.wqkv_int4(x, out=qkv, arena=ctx.arena, plain_copy=not ctx.captured)
+            cache.products.get(self, self.wqkv)(x, out=qkv, arena=ctx.arena, plain_copy=not ctx.captured)
             ops.rope_kv4_write(qkv, ctx.positions, ctx.token_req, table, pos.inv_freq, int4, s.heads, s.kv_heads, s.head_dim, pos.rotary_dim,
                                write_kv=owns_cache, **self._form)
         elif self.wqkv_rope is not None and n <= 16 and ops.tiled_takes(x.x if isinstance(x, ops.PreNormed) else x, s.hidden):

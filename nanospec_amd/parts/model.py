@@ -165,14 +165,30 @@ class DecoderModel:
         torch.cuda.synchronize(self.device)
         return self
 
-    def serve_int4_cache(self) -> None:
-        """The layers are about to be handed keys and values in 4 bits (``cache.storage``)."""
+    def serve_int4_cache(self) -> dict:
+        """The layers are about to be handed keys and values in 4 bits (``cache.storage``).  -> mixer -> what it runs its first product with for such a cache, which is whoever's that hands it to them."""
+        products = {}
         for layer in self.layers:
             for part in getattr(layer, "parts", ()):
                 for one in (part, *getattr(part, "sides", ())):
-                    if hasattr(one, "serve_int4_cache"):
-                        one.serve_int4_cache()
+                    product = one.serve_int4_cache() if hasattr(one, "serve_int4_cache") else None
+                    if product is not None:
+                        products[one] = product
         torch.cuda.synchronize(self.device)
+        return products
+
+    def stream_one_order(self, products: dict) -> bool:
+        """For whoever has no room for what ``serve_int4_cache`` gives: the layers have one copy of their first matrix for few rows, which serves every cache.  Not once a runner has been made for the model: a step under way or
+        captured may read the other."""
+        mixers = [] if self.has_runner else [one for layer in self.layers for part in getattr(layer, "parts", ()) for one in (part, *getattr(part, "sides", ())) if getattr(one, "wqkv_rope", None) is not None]
+        if mixers:
+            torch.cuda.synchronize(self.device)
+            for one in mixers:
+                one.stream_one_order(products.pop(one, None))
+            torch.cuda.empty_cache()
+            print("[nanospec_amd] the layers' first matrices are kept for few rows in one order, to leave room for a cache in 4 bits; over a cache in the model's precision steps of a few requests are slower",
+                  file=sys.stderr, flush=True)
+        return bool(mixers)
 
     def give_back_second_copies(self) -> bool:
         """For whoever needs the memory (``cache.storage``): the second copies of float32 matrices, which only make products of many rows faster, are given back.  Not once a runner has been made for

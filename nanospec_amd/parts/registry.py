@@ -40,7 +40,8 @@ Optional:
                                                   (what its products run in, ``parts.linear.PRODUCTS``);
                check_products(products)           raises a ValueError, before anything is read, if they do not
   mixer        takes_int4_cache: bool; serve_int4_cache() is called before it is handed a cache in 4 bits
-                                                  (``cache.storage.Int4View``), which its ``PagedNeed`` says it takes
+                                                  (``cache.storage.Int4View``), which its ``PagedNeed`` says it takes; what it
+                                                  returns lives as long as that cache (``Int4View.products[mixer]``)
 
 Optional, for parts whose products can do the work of the RMS norms around them (``parts.linear.IntoResidual``):
   norm         links_products = True, weight, spec.eps

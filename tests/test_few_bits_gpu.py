@@ -300,3 +300,78 @@ def test_what_a_cache_in_4_bits_takes(folders):
     for storage in (few, full):
         k, v = storage.kept(1, t, torch.zeros_like(t), table)
         assert k.shape == v.shape == (40, 2, 64) and not k.any() and not v.any()  # pages of zeros stand for zeros
+
+
+def _wide(tmp_path_factory):
+    """A folder whose q/k/v matrices are large enough to be counted: 4 layers of 1,536 x 1,024, 3 MiB each in bfloat16."""
+    from nanospec_amd.config import LlamaConfig
+    from nanospec_amd.weights import write_model_folder
+
+    cfg = dict(BASE, num_hidden_layers=4, vocab_size=300, hidden_size=1024, intermediate_size=512, num_attention_heads=16, num_key_value_heads=4, head_dim=64)
+    return write_model_folder(tmp_path_factory.mktemp("wide"), LlamaConfig.from_hf(cfg), 3, torch.float32)
+
+
+def _allocated():
+    import gc
+
+    gc.collect()
+    torch.cuda.synchronize()
+    return torch.cuda.memory_allocated()
+
+
+def test_a_cache_in_4_bits_leaves_a_model_as_it_was(tmp_path_factory):
+    """The copies of the q/k/v matrices that layers run over such a cache belong to it: two caches share them, and the last one takes them along."""
+    from nanospec_amd import load_model
+    from nanospec_amd.cache.storage import CacheStorage
+
+    model = load_model(_wide(tmp_path_factory), layouts="both")
+    before, copies = _allocated(), 4 * 1536 * 1024 * 2
+    make = lambda: CacheStorage(model, [8], 16, 4, torch.bfloat16, "cuda", "int4")
+    one = make()
+    pages = sum(t.numel() for t in one.int4)
+    first = _allocated()
+    assert len(one.products) == 4 and copies <= first - before - pages < 1.5 * copies
+    two = make()
+    assert _allocated() - first < pages + copies / 8 and all(two.products[k] is v for k, v in one.products.items())
+    del one
+    assert all(p is not None for p in two.products.values()) and _allocated() - before >= copies
+    del two
+    assert _allocated() - before < copies / 8
+
+
+@pytest.mark.parametrize("fails", ["pages", "copies"])
+def test_a_cache_in_4_bits_where_memory_is_short(tmp_path_factory, monkeypatch, fails, capsys):
+    """No room beside two copies of the q/k/v matrices: the layers keep one, and serve either cache with it."""
+    from nanospec_amd import load_model
+    from nanospec_amd.cache.storage import CacheStorage
+    from nanospec_amd.engine.replay import Replayer
+    from nanospec_amd.parts.attention import Attention
+
+    folder = _wide(tmp_path_factory)
+    model, other = load_model(folder, layouts="both"), load_model(folder, layouts="both")
+    before = _allocated()
+    owner, name = (CacheStorage, "_allocate") if fails == "pages" else (Attention, "serve_int4_cache")
+    plain, calls = getattr(owner, name), []
+
+    def short(self, *args, **kw):
+        calls.append(self)
+        if len(calls) == (1 if fails == "pages" else 3):
+            raise torch.OutOfMemoryError("no room")
+        return plain(self, *args, **kw)
+
+    monkeypatch.setattr(owner, name, short)
+    rep = Replayer(model, 512, 16, True, kv_format="int4")
+    monkeypatch.undo()
+    assert not rep.storage.products and all(layer.mixer.wqkv_rope is None and layer.mixer.wqkv.tiled is not None for layer in model.layers)
+    assert "in one order" in capsys.readouterr().err
+    steps = [[{"id": "a", "tokens": random_tokens(n, 300, n + i), "want": [n - 1]}] for i, n in enumerate((40, 1, 1, 200, 1))]
+    for kv_format, made in (("int4", rep), ("model", Replayer(model, 512, 16, True))):
+        whole = Replayer(other, 512, 16, True, kv_format=kv_format)
+        assert kv_format == "model" or len(whole.storage.products) == 4
+        for step in steps:
+            a, b = made.step(step, []), whole.step(step, [])
+            # other kernels' roundings of q, k and v; a value between two codes may go the other way (0.03, as for captured steps; in bfloat16 8 units of the row's largest besides)
+            assert float((a - b).abs().max() / b.abs().max()) <= 0.03 + LOGITS[torch.bfloat16]
+    del rep, whole, made, a, b
+    model.has_runner = True
+    assert not model.stream_one_order({})
