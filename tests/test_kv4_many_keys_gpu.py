@@ -17,7 +17,7 @@ DEV = "cuda:0"
 NORM = 2.4e-3
 
 
-def _attend(keys, tokens, heads, kv_heads, hd, rows, splits, form, seed, window=0):
+def _attend(keys, tokens, heads, kv_heads, hd, rows, splits, form, seed, window=0, groups=512, used=None):
     """``tokens`` tokens at the end of ``keys`` keys (``rows``: each at its own end).  -> result and 64 bits, [tokens, heads, hd] on the GPU"""
     from nanospec_amd.kernels import ops
 
@@ -46,7 +46,9 @@ def _attend(keys, tokens, heads, kv_heads, hd, rows, splits, form, seed, window=
     work = tuple(torch.full((columns * splits * w,), math.nan, device=DEV) for w in (hd, 1)) if splits > 1 else None
     out = torch.full((tokens, heads * hd), 7.0, dtype=torch.bfloat16, device=DEV)
     scale = hd**-0.5
-    ops.attention_kv4(q, out, pool, tiles, table, heads, kv_heads, hd, scale, rows, window=window, splits=splits, workspace=work, groups=512, form=form)
+    ops.attention_kv4(q, out, pool, tiles, table, heads, kv_heads, hd, scale, rows, window=window, splits=splits, workspace=work, groups=groups, form=form)
+    if used is not None:
+        used.append((work[1].view(columns, splits)[:heads] > -math.inf).sum(1))  # ranges of the first token's columns
     want = torch.empty((tokens, heads, hd), dtype=torch.float64, device=DEV)
     key = torch.arange(keys, device=DEV)
     hidden = key[None] > pos[:, None]
@@ -174,3 +176,16 @@ def test_great_lowest_values_beside_small_steps(dtype):
     got, want = _of_values(v, dtype, 64)
     for form, out in got:
         assert float((out - want).norm() / want.norm()) <= _bound(dtype), form
+
+
+@pytest.mark.parametrize("splits", [2, 8, 9, 33, 64])
+@pytest.mark.parametrize("rows,tokens,heads,kv_heads,hd", [(True, 3, 4, 2, 64), (True, 140, 32, 8, 64), (True, 2, 8, 1, 128), (False, 40, 4, 2, 128), (False, 140, 32, 8, 64)])
+def test_every_range_counts(rows, tokens, heads, kv_heads, hd, splits):
+    """Few columns and many (a wave and four that join them), as many ranges as asked for: 64 of 256 keys are 16,384.  A range that is left out, or has another's weight, changes the result by the root of its share, 12% of 64."""
+    used = []
+    got, want = _attend(20_000, tokens, heads, kv_heads, hd, rows, splits, 4 if rows else 16, splits, groups=1 << 24, used=used)
+    # (a range has share = blocks / splits + 1 of 625 blocks: of single tokens 64 make 10 each, 63 ranges)
+    blocks = 20_000 // 32
+    share = blocks // splits + 1 if rows else -(-blocks // splits)
+    assert bool((used[0] == -(-blocks // share)).all()) and -(-blocks // share) >= splits - 1
+    assert _off(got, want) <= NORM
