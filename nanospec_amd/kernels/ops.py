@@ -1512,7 +1512,8 @@ def rope_kv4_write(qkv: torch.Tensor, positions: torch.Tensor, token_req: torch.
                    q_out: torch.Tensor | None = None) -> None:
     """``rope_kv_write`` for pages of 4 bits: q rotated inside ``qkv`` [N, (heads + 2 kv_heads) * head_dim], or into ``q_out`` [N, heads * head_dim], which leaves ``qkv`` as it is;
     k rotated, and k and v of every head quantised in 32-bit (``Kv4Pages``) and written into the pages ``block_table[token_req[t], position // page]``.  A key or value that holds
-    an infinity or no number, or reaches further than 2^100, is kept as no number: whoever sees it gets no number.  Two tokens at one place leave either."""
+    an infinity or no number, or reaches further than 2^100, is kept as no number: whoever sees it gets no number.  Two tokens at one place leave a mixture of
+    both there (the padding of a captured step, in a page that nobody reads)."""
     n = _check_kv4(pages, positions, token_req, block_table, kv_heads, head_dim, "rope_kv4_write")
     _one_gpu(qkv, inv_freq, q_out)
     width = (heads + 2 * kv_heads) * head_dim
@@ -1571,7 +1572,8 @@ def kv4_tiles_take(head_dim: int) -> bool:
 def attention_kv4(q, out, pages: Kv4Pages, tiles, block_table, heads: int, kv_heads: int, head_dim: int, scale: float, rows: bool, window: int = 0, splits: int = 1,
                   workspace: tuple[torch.Tensor, torch.Tensor] | None = None, groups: int = 1, form: int = 0) -> torch.Tensor:
     """Attention over 4-bit pages on the matrix cores, head sizes 64 and 128, bfloat16 and float32, of the tokens that ``tiles`` (int32 [n_tiles, 8], as for ``attention_mfma``) describe:
-    with ``rows`` single tokens, a tile each, otherwise portions in tiles of up to 32 tokens.  Tokens that no tile describes are left as they are.  A token all of whose scores lie below float32's range has zeros.  ``splits`` > 1 cuts the keys of every tile into
+    with ``rows`` single tokens, a tile each, otherwise portions in tiles of up to 32 tokens.  Tokens that no tile describes are left as they are.  A token all of whose scores lie below float32's range has zeros; above it (and
+    of bfloat16 queries beyond 2^110) it has no number.  ``splits`` > 1 cuts the keys of every tile into
     that many ranges and needs ``workspace`` = float32 tensors of columns * splits * head_dim and columns * splits values, columns = tiles * (1 or 32) * heads.  Single tokens
     use as many of their ranges as make about ``groups`` workgroups of all tokens' keys.  ``form``: the waves of a workgroup for single tokens (4 or 8), the tokens of a portion's tile that a wave takes (16 or, of bfloat16, 32)."""
     if not isinstance(pages, Kv4Pages):

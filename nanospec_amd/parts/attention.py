@@ -260,14 +260,14 @@ def kv4_portion_ranges(tiles: int, heads: int, longest: int, wave_tokens: int, u
 
 def kv4_attention(ctx, q, out, pages, table, heads: int, kv_heads: int, head_dim: int, scale: float, window: int = 0) -> torch.Tensor:
     """Attention of the batch's tokens over pages of 4 bits (``ops.Kv4Pages``): head sizes 64 and 128 on the matrix cores, portions and single tokens by their tiles, others in plain
-    32-bit arithmetic.  A batch without tiles has its tokens all in the latter."""
+    32-bit arithmetic."""
     take, units, group = ctx.arena.take, ops._units_of(q), heads // kv_heads
     span = window or 1 << 30
 
     def workspace(columns: int, splits: int):
         return (take((columns * splits * head_dim,), torch.float32), take((columns * splits,), torch.float32)) if splits > 1 else None
 
-    if not ops.kv4_tiles_take(head_dim) or TilePlan.key not in ctx.plans:
+    if not ops.kv4_tiles_take(head_dim):
         # a workgroup a token, head and range of keys, until there are four for each compute unit
         n, longest = q.shape[0], min(ctx.max_kv_len, span)
         splits = max(1, min(KV4_MAX_RANGES, 4 * units // max(1, n * heads), -(-longest // KV4_RANGE_KEYS)))
