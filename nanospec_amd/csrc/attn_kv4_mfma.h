@@ -341,14 +341,13 @@ struct Kv4Wave {
         }
         continue;
       }
-      w[2] = ~w[2], w[3] = ~w[3];  // 15 - u
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         uint32_t r[4];
 #pragma unroll
         for (int x = 0; x < 4; ++x) {
           const uint32_t y = i >= 2 ? w[x] >> 8 : w[x];
-          r[x] = i & 1 ? kv4_sixteens(y) : kv4_ones(y);
+          r[x] = i & 1 ? kv4_sixteens(x < 2 ? y : ~y) : kv4_ones(x < 2 ? y : ~y);  // the last four keys' as 15 - u
         }
         const f16x8 va = as_f16x8(r[0], r[1], r[2], r[3]);
 #pragma unroll
