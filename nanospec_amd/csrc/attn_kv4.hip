@@ -174,7 +174,7 @@ __global__ __launch_bounds__(WAVES * NS_WAVE) void attn_kv4_join_kernel(const Kv
 }
 template <typename T>
 static void launch_join(const Kv4AttnParams& a, unsigned columns, int tile_tokens, hipStream_t stream) {
-  // (many columns fill the card with a wave each: 21,000 of 9 ranges 24 us, with four 47)
+  // (many columns fill the card with a wave each: 22,500 of 11 ranges 18 us; as first measured, 21,000 of 9, 24, with four 47)
   if (a.splits <= 8 || columns > 4096)
     attn_kv4_join_kernel<T, 1><<<columns, NS_WAVE, 0, stream>>>(a, tile_tokens);
   else

@@ -384,8 +384,8 @@ struct Kv4Wave {
 
 // Single tokens: a workgroup a (token, key/value head, 16 query heads of its group, range of keys), whose waves take blocks of 32 keys in turn and meet in LDS.  Ranges are even and as many
 // as give ``a.groups`` workgroups over all tokens: a row twice as long as others has twice as many.
-// Bound by memory where the rows are long and many (61 rows of 200 to 12,000 keys, 8 key/value heads of 128 channels: 94 us, 4.2 TB/s; 64 rows of 6,000: 5.3), by one workgroup's
-// chain of loads where they are few (a row of 1,000, in eight waves: 9.3 us).  Two blocks on their way at a time were slower everywhere (their registers cost a wave a SIMD).
+// Bound by memory where the rows are long and many (61 rows of 200 to 12,000 keys, 8 key/value heads of 128 channels: 96 us, 4.2 TB/s; 64 rows of 6,000: 90 us, 4.65), by one workgroup's
+// chain of loads where they are few (a row of 1,000, in eight waves: 8.9 us).  Two blocks on their way at a time were slower everywhere (their registers cost a wave a SIMD).
 template <typename T, int HD, bool EXACT, int WAVES>
 __global__ __launch_bounds__(WAVES * 64) __attribute__((amdgpu_waves_per_eu(3))) void attn_kv4_rows_kernel(const Kv4AttnParams a) {
   typedef Kv4Wave<T, HD, 1, EXACT> Wave;
@@ -501,8 +501,8 @@ __device__ __forceinline__ void kv4_columns_out(const Wave& w, const Kv4AttnPara
 }
 
 // Portions: a wave 16 CT tokens of a head, four waves a workgroup that share nothing but their place.
-// Bound by vector instructions: a block of 32 keys and 32 columns of 128 channels has 32 matrix instructions (512 cycles) and about 320 others (1,430), of which 112 make operands of the
-// codes and 16 are exponentials; they are under way 73% of the time.  2,048 tokens at 16,000 keys: 809 us, 706 TFLOP/s; 2,048 at none 73 us.  Four tiles of columns a wave (each operand made
+// Bound by vector instructions: a block of 32 keys and 32 columns of 128 channels has 32 matrix instructions (512 cycles) and 355 others (counted; 1,610 cycles), of which 80 make operands of the
+// codes and 16 are exponentials; they are under way 84% of the time.  2,048 tokens at 16,000 keys: 811 us, 704 TFLOP/s; 2,048 at none, 16 columns a wave, 72 us.  Four tiles of columns a wave (each operand made
 // for twice as many) leave one wave a SIMD and nothing to fill its waits: 1,203 and 149 us.  Operands made by four waves for each other, by way of LDS, with a barrier a block: 828 and 90, where these took 772 and 75.
 template <typename T, int HD, int CT, bool EXACT>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void attn_kv4_tiles_kernel(const Kv4AttnParams a) {

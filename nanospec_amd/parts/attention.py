@@ -31,22 +31,22 @@ F32_RANGE_KEYS = 128  # keys of a range of a single token's row in 32-bit: two t
 # Attention over keys and values in 4 bits (us, 32 heads on 8 of 128 channels unless said otherwise)
 KV4_MAX_RANGES = 64  # of a row's keys
 KV4_RANGE_KEYS = 256  # the fewest keys of a single token's: with fewer a workgroup's beginning and end are longer than its blocks
-# The fewest keys of a range of a portion's, and the most where there are ranges at all (their lengths differ with the tiles': 666 tokens at 20,000 keys 461 in 2 ranges, 380 in 4, 363 in 6,
-# 352 in 8, 364 in 12, and 390 in 9, whose waves come to 3.1 rounds of the card; 512 at 8,000 169 in 2, 122 in 4, 133 in 6).  Ranges cost what joining their results takes: 2,048 tokens 78 in one range, 103 in two; 100 tokens at 1,000 keys 31 and, in 8, 23.
+# The fewest keys of a range of a portion's, and the most where there are ranges at all (their lengths differ with the tiles': 666 tokens at 20,000 keys 493 in 2 ranges, 402 in 4, 344 in 6, 355 in 9,
+# 365 in 12, and 388 in 8, whose waves come to 2.6 rounds of the card; 512 at 8,000 166 in 2, 123 in 4, 133 in 6).  Ranges cost what joining their results takes: 2,048 tokens 73 in one range, 110 in two; 100 tokens at 1,000 keys 32 and, in 8, 22.
 KV4_PORTION_KEYS = 128, 2560
 # ... and the most rounds of the card that they come to, which bounds their results' memory (134 MB of heads of 128 channels) where a captured step's table, as wide as the longest request has needed, stands for its portions'
 # keys: of 4 rounds and of ranges of 2,560 keys 1,024 tokens at 100,000 2,293 and 2,465 (671 MB), 256 626 and 637, 512 at 50,000 626 and 648, 700 of 64 heads at 60,000 1,949 and 2,031
 KV4_PORTION_ROUNDS = 4
 # The keys up to which a wave takes 16 tokens of a portion (three or four waves a SIMD, which hide each other's waits and end evenly) instead of 32 (two, each key made an operand once for
-# both halves).  2,048 tokens 78 and 81 (of 64 channels 57 and 64), 100 at 1,000 keys 21 and 24; 512 at 2,000 54 and 53, 4,096 at none 238 and 218, 1,024 of 64 heads at 3,000 216 and 180, 512 at 8,000 138 and 122, 2,048 at
-# 16,000 933 and 811.
+# both halves).  2,048 tokens 73 and 79 (of 64 channels 58 and 65), 100 at 1,000 keys 22 and 24; 512 at 2,000 66 and 56, 4,096 at none 249 and 220, 1,024 of 64 heads at 3,000 226 and 179, 512 at 8,000 151 and 123, 2,048 at
+# 16,000 1,054 and 811.
 KV4_NARROW_KEYS = 2048
-# Workgroups of four waves that single tokens' keys are cut for, for each compute unit.  Of 1, 2, 3 and 4: 8 rows of 4,000 keys 18.2, 17.6, 20.6, 21.4; 61 of 200 to 12,000 89, 93, 95, 90;
-# 2 of 100,000 (64 heads) 64, 62, 67, 70; one of 32,000 20, 24, 24, 24; 64 of 6,000 (64 channels) 67, 62, 62, 65.
+# Workgroups of four waves that single tokens' keys are cut for, for each compute unit.  Of 1, 2, 3 and 4: 8 rows of 4,000 keys 18.6, 16.8, 18.3, 18.5; 61 of 200 to 12,000 98, 103, 100, 94;
+# 2 of 100,000 (64 heads) 64, 49, 53, 54; one of 32,000 16.2, 16.1, 16.1, 16.1; 64 of 6,000 (64 channels) 71, 59, 58, 57.
 KV4_GROUPS_PER_UNIT = 2
 # Rows are not cut, and nothing is joined, up to the first of these keys, or, of many (row, key/value head)s, up to so many keys for each of them, but to no more than the last.  Cut, and whole with 8
-# waves a workgroup (with 4): 1 row of 1,000 keys 10.4, 9.3 (10.5), of 1,500 9.9, 11.2 (13.5); 8 of 1,000 10.9, 10.8 (12.8); 16 of 2,000 16.8, 17.0 (22.5); 32 of 4,000 36.1, 30.9 (42.4);
-# 64 of 500 19.3, 16.0 (12.7), of 2,000 38.1, 32.8 (30.5).  Whole rows have 8 waves where there are no more of them than compute units.
+# waves a workgroup (with 4): 1 row of 1,000 keys 10.2, 8.9 (10.3), of 1,500 9.6, 11.0 (13.6); 8 of 1,000 11.2, 10.3 (12.4); 16 of 2,000 16.7, 16.5 (21.1); 32 of 4,000 35.8, 31.3 (43.2);
+# 64 of 500 18.1, 15.7 (12.1), of 2,000 36.1, 34.0 (30.7).  Whole rows have 8 waves where there are no more of them than compute units.
 KV4_WHOLE_KEYS = 1152, 16, 4096
 QKV_JOIN_MAX_RANGES = 4  # 17 to 128 rows: the kernel that joins the ranges of the q/k/v product, rotates and writes the cache reads
 #                          every range, so more of them cost it what they gain the product
