@@ -450,7 +450,7 @@ class Attention:
         """A stacked product that leaves q, k and v as they are and streams its matrix for few rows: with 4-bit pages the rotation and the write are a kernel of their own, also there.  None where ``wqkv`` is that; beside a
         copy for the kernel with both in its epilogue, whose rows lie in that kernel's order, one in the matrix' own order is made.  It belongs to the caches that are made for this layer: they share it, and it goes with the
         last of them."""
-        if not self.takes_int4_cache or self.wqkv_rope is None or self.wqkv.plain is None:
+        if not self.two_orders:
             return None
         product = self._int4_product() if self._int4_product is not None else None
         if product is None:
@@ -458,11 +458,16 @@ class Attention:
             self._int4_product = weakref.ref(product)
         return product
 
+    @property
+    def two_orders(self) -> bool:
+        """Whether a cache in 4 bits has a copy of the stacked matrix made (``serve_int4_cache``)."""
+        return self.takes_int4_cache and self.wqkv_rope is not None and self.wqkv.plain is not None
+
     def stream_one_order(self, product: "LinearWeight | None" = None) -> None:
-        """Where there is no room for two copies of the stacked matrix for few rows: the one in its own order alone (``product``, which ``serve_int4_cache`` gave, or a new one) in the place of the other, for every cache."""
-        if self.takes_int4_cache and self.wqkv_rope is not None and self.wqkv.plain is not None:
-            self.wqkv_rope = None
-            self.wqkv = product if product is not None else LinearWeight(self.wqkv.plain)
+        """Where there is no room for two copies of the stacked matrix for few rows (``two_orders``): the one in its own order alone (``product``, which ``serve_int4_cache`` gave, or a new one) in the place of the other, for
+        every cache."""
+        self.wqkv_rope = None
+        self.wqkv = product if product is not None else LinearWeight(self.wqkv.plain)
 
     def cache_need(self):
         s = self.spec

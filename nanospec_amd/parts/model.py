@@ -180,7 +180,7 @@ class DecoderModel:
     def stream_one_order(self, products: dict) -> bool:
         """For whoever has no room for what ``serve_int4_cache`` gives: the layers have one copy of their first matrix for few rows, which serves every cache.  Not once a runner has been made for the model: a step under way or
         captured may read the other."""
-        mixers = [] if self.has_runner else [one for layer in self.layers for part in getattr(layer, "parts", ()) for one in (part, *getattr(part, "sides", ())) if getattr(one, "wqkv_rope", None) is not None]
+        mixers = [] if self.has_runner else [one for layer in self.layers for part in getattr(layer, "parts", ()) for one in (part, *getattr(part, "sides", ())) if getattr(one, "two_orders", False)]
         if mixers:
             torch.cuda.synchronize(self.device)
             for one in mixers:

@@ -373,5 +373,25 @@ def test_a_cache_in_4_bits_where_memory_is_short(tmp_path_factory, monkeypatch, 
             # other kernels' roundings of q, k and v; a value between two codes may go the other way (0.03, as for captured steps; in bfloat16 8 units of the row's largest besides)
             assert float((a - b).abs().max() / b.abs().max()) <= 0.03 + LOGITS[torch.bfloat16]
     del rep, whole, made, a, b
-    model.has_runner = True
-    assert not model.stream_one_order({})
+    assert not other.stream_one_order({}) and all(layer.mixer.wqkv_rope is not None for layer in other.layers)  # (it has run)
+
+
+def test_a_model_with_one_copy_has_none_to_give(tmp_path_factory, monkeypatch, capsys):
+    """In the tiled layout layers run their own product over either cache: nothing is made for one in 4 bits, and where its pages do not fit nothing changes."""
+    from nanospec_amd import load_model
+    from nanospec_amd.cache.storage import CacheStorage
+
+    model = load_model(_wide(tmp_path_factory), layouts="tiled")
+    capsys.readouterr()
+    plain, calls = CacheStorage._allocate, []
+
+    def short(self, *args, **kw):
+        calls.append(self)
+        if len(calls) == 1:
+            raise torch.OutOfMemoryError("no room")
+        return plain(self, *args, **kw)
+
+    monkeypatch.setattr(CacheStorage, "_allocate", short)
+    storage = CacheStorage(model, [8], 16, 4, torch.bfloat16, "cuda", "int4")
+    assert len(calls) == 2 and not storage.products and storage.views[0].products is storage.products
+    assert all(layer.mixer.wqkv_rope is not None for layer in model.layers) and not capsys.readouterr().err
