@@ -1415,6 +1415,7 @@ def linear_int8(x: Int8Rows, w: Int8Weight, out: torch.Tensor | None = None, dty
 
 KV4_TOKENS = 8  # tokens that lie together in a record of a 4-bit page (csrc/kv4.h says how); a page is a power of two of tokens, from 8
 KV4_MAX_HEAD = 256
+KV4_ROW_KEYS = 1 << 27  # of a single token's row: its ranges are cut by quotients in float32, whose error stays below a 64th of a block of 32 keys up to here
 
 
 def kv4_takes(head_dim: int, page_size: int) -> bool:
@@ -1587,6 +1588,8 @@ def attention_kv4(q, out, pages: Kv4Pages, tiles, block_table, heads: int, kv_he
         raise KernelRefused(f"attention_kv4: tiles must be int32 [n_tiles, {TILE_INTS}]")
     if groups < 1 or pages.records >= 1 << 31:
         raise KernelRefused("attention_kv4: at least one workgroup, and fewer than 2^31 records in the pool")
+    if rows and block_table.shape[1] * pages.page > KV4_ROW_KEYS:
+        raise KernelRefused(f"attention_kv4: single tokens' tables have room for up to {KV4_ROW_KEYS} keys, not {block_table.shape[1] * pages.page}")
     form = form or (4 if rows else 16)
     if form not in ((4, 8) if rows else (16,) if q.dtype == torch.float32 else (16, 32)):
         raise KernelRefused("attention_kv4: a workgroup has 4 or 8 waves for single tokens; a wave takes 16 tokens of a portion, of bfloat16 also 32")

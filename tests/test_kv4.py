@@ -190,3 +190,26 @@ def test_ranges_of_portions_keep_within_their_memory():
     assert all(tiles * 32 * 32 * 128 * 4 * att.kv4_portion_ranges(tiles, 32, 131_072, 32, units) <= 128 << 20 for tiles in (17, 33))
     # as measured
     assert [att.kv4_portion_ranges(t, 32, n, 32, units) for t, n in ((22, 20333), (16, 8512), (64, 2048))] == [8, 4, 1]
+
+
+def test_rows_of_more_keys_than_their_ranges_are_cut_for_are_refused(monkeypatch):
+    monkeypatch.setattr(ops, "_gpu", lambda *tensors: None)
+    args = dict(q=torch.zeros(1, 256), out=torch.zeros(1, 256), pages=ops.Kv4Pages.empty(2, 2, 8, 64, "cpu"), tiles=torch.zeros((1, 8), dtype=torch.int32),
+                block_table=torch.zeros((1, ops.KV4_ROW_KEYS // 8 + 1), dtype=torch.int32), heads=4, kv_heads=2, head_dim=64, scale=1.0)
+    with pytest.raises(ops.KernelRefused, match="room for up to 134217728 keys"):
+        ops.attention_kv4(**args, rows=True)
+
+
+def test_ranges_by_reciprocals_hold_every_block():
+    """The share of a row's blocks that the kernel for single tokens computes, in float32 with a reciprocal that is off by a unit of its last place either way: as many ranges of it hold all blocks, up to the most keys."""
+    import numpy as np
+
+    most = ops.KV4_ROW_KEYS // 32
+    blocks = np.unique(np.concatenate([np.arange(1, 5000), most - np.arange(5000), np.random.RandomState(1).randint(1, most, 20000)]))
+    for ranges in range(1, 65):
+        blocks_r = np.unique(np.concatenate([blocks, blocks // ranges * ranges, np.minimum(blocks // ranges * ranges + 1, most)]))
+        blocks_r = blocks_r[blocks_r > 0]
+        exact = np.float32(1) / np.float32(ranges)
+        for inverse in (np.nextafter(exact, np.float32(0)), exact, np.nextafter(exact, np.float32(2))):
+            share = (blocks_r.astype(np.float32) * inverse).astype(np.int64) + 1
+            assert (share * ranges >= blocks_r).all()
